@@ -338,7 +338,8 @@ def _run_append(state):
         pool = state[name + "_pool"]
         pool.view(-1, *pool.shape[2:])[slots] = state[name][kept]
     index = state["index"][kept].float()
-    scales = index.abs().amax(-1).clamp(min=1e-4) / 448.0
+    amax = index.abs().amax(-1).clamp(min=1e-4)
+    scales = amax / torch.full_like(amax, 448.0)           # by a tensor: a division, not a product with 1/448
     state["index_pool"].view(torch.uint8).view(-1, 128)[slots] = (index / scales.unsqueeze(1)).to(torch.float8_e4m3fn).view(torch.uint8)
     state["index_scales"].view(-1)[slots] = scales
     return pools

@@ -28,6 +28,13 @@ MAX_PAIR_SOURCES = 16
 MAX_CTAS = 256
 STATIC_MAX_ROWS = 256
 STATUS_WAIT_EXPIRED = 1
+MAX_PLAN_REQUESTS = 16384
+ELEMENT_BF16 = 0
+ELEMENT_FP16 = 1
+SERVING_STATUS = {
+    1: "a bounded wait of the attention kernel expired", 2: "lengths that are negative, decrease or exceed their buffers",
+    4: "a page or slot outside its pool", 8: "a page plan ran out of pages", 16: "misaligned shared memory",
+}
 
 EXPORTED_SYMBOLS = (
     "itk_version", "itk_last_error", "itk_init", "itk_resource_report", "itk_workspace_bytes",
@@ -36,6 +43,7 @@ EXPORTED_SYMBOLS = (
     "itk_merge_candidate_lists", "itk_fused_topk_static", "itk_quantize_rows_e4m3",
     "itk_gather_sampled_kv_paged", "itk_repair_produce_paged", "itk_merge_shard_lists",
     "itk_compact_flagged_rows", "itk_repair_merge_chunk", "itk_flagged_scope_begin", "itk_flagged_scope_end",
+    "itk_serving_status", "itk_plan_pages", "itk_append_tokens", "itk_attention", "itk_attention_workspace_bytes",
 )
 
 
@@ -66,6 +74,50 @@ class FusedArgs(ctypes.Structure):
         ("tile_table", c_void_p), ("physical_keys", c_int),
         ("sampled_kv", c_void_p), ("sampled_scales", c_void_p), ("sample_ids", c_void_p), ("thresholds_out", c_void_p),
         ("samples", c_int), ("sample_rank", c_int), ("target_candidates", c_int),
+    ]
+
+
+class PagePlanArgs(ctypes.Structure):
+    _fields_ = [
+        ("table", c_void_p), ("old", c_void_p), ("fresh", c_void_p), ("free_pages", c_void_p),
+        ("slots", c_void_p), ("cu_q", c_void_p), ("lengths", c_void_p), ("flat", c_void_p),
+        ("k_start", c_void_p), ("k_end", c_void_p), ("pages_needed", c_void_p), ("table_stride", c_longlong),
+        ("requests", c_int), ("table_pages", c_int), ("page_size", c_int), ("free_count", c_int), ("rows", c_int),
+    ]
+
+
+class AppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("slots", c_void_p), ("k", c_void_p), ("v", c_void_p), ("k_pool", c_void_p), ("v_pool", c_void_p),
+        ("index_source", c_void_p), ("index_pool", c_void_p), ("index_scales", c_void_p),
+        ("k_token_stride", c_longlong), ("k_head_stride", c_longlong),
+        ("v_token_stride", c_longlong), ("v_head_stride", c_longlong),
+        ("k_page_stride", c_longlong), ("k_row_stride", c_longlong), ("k_pool_head_stride", c_longlong),
+        ("v_page_stride", c_longlong), ("v_row_stride", c_longlong), ("v_pool_head_stride", c_longlong),
+        ("index_stride", c_longlong),
+        ("index_dtype", c_int), ("tokens", c_int), ("kv_heads", c_int), ("dim", c_int), ("pages", c_int),
+        ("page_size", c_int),
+    ]
+
+
+class KvSegment(ctypes.Structure):
+    _fields_ = [
+        ("k", c_void_p), ("v", c_void_p), ("table", c_void_p), ("table_stride", c_longlong),
+        ("k_page_stride", c_longlong), ("k_row_stride", c_longlong), ("k_head_stride", c_longlong),
+        ("v_page_stride", c_longlong), ("v_row_stride", c_longlong), ("v_head_stride", c_longlong),
+        ("pages", c_int), ("page_size", c_int), ("table_pages", c_int),
+    ]
+
+
+class AttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", c_void_p), ("out", c_void_p), ("lse", c_void_p), ("cu_q", c_void_p), ("cu_k", c_void_p),
+        ("lens_k", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+        ("q_token_stride", c_longlong), ("q_head_stride", c_longlong),
+        ("out_token_stride", c_longlong), ("out_head_stride", c_longlong), ("wait_limit_ns", ctypes.c_ulonglong),
+        ("own", KvSegment), ("prefix", KvSegment), ("scale", ctypes.c_float), ("element", c_int),
+        ("tokens", c_int), ("heads", c_int), ("kv_heads", c_int), ("dim", c_int), ("requests", c_int),
+        ("prefix_keys", c_int), ("causal", c_int), ("clear_tail", c_int),
     ]
 
 
@@ -116,6 +168,11 @@ def load_library() -> ctypes.CDLL:
     library.itk_gather_sampled_kv_paged.argtypes = [c_void_p] * 6 + [c_int, c_int, c_int, c_void_p]
     library.itk_repair_produce_paged.argtypes = [c_void_p] * 8 + [c_int] * 7 + [c_void_p, c_int, c_void_p, c_void_p]
     library.itk_quantize_rows_e4m3.argtypes = [c_void_p, c_int] + [c_void_p] * 4 + [c_longlong, c_void_p]
+    library.itk_serving_status.argtypes = [POINTER(c_int), c_int]
+    library.itk_plan_pages.argtypes = [POINTER(PagePlanArgs), c_void_p]
+    library.itk_append_tokens.argtypes = [POINTER(AppendArgs), c_void_p]
+    library.itk_attention.argtypes = [POINTER(AttentionArgs), c_void_p]
+    library.itk_attention_workspace_bytes.argtypes = [POINTER(AttentionArgs), POINTER(c_size_t)]
     for name in EXPORTED_SYMBOLS:
         function = getattr(library, name)
         if name not in ("itk_version", "itk_last_error"):
@@ -163,6 +220,21 @@ def workspace_sizes(rows: int, keys: int, shards: int = 1) -> WorkspaceSizes:
     return sizes
 
 
+def check_serving_status(device: Any = None) -> None:
+    """Raise when a page plan, an append or an attention call on ``device`` met something it had to clamp, skip or give up.
+
+    Synchronises the device and clears what it reports.  One word per device: it does not say which call it was.
+    """
+
+    import torch
+
+    status = c_int(0)
+    with torch.cuda.device(device):
+        check(load_library().itk_serving_status(ctypes.byref(status), 1))
+    if status.value:
+        raise ItkError("serving status: " + "; ".join(text for bit, text in SERVING_STATUS.items() if status.value & bit))
+
+
 def pointer_table(tensors: list[Any]) -> Any:
     table = (c_void_p * len(tensors))()
     for index, tensor in enumerate(tensors):
@@ -171,8 +243,9 @@ def pointer_table(tensors: list[Any]) -> Any:
 
 
 __all__ = [
-    "BLOCK_Q", "EXPORTED_SYMBOLS", "FusedArgs", "HEADS", "HEAD_DIM", "ItkError", "LIBRARY_PATH", "MAX_KEYS",
-    "MAX_PAIR_SOURCES", "REPAIR_CHUNK", "SPILL_U64_PER_ROW", "STATUS_WAIT_EXPIRED", "TOP_K", "WorkspaceSizes",
-    "check", "current_stream", "load_library", "pointer_table", "ptr", "resource_report", "version",
+    "AppendArgs", "AttentionArgs", "BLOCK_Q", "ELEMENT_BF16", "ELEMENT_FP16", "EXPORTED_SYMBOLS", "FusedArgs", "HEADS",
+    "HEAD_DIM", "ItkError", "KvSegment", "LIBRARY_PATH", "MAX_KEYS", "MAX_PAIR_SOURCES", "MAX_PLAN_REQUESTS", "PagePlanArgs",
+    "SERVING_STATUS", "REPAIR_CHUNK", "SPILL_U64_PER_ROW", "STATUS_WAIT_EXPIRED", "TOP_K", "WorkspaceSizes",
+    "check", "check_serving_status", "current_stream", "load_library", "pointer_table", "ptr", "resource_report", "version",
     "workspace_sizes", "c_int32", "c_uint64",
 ]

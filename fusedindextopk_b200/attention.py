@@ -1,0 +1,215 @@
+"""Attention of packed, paged and shared-prefix batches.
+
+The operator of this package picks keys for a sparse attention; next to it a
+serving step attends densely: to prompts that are shorter than the selection, in
+layers without an indexer, and to long prefixes that a batch has in common.  The
+layouts are those of ``batched`` and ``paged``: queries packed as ``[sum Q_b, Hq, D]``
+with int32 prefix sums, the queries of a request being its LAST ``Q_b`` tokens, keys
+and values packed as ``[sum N_b, H, D]`` or in pools of pages (``page_size`` a multiple
+of 128) behind a block table.  ``Hq`` is a multiple of ``H``; query head ``h`` reads key
+head ``h // (Hq // H)``.  The reference selects keys only and attends nowhere.
+
+* ``attention_varlen``: whole prompts, chunks at the end of a context, single tokens;
+* ``attention_paged``: the same with keys behind a block table;
+* ``shared_prefix_attention``, ``shared_prefix_attention_paged``: a prefix that the
+  whole batch shares, read once for all requests, in front of every request's own keys.
+
+All of them take bf16 or fp16 with head dimension 64 or 128, keep scores, softmax
+statistics and sums in fp32 and never read lengths back to the host, so a call can be
+captured into a CUDA graph and replayed with other lengths in the same buffers.  A row
+that sees no key gets zeros and a log-sum-exp of ``-inf``.  There is no backward pass:
+the framework serves.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Any
+
+from . import _lib
+from .operator import _require
+
+TILE_KEYS = 128
+check_status = _lib.check_serving_status
+
+
+def _rows_ok(tensor: Any) -> bool:
+    """Contiguous heads that start on 16-byte boundaries."""
+
+    *outer, inner = tensor.stride()
+    return inner == 1 and all(s % 8 == 0 for s in outer) and tensor.data_ptr() % 16 == 0
+
+
+def _check_kv(torch: Any, q: Any, k: Any, v: Any, what: str, rank: int) -> None:
+    _require(k.dim() == rank and k.shape == v.shape,
+             f"{what} keys and values must both have shape {'[N, H, D]' if rank == 3 else '[P, page_size, H, D]'}")
+    _require(k.dtype == q.dtype and v.dtype == q.dtype, f"{what} keys and values must have the type of q")
+    _require(k.device == q.device and v.device == q.device, f"{what} keys and values must live on the same device as q")
+    _require(k.shape[-1] == q.shape[-1], f"{what} keys must have the head dimension of q")
+    heads = k.shape[-2]
+    _require(heads > 0 and q.shape[1] % heads == 0 and q.shape[1] // heads <= 128,
+             f"the query heads must be a multiple of the {what} key heads, at most 128 times as many")
+    _require(k.numel() == 0 or (_rows_ok(k) and _rows_ok(v)),
+             f"{what} keys and values must be contiguous in their last dimension and 16-byte aligned in every row")
+
+
+def _packed_segment(k: Any, v: Any) -> Any:
+    rows = k.shape[0]
+    if rows == 0:
+        return _lib.KvSegment(None, None, None, 0, 0, 0, 0, 0, 0, 0, 1, 0, 0)
+    return _lib.KvSegment(k.data_ptr(), v.data_ptr(), None, 0, 0, k.stride(0), k.stride(1), 0, v.stride(0), v.stride(1), 1, rows, 0)
+
+
+def _paged_segment(k_pool: Any, v_pool: Any, table: Any, table_stride: int) -> Any:
+    return _lib.KvSegment(k_pool.data_ptr(), v_pool.data_ptr(), table.data_ptr(), table_stride, *k_pool.stride()[:3],
+                          *v_pool.stride()[:3], k_pool.shape[0], k_pool.shape[1], table.shape[-1])
+
+
+def _check_pool(k_pool: Any) -> None:
+    pages, page_size = k_pool.shape[:2]
+    _require(pages > 0 and page_size > 0 and page_size % TILE_KEYS == 0, "page_size must be a positive multiple of 128")
+    _require(pages * page_size < 1 << 31, "pages * page_size must stay below 2^31")
+
+
+def _check_ints(torch: Any, tensor: Any, name: str, device: Any, count: int | None) -> None:
+    _require(tensor.dtype == torch.int32 and tensor.dim() == 1 and tensor.is_contiguous(), f"{name} must be contiguous int32")
+    _require(count is None or tensor.shape[0] == count, f"{name} must have {count} entries")
+    _require(tensor.device == device, f"{name} must live on the same device as q")
+
+
+def _attend(torch: Any, q: Any, kv_heads: int, own: Any, prefix: Any, prefix_keys: int, cu_seqlens_q: Any, cu_seqlens_k: Any,
+            lengths: Any, causal: bool, scale: float | None, out: Any, return_lse: bool) -> Any:
+    tokens, heads, dim = q.shape
+    device = q.device
+    _check_ints(torch, cu_seqlens_q, "cu_seqlens_q", device, None)
+    requests = cu_seqlens_q.shape[0] - 1
+    _require(requests >= 1, "cu_seqlens_q must be [B+1] with B >= 1")
+    if cu_seqlens_k is not None:
+        _check_ints(torch, cu_seqlens_k, "cu_seqlens_k", device, requests + 1)
+    else:
+        _check_ints(torch, lengths, "seqlens_k", device, requests)
+    _require(tokens * heads < 1 << 31, "rows * heads must stay below 2^31")
+    clear_tail = out is None
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=device)
+    else:
+        _require(out.shape == q.shape and out.dtype == q.dtype and out.device == device and (out.numel() == 0 or _rows_ok(out)),
+                 "out must have the shape, type and device of q and 16-byte aligned rows")
+        _require(tokens < 2 or out.stride(0) >= dim and out.stride(1) >= dim or heads == 1 and out.stride(0) >= dim,
+                 "out must not overlap itself")
+    lse = torch.empty((tokens, heads), dtype=torch.float32, device=device) if return_lse else None
+    if tokens:
+        scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
+        _require(math.isfinite(scale), "scale must be finite")
+        args = _lib.AttentionArgs(
+            q.data_ptr(), out.data_ptr(), _lib.ptr(lse), cu_seqlens_q.data_ptr(), _lib.ptr(cu_seqlens_k), _lib.ptr(lengths),
+            None, 0, q.stride(0), q.stride(1), out.stride(0), out.stride(1), 0, own, prefix, scale,
+            _lib.ELEMENT_BF16 if q.dtype == torch.bfloat16 else _lib.ELEMENT_FP16, tokens, heads, kv_heads, dim, requests,
+            prefix_keys, int(causal), int(clear_tail))
+        library = _lib.load_library()
+        needed = ctypes.c_size_t(0)
+        _lib.check(library.itk_attention_workspace_bytes(ctypes.byref(args), ctypes.byref(needed)))
+        with torch.cuda.device(device):
+            # of the caching allocator, on the call's stream: two calls, streams or captured graphs never share it
+            workspace = torch.empty(needed.value, dtype=torch.uint8, device=device)
+            args.workspace, args.workspace_bytes = workspace.data_ptr(), needed.value
+            _lib.check(library.itk_attention(ctypes.byref(args), _lib.current_stream(torch, device)))
+    return (out, lse) if return_lse else out
+
+
+def _check_q(torch: Any, q: Any) -> None:
+    _require(q.is_cuda, "q must be a CUDA tensor (there is no CPU path)")
+    _require(q.dim() == 3, "q must have shape [T, Hq, D]")
+    _require(q.dtype in (torch.bfloat16, torch.float16), "q must be bfloat16 or float16")
+    _require(q.shape[2] in (64, 128), "the head dimension must be 64 or 128")
+    _require(q.numel() == 0 or _rows_ok(q), "q must be contiguous in its last dimension and 16-byte aligned in every row")
+
+
+def attention_varlen(q: Any, kv: tuple[Any, Any], cu_seqlens_q: Any, cu_seqlens_k: Any, *, causal: bool = True,
+                     scale: float | None = None, out: Any = None, return_lse: bool = False) -> Any:
+    """Attention of a packed batch; ``[T, Hq, D]`` like ``q``, with ``return_lse`` also fp32 ``[T, Hq]``.
+
+    ``q`` is ``[T, Hq, D]``, ``kv = (k, v)`` both ``[N, H, D]``; request ``b`` owns rows
+    ``cu_seqlens_q[b]:cu_seqlens_q[b+1]`` and keys ``cu_seqlens_k[b]:cu_seqlens_k[b+1]`` (int32 ``[B+1]`` each, lengths of
+    zero allowed).  With ``causal`` row i of its Q sees its first ``N - Q + i + 1`` keys, else all N.  ``scale`` defaults to
+    ``D ** -0.5``.  Rows behind the last request are zero (log-sum-exp ``-inf``), or left as they were in a given ``out``.
+    """
+
+    import torch
+
+    k, v = kv
+    _check_q(torch, q)
+    _check_kv(torch, q, k, v, "own", 3)
+    return _attend(torch, q, k.shape[1], _packed_segment(k, v), _lib.KvSegment(), 0, cu_seqlens_q, cu_seqlens_k, None, causal, scale,
+                   out, return_lse)
+
+
+def _own_pages(torch: Any, q: Any, pools: tuple[Any, Any], block_table: Any, cu_seqlens_q: Any) -> Any:
+    k_pool, v_pool = pools
+    _check_q(torch, q)
+    _check_kv(torch, q, k_pool, v_pool, "own", 4)
+    _check_pool(k_pool)
+    _require(block_table.dtype == torch.int32 and block_table.dim() == 2, "block_table must be int32 [B, table_pages]")
+    _require(block_table.shape[0] == cu_seqlens_q.shape[0] - 1, "block_table must have one row per request")
+    _require(block_table.shape[1] > 0, "block_table must have at least one column")
+    _require(block_table.device == q.device, "block_table must live on the same device as q")
+    _require(block_table.stride(1) == 1 or block_table.shape[1] == 1, "block_table rows must be contiguous")
+    return _paged_segment(k_pool, v_pool, block_table, block_table.stride(0))
+
+
+def attention_paged(q: Any, pools: tuple[Any, Any], block_table: Any, cu_seqlens_q: Any, seqlens_k: Any, *, causal: bool = True,
+                    scale: float | None = None, out: Any = None, return_lse: bool = False) -> Any:
+    """``attention_varlen`` with the keys in ``pools = (k_pool, v_pool)``, both ``[P, page_size, H, D]``.
+
+    Key j of request b lies on page ``block_table[b, j // page_size]`` (int32 ``[B, table_pages]``); ``seqlens_k`` int32 ``[B]``
+    counts the request's keys (``PagePlan.lengths``).  Page ids outside the pool are clamped and reported by
+    ``check_status``.
+    """
+
+    import torch
+
+    own = _own_pages(torch, q, pools, block_table, cu_seqlens_q)
+    return _attend(torch, q, pools[0].shape[2], own, _lib.KvSegment(), 0, cu_seqlens_q, None, seqlens_k, causal, scale, out, return_lse)
+
+
+def shared_prefix_attention(q: Any, prefix_kv: tuple[Any, Any], kv: tuple[Any, Any], cu_seqlens_q: Any, cu_seqlens_k: Any, *,
+                            scale: float | None = None, out: Any = None, return_lse: bool = False) -> Any:
+    """Causal attention of a packed batch whose requests all continue the same prefix.
+
+    ``prefix_kv`` ``[P, H, D]`` each: every row sees all P prefix keys, then its own keys as in ``attention_varlen``.  The
+    prefix is attended by the rows of all requests together, so its keys and values are read once for the batch.
+    """
+
+    import torch
+
+    k, v = kv
+    k_prefix, v_prefix = prefix_kv
+    _check_q(torch, q)
+    _check_kv(torch, q, k, v, "own", 3)
+    _check_kv(torch, q, k_prefix, v_prefix, "prefix", 3)
+    _require(k_prefix.shape[1] == k.shape[1], "prefix and own keys must have the same heads")
+    return _attend(torch, q, k.shape[1], _packed_segment(k, v), _packed_segment(k_prefix, v_prefix), k_prefix.shape[0],
+                   cu_seqlens_q, cu_seqlens_k, None, True, scale, out, return_lse)
+
+
+def shared_prefix_attention_paged(q: Any, pools: tuple[Any, Any], prefix_table: Any, prefix_keys: int, block_table: Any,
+                                  cu_seqlens_q: Any, seqlens_k: Any, *, scale: float | None = None, out: Any = None,
+                                  return_lse: bool = False) -> Any:
+    """``shared_prefix_attention`` with prefix and own keys in the same pools.
+
+    ``prefix_table`` int32 lists the pages of the ``prefix_keys`` prefix keys; ``block_table`` and ``seqlens_k`` describe every
+    request's own keys, which start on a page of their own.
+    """
+
+    import torch
+
+    own = _own_pages(torch, q, pools, block_table, cu_seqlens_q)
+    prefix_keys = int(prefix_keys)
+    _check_ints(torch, prefix_table, "prefix_table", q.device, None)
+    _require(0 <= prefix_keys <= prefix_table.shape[0] * pools[0].shape[1], "prefix_table does not cover the prefix keys")
+    prefix = _paged_segment(pools[0], pools[1], prefix_table, 0) if prefix_keys else _lib.KvSegment()
+    return _attend(torch, q, pools[0].shape[2], own, prefix, prefix_keys, cu_seqlens_q, None, seqlens_k, True, scale, out, return_lse)
+
+
+__all__ = ["attention_paged", "attention_varlen", "check_status", "shared_prefix_attention", "shared_prefix_attention_paged"]

@@ -1,7 +1,7 @@
 """Build ``libitk_b200.so`` in-tree with nvcc for sm_100a.
 
-``python -m fusedindextopk_b200.build`` compiles ``csrc/itk_api.cu`` (which
-includes the kernel headers) into ``fusedindextopk_b200/libitk_b200.so``.  The
+``python -m fusedindextopk_b200.build`` compiles ``csrc/*.cu`` (which include
+the kernel headers) into ``fusedindextopk_b200/libitk_b200.so``.  The
 build is ahead-of-time: nvcc cross-compiles without a GPU, and the resulting
 library needs only the CUDA runtime and driver on the target machine.
 """
@@ -23,7 +23,7 @@ STAMP = PACKAGE_DIR / "libitk_b200.so.srchash"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
-    "-lineinfo", "-O3", "-std=c++17",
+    "-lineinfo", "-O3", "-std=c++17", "--threads", "2",
     "--shared", "-Xcompiler", "-fPIC",
     "-Xptxas", "-v",
 ]
@@ -58,7 +58,8 @@ def build(*, force: bool = False, verbose: bool = False) -> Path:
 
     if not force and is_current():
         return LIBRARY
-    command = [find_nvcc(), *NVCC_FLAGS, "-I", str(INCLUDE), "-o", str(LIBRARY), str(CSRC / "itk_api.cu")]
+    command = [find_nvcc(), *NVCC_FLAGS, "-I", str(INCLUDE), "-o", str(LIBRARY),
+               *(str(path) for path in sorted(CSRC.glob("*.cu")))]
     result = subprocess.run(command, capture_output=True, text=True)
     if verbose or result.returncode != 0:
         sys.stderr.write(result.stdout + result.stderr)

@@ -3,64 +3,18 @@
 // no JIT step and no dependency beyond the CUDA runtime and driver.
 #include "../../include/itk_b200.h"
 
-#include <cstdarg>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
 #include <string>
 
+#include "itk_host.cuh"
 #include "itk_quantize.cuh"
 #include "itk_select.cuh"
 
 namespace {
 
 using namespace itk;
-
-thread_local std::string g_last_error;
-
-int fail(int code, const char* format, ...) {
-    char buffer[512];
-    va_list args;
-    va_start(args, format);
-    vsnprintf(buffer, sizeof(buffer), format, args);
-    va_end(args);
-    g_last_error = buffer;
-    return code;
-}
-
-#define ITK_REQUIRE(condition, ...)                             \
-    do {                                                        \
-        if (!(condition)) return fail(ITK_ERR_ARGUMENT, __VA_ARGS__); \
-    } while (0)
-
-#define ITK_CUDA(call)                                                                        \
-    do {                                                                                      \
-        const cudaError_t status_ = (call);                                                   \
-        if (status_ != cudaSuccess)                                                           \
-            return fail(ITK_ERR_CUDA, "%s failed: %s", #call, cudaGetErrorString(status_));   \
-    } while (0)
-
-bool aligned16(const void* pointer) { return (reinterpret_cast<uintptr_t>(pointer) & 15u) == 0; }
-
-// ---------------------------------------------------------------- driver entry point
-
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiled encode_tiled_entry() {
-    static EncodeTiled entry = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void* symbol = nullptr;
-        cudaDriverEntryPointQueryResult query;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &symbol, cudaEnableDefault, &query) == cudaSuccess &&
-            query == cudaDriverEntryPointSuccess) {
-            entry = reinterpret_cast<EncodeTiled>(symbol);
-        }
-    });
-    return entry;
-}
 
 // [rows, 128] bytes, row-major, box of `box_rows` rows x 128 bytes, 128-byte swizzle.
 int make_row_map(CUtensorMap* map, const void* base, long long rows, int box_rows) {
@@ -171,7 +125,7 @@ extern "C" {
 
 const char* itk_version(void) { return "fusedindextopk_b200 0.1.0 (sm_100a)"; }
 
-const char* itk_last_error(void) { return g_last_error.c_str(); }
+const char* itk_last_error(void) { return last_error().c_str(); }
 
 int itk_init(int device) {
     ITK_CUDA(cudaSetDevice(device));

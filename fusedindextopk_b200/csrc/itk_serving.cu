@@ -1,0 +1,203 @@
+// C-ABI entry points of the serving step around the operator: page plans, token appends and attention.
+#include "itk_host.cuh"
+
+#include <algorithm>
+#include <initializer_list>
+
+#include "itk_attention.cuh"
+#include "itk_pages.cuh"
+
+namespace {
+
+using namespace itk;
+
+// One status word per device context, part of the library image: every serving kernel reports into it, and no
+// caller has to carry a buffer for it.
+__device__ int g_serving_status;
+
+constexpr int kMaxDevices = 64;
+
+struct DeviceState {
+    bool ready = false;
+    int sm_count = 0;
+    int* status = nullptr;
+};
+std::mutex g_device_mutex;
+DeviceState g_devices[kMaxDevices];
+
+int current_device(DeviceState* state) {
+    int device = 0;
+    ITK_CUDA(cudaGetDevice(&device));
+    if (device < 0 || device >= kMaxDevices) return fail(ITK_ERR_UNSUPPORTED, "device index %d out of range", device);
+    std::lock_guard<std::mutex> lock(g_device_mutex);
+    DeviceState& d = g_devices[device];
+    if (!d.ready) {
+        int major = 0;
+        ITK_CUDA(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device));
+        if (major != 10) return fail(ITK_ERR_UNSUPPORTED, "device %d is not sm_100; this library is built for sm_100a only", device);
+        ITK_CUDA(cudaDeviceGetAttribute(&d.sm_count, cudaDevAttrMultiProcessorCount, device));
+        void* address = nullptr;
+        ITK_CUDA(cudaGetSymbolAddress(&address, g_serving_status));
+        d.status = static_cast<int*>(address);
+        ITK_CUDA(cudaFuncSetAttribute(itk_plan_pages_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (3 * ITK_MAX_PLAN_REQUESTS + 1) * static_cast<int>(sizeof(int))));
+        d.ready = true;
+    }
+    *state = d;
+    return ITK_OK;
+}
+
+int launched(const char* what) {
+    const cudaError_t status = cudaGetLastError();
+    if (status != cudaSuccess) return fail(ITK_ERR_CUDA, "%s launch failed: %s", what, cudaGetErrorString(status));
+    return ITK_OK;
+}
+
+bool strides_ok(std::initializer_list<long long> strides) {
+    for (const long long s : strides)
+        if (s < 0 || s % 8 != 0) return false;
+    return true;
+}
+
+// Rows of a pool are counted in 31 bits; addresses are formed in 64.
+bool pool_rows_ok(long long pages, long long page_size) { return pages > 0 && page_size > 0 && pages * page_size < (1ll << 31); }
+
+int check_segment(const itk_kv_segment& s, const char* what) {
+    ITK_REQUIRE(s.k && s.v, "%s: keys and values must not be null", what);
+    ITK_REQUIRE(aligned16(s.k) && aligned16(s.v), "%s: keys and values must be 16-byte aligned", what);
+    ITK_REQUIRE(strides_ok({s.k_page_stride, s.k_row_stride, s.k_head_stride, s.v_page_stride, s.v_row_stride, s.v_head_stride}),
+                "%s: strides must be multiples of 8 elements", what);
+    ITK_REQUIRE(pool_rows_ok(s.pages, s.page_size), "%s: need 0 < pages * page_size < 2^31", what);
+    if (s.table != nullptr) {
+        ITK_REQUIRE(s.page_size % 128 == 0, "%s: page_size must be a multiple of 128", what);
+        ITK_REQUIRE(s.table_pages >= 0 && s.table_stride >= 0, "%s: table sizes must not be negative", what);
+    } else {
+        ITK_REQUIRE(s.pages == 1, "%s: keys without a table are one page", what);
+    }
+    return ITK_OK;
+}
+
+int check_attention(const itk_attention_args& a) {
+    ITK_REQUIRE(a.tokens >= 0 && a.requests >= 0 && a.prefix_keys >= 0, "sizes must not be negative");
+    ITK_REQUIRE(a.heads > 0 && a.kv_heads > 0 && a.heads % a.kv_heads == 0 && a.heads / a.kv_heads <= 128,
+                "heads must be a multiple of kv_heads, at most 128 times as many");
+    ITK_REQUIRE(a.dim == 64 || a.dim == 128, "head dimension must be 64 or 128");
+    ITK_REQUIRE(a.element == ITK_ELEMENT_BF16 || a.element == ITK_ELEMENT_FP16, "element must be bf16 or fp16");
+    ITK_REQUIRE(static_cast<long long>(a.tokens) * a.heads < (1ll << 31), "tokens * heads must stay below 2^31");
+    return ITK_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int itk_serving_status(int* status, int clear) {
+    ITK_REQUIRE(status != nullptr, "status must not be null");
+    DeviceState device;
+    const int rc = current_device(&device);
+    if (rc != ITK_OK) return rc;
+    ITK_CUDA(cudaDeviceSynchronize());
+    ITK_CUDA(cudaMemcpy(status, device.status, sizeof(int), cudaMemcpyDeviceToHost));
+    if (clear) ITK_CUDA(cudaMemset(device.status, 0, sizeof(int)));
+    return ITK_OK;
+}
+
+int itk_plan_pages(const itk_page_plan_args* args, itk_stream_t stream) {
+    ITK_REQUIRE(args != nullptr, "args must not be null");
+    const itk_page_plan_args& a = *args;
+    ITK_REQUIRE(a.requests > 0 && a.requests <= ITK_MAX_PLAN_REQUESTS, "need 0 < requests <= %d", ITK_MAX_PLAN_REQUESTS);
+    ITK_REQUIRE(a.rows >= 0 && a.free_count >= 0, "sizes must not be negative");
+    ITK_REQUIRE(a.table_pages > 0 && a.page_size > 0 && a.table_stride >= a.table_pages &&
+                    static_cast<long long>(a.requests) * a.table_pages < (1ll << 31) / a.page_size,
+                "need 0 < requests * table_pages * page_size < 2^31 and a row stride of at least table_pages");
+    ITK_REQUIRE(a.table && a.old && a.fresh && a.cu_q && a.lengths && a.flat && a.pages_needed &&
+                    (a.free_pages || a.free_count == 0) && ((a.slots && a.k_start && a.k_end) || a.rows == 0),
+                "page plan pointers must not be null");
+    DeviceState device;
+    const int rc = current_device(&device);
+    if (rc != ITK_OK) return rc;
+    const long long work = std::max(static_cast<long long>(a.requests) * a.table_pages, static_cast<long long>(a.rows));
+    const int grid = static_cast<int>(std::min<long long>(2 * device.sm_count, (work + 2 * kPlanThreads - 1) / (2 * kPlanThreads)));
+    const size_t smem = (3 * static_cast<size_t>(a.requests) + 1) * sizeof(int);
+    itk_plan_pages_kernel<<<grid, kPlanThreads, smem, stream>>>(a, device.status);
+    return launched("itk_plan_pages_kernel");
+}
+
+int itk_append_tokens(const itk_append_args* args, itk_stream_t stream) {
+    ITK_REQUIRE(args != nullptr, "args must not be null");
+    const itk_append_args& a = *args;
+    ITK_REQUIRE(a.tokens >= 0 && a.kv_heads > 0, "need tokens >= 0 and kv_heads > 0");
+    ITK_REQUIRE(a.dim == 64 || a.dim == 128, "head dimension must be 64 or 128");
+    ITK_REQUIRE(pool_rows_ok(a.pages, a.page_size), "need 0 < pages * page_size < 2^31");
+    if (a.tokens == 0) return ITK_OK;
+    ITK_REQUIRE(a.slots && a.k && a.v && a.k_pool && a.v_pool, "append pointers must not be null");
+    ITK_REQUIRE(aligned16(a.k) && aligned16(a.v) && aligned16(a.k_pool) && aligned16(a.v_pool),
+                "keys, values and their pools must be 16-byte aligned");
+    ITK_REQUIRE(strides_ok({a.k_token_stride, a.k_head_stride, a.v_token_stride, a.v_head_stride, a.k_page_stride, a.k_row_stride,
+                            a.k_pool_head_stride, a.v_page_stride, a.v_row_stride, a.v_pool_head_stride}),
+                "strides must be multiples of 8 elements");
+    if (a.index_source != nullptr) {
+        ITK_REQUIRE(a.index_pool && a.index_scales, "index keys need an index pool and its scales");
+        ITK_REQUIRE(a.index_dtype == ITK_SOURCE_F32 || a.index_dtype == ITK_SOURCE_BF16,
+                    "index_dtype must be ITK_SOURCE_F32 or ITK_SOURCE_BF16");
+        ITK_REQUIRE(aligned16(a.index_source) && aligned16(a.index_pool) && a.index_stride >= 0 && a.index_stride % 8 == 0,
+                    "index keys and their pool must be 16-byte aligned");
+    }
+    DeviceState device;
+    const int rc = current_device(&device);
+    if (rc != ITK_OK) return rc;
+    constexpr int kTokensPerBlock = kAppendThreads / 32;
+    const unsigned grid = static_cast<unsigned>((a.tokens + kTokensPerBlock - 1) / kTokensPerBlock);
+    if (a.index_source != nullptr && a.index_dtype == ITK_SOURCE_BF16)
+        itk_append_tokens_kernel<__nv_bfloat16><<<grid, kAppendThreads, 0, stream>>>(a, device.status);
+    else
+        itk_append_tokens_kernel<float><<<grid, kAppendThreads, 0, stream>>>(a, device.status);
+    return launched("itk_append_tokens_kernel");
+}
+
+int itk_attention_workspace_bytes(const itk_attention_args* args, size_t* bytes) {
+    ITK_REQUIRE(args != nullptr && bytes != nullptr, "args and bytes must not be null");
+    const int rc = check_attention(*args);
+    if (rc != ITK_OK) return rc;
+    *bytes = 0;
+    return ITK_OK;
+}
+
+int itk_attention(const itk_attention_args* args, itk_stream_t stream) {
+    ITK_REQUIRE(args != nullptr, "args must not be null");
+    const itk_attention_args& a = *args;
+    int rc = check_attention(a);
+    if (rc != ITK_OK) return rc;
+    if (a.tokens == 0) return ITK_OK;
+    ITK_REQUIRE(a.requests > 0, "need at least one request");
+    ITK_REQUIRE(a.q && a.out && a.cu_q, "q, out and cu_q must not be null");
+    ITK_REQUIRE((a.cu_k != nullptr) != (a.lens_k != nullptr), "own keys need either cu_k (packed) or lens_k (paged)");
+    ITK_REQUIRE((a.lens_k != nullptr) == (a.own.table != nullptr), "paged own keys need a block table, packed ones have none");
+    ITK_REQUIRE(aligned16(a.q) && aligned16(a.out), "q and out must be 16-byte aligned");
+    ITK_REQUIRE(strides_ok({a.q_token_stride, a.q_head_stride, a.out_token_stride, a.out_head_stride}),
+                "strides must be multiples of 8 elements");
+    // packed batches may have no own key at all (every key is in the prefix): then there is nothing to point at
+    if (a.own.k == nullptr)
+        ITK_REQUIRE(a.cu_k != nullptr && a.own.page_size == 0, "own keys: keys and values must not be null");
+    else if ((rc = check_segment(a.own, "own keys")) != ITK_OK)
+        return rc;
+    if (a.prefix.k != nullptr) {
+        if ((rc = check_segment(a.prefix, "prefix keys")) != ITK_OK) return rc;
+        const long long room = a.prefix.table != nullptr ? static_cast<long long>(a.prefix.table_pages) * a.prefix.page_size : a.prefix.page_size;
+        ITK_REQUIRE(a.prefix_keys <= room, "prefix_keys exceeds the prefix");
+    }
+    DeviceState device;
+    if ((rc = current_device(&device)) != ITK_OK) return rc;
+    const long long rows = static_cast<long long>(a.tokens) * a.heads;
+    const unsigned grid = static_cast<unsigned>((rows + 3) / 4);
+    if (a.element == ITK_ELEMENT_BF16) {
+        if (a.dim == 128) itk_attention_rows_kernel<__nv_bfloat16, 128><<<grid, kRowsKernelThreads, 0, stream>>>(a, device.status);
+        else itk_attention_rows_kernel<__nv_bfloat16, 64><<<grid, kRowsKernelThreads, 0, stream>>>(a, device.status);
+    } else {
+        if (a.dim == 128) itk_attention_rows_kernel<__half, 128><<<grid, kRowsKernelThreads, 0, stream>>>(a, device.status);
+        else itk_attention_rows_kernel<__half, 64><<<grid, kRowsKernelThreads, 0, stream>>>(a, device.status);
+    }
+    return launched("itk_attention_rows_kernel");
+}
+
+}  // extern "C"

@@ -13,10 +13,18 @@ tile's row offset (``tile_table[t] * 128``), and everything a caller sees (ids,
 Together with ``batched.varlen_ranges`` one block table serves a whole batch: the
 logical key space is the concatenation of the sequences, each starting on a page
 boundary.
+
+The bookkeeping of such a cache runs on the device as well, without a host read:
+``plan_pages`` turns request lengths and a list of free pages into block tables,
+slots, the flat block table and the key ranges that ``fused_index_topk_paged``
+takes; ``append_tokens`` writes a step's keys, values and (quantised) index keys
+to those slots; ``attention.attention_paged`` reads them.
 """
 
 from __future__ import annotations
 
+import ctypes
+from dataclasses import dataclass
 from typing import Any
 
 from . import _lib
@@ -162,4 +170,155 @@ def fused_index_topk_paged(q: Any, kv_pool_pair: tuple[Any, Any], block_table: A
                          key_extra=(int(block_table.data_ptr()),))
 
 
-__all__ = ["block_table_was_valid", "expand_block_table", "fused_index_topk_paged", "scatter_to_pages"]
+@dataclass
+class PagePlan:
+    """Buffers of one step's page plan (``make_page_plan``); ``plan_pages`` fills them in place.
+
+    ``block_table``  the caller's int32 ``[B, table_pages]`` table, updated in place, -1 behind a request's pages
+    ``slots``        int64 ``[rows]`` position of every new token in the pools (page * page_size + offset), -1 = padding
+    ``cu_seqlens_q`` int32 ``[B+1]`` prefix sums of the new tokens
+    ``lengths``      int32 ``[B]`` keys of every request after the step
+    ``flat_table``   int32 ``[B * table_pages]`` the requests' pages one after another, 0 behind them
+    ``k_start, k_end`` int32 ``[rows]`` causal key range of every new token in the key space of ``flat_table``
+    ``pages_needed`` int32 ``[1]`` pages taken from the free list
+    """
+
+    requests: int
+    table_pages: int
+    rows: int
+    page_size: int
+    slots: Any
+    cu_seqlens_q: Any
+    lengths: Any
+    flat_table: Any
+    k_start: Any
+    k_end: Any
+    pages_needed: Any
+    block_table: Any = None
+
+
+def make_page_plan(requests: int, table_pages: int, rows: int, *, page_size: int, device: Any) -> PagePlan:
+    """Buffers for the page plans of steps with ``requests`` requests and at most ``rows`` new tokens.
+
+    ``table_pages`` is the width of the block table.  ``page_size`` must be a multiple of 128.
+    """
+
+    import torch
+
+    _require(0 < requests <= _lib.MAX_PLAN_REQUESTS, f"need 0 < requests <= {_lib.MAX_PLAN_REQUESTS}")
+    _require(table_pages > 0 and rows >= 0, "need table_pages > 0 and rows >= 0")
+    _require(page_size >= TILE_KEYS and page_size % TILE_KEYS == 0, "page_size must be a positive multiple of 128")
+    _require(requests * table_pages * page_size < 1 << 31, "requests * table_pages * page_size must stay below 2^31")
+    device = torch.device(device)
+    _require(device.type == "cuda", "a page plan lives on a CUDA device (there is no CPU path)")
+
+    def buffer(count, dtype=torch.int32):
+        return torch.empty(count, dtype=dtype, device=device)
+
+    return PagePlan(requests, table_pages, rows, page_size, buffer(rows, torch.int64), buffer(requests + 1), buffer(requests),
+                    buffer(requests * table_pages), buffer(rows), buffer(rows), buffer(1))
+
+
+def plan_pages(plan: PagePlan, block_table: Any, lengths: Any, new_tokens: Any, free_pages: Any) -> PagePlan:
+    """Pages, slots and key ranges of one step, in one launch and without a host read.
+
+    Request ``b`` holds ``lengths[b]`` tokens (int32 ``[B]``) on the first ``ceil(lengths[b] / page_size)`` pages of its
+    row of ``block_table`` (int32 ``[B, table_pages]``) and gets ``new_tokens[b]`` more; the pages it lacks are taken from
+    ``free_pages`` (int32 ``[F]``) in request order, the first ``pages_needed[0]`` of them.  Everything lands in the
+    plan's buffers and in ``block_table`` itself; calling it again with the same arguments gives the same result.
+
+    A request that outgrows its table row, a free list that is too short and more new tokens than ``rows`` are reported
+    by ``check_serving_status``; their tokens get slot -1 (or no row), their cells -1, and nothing is written out of range.
+    """
+
+    import torch
+
+    rows, requests = plan.rows, plan.requests
+    device = plan.slots.device
+    for name, tensor, count in (("lengths", lengths, requests), ("new_tokens", new_tokens, requests),
+                                ("free_pages", free_pages, None)):
+        _require(tensor.dtype == torch.int32 and tensor.dim() == 1 and tensor.is_contiguous(), f"{name} must be contiguous int32")
+        _require(tensor.device == device, f"{name} must live on the plan's device")
+        _require(count is None or tensor.shape[0] == count, f"{name} must have one entry per request")
+    _require(block_table.dtype == torch.int32 and tuple(block_table.shape) == (requests, plan.table_pages),
+             "block_table must be int32 [requests, table_pages]")
+    _require(block_table.device == device, "block_table must live on the plan's device")
+    _require((block_table.stride(1) == 1 or plan.table_pages == 1) and (block_table.stride(0) >= plan.table_pages or requests == 1),
+             "block_table rows must be contiguous and must not overlap")
+    args = _lib.PagePlanArgs(
+        block_table.data_ptr(), lengths.data_ptr(), new_tokens.data_ptr(), free_pages.data_ptr(), plan.slots.data_ptr(),
+        plan.cu_seqlens_q.data_ptr(), plan.lengths.data_ptr(), plan.flat_table.data_ptr(), plan.k_start.data_ptr(),
+        plan.k_end.data_ptr(), plan.pages_needed.data_ptr(), max(block_table.stride(0), plan.table_pages), requests,
+        plan.table_pages, plan.page_size, free_pages.shape[0], rows)
+    with torch.cuda.device(device):
+        _lib.check(_lib.load_library().itk_plan_pages(ctypes.byref(args), _lib.current_stream(torch, device)))
+    plan.block_table = block_table
+    return plan
+
+
+def append_tokens(slots: Any, kv: tuple[Any, Any], pools: tuple[Any, Any], *, index_keys: Any = None,
+                  index_pools: tuple[Any, Any] | None = None) -> None:
+    """Write a step's tokens to their slots of the pools, in one launch.
+
+    ``slots`` int64 ``[T]`` (``PagePlan.slots``; tokens with a negative slot are skipped); ``kv = (k, v)`` bf16 or fp16
+    ``[T, H, D]`` (D 64 or 128, any token and head strides that are multiples of 8); ``pools = (k_pool, v_pool)`` of the same
+    type ``[P, page_size, H, D]``.  ``index_keys`` ``[T, 128]`` fp32 or bf16 are quantised like
+    ``quantize.quantize_contiguous_index_kv`` does into ``index_pools = (kv_pool e4m3 [P, page_size, 128], scale_pool fp32
+    [P, page_size])``, the pools ``fused_index_topk_paged`` reads.
+
+    Slots must differ from one another: of two tokens with the same slot either may be kept, in parts too.  A slot behind the
+    pool is skipped and reported by ``check_serving_status``.
+    """
+
+    import torch
+
+    k, v = kv
+    k_pool, v_pool = pools
+    _require(k.is_cuda, "k must be a CUDA tensor (there is no CPU path)")
+    device = k.device
+    _require(k.dim() == 3 and k.shape == v.shape, "k and v must both have shape [T, H, D]")
+    tokens, heads, dim = k.shape
+    _require(dim in (64, 128), "the head dimension must be 64 or 128")
+    _require(k.dtype in (torch.bfloat16, torch.float16), "k and v must be bfloat16 or float16")
+    _require(k_pool.dim() == 4 and k_pool.shape == v_pool.shape and tuple(k_pool.shape[2:]) == (heads, dim),
+             "the pools must both have shape [P, page_size, H, D]")
+    pages, page_size = k_pool.shape[0], k_pool.shape[1]
+    _require(0 < pages * page_size < 1 << 31, "need 0 < pages * page_size < 2^31")
+    _require(slots.dtype == torch.int64 and tuple(slots.shape) == (tokens,) and slots.is_contiguous(), "slots must be contiguous int64 [T]")
+    for name, tensor in (("k", k), ("v", v), ("k_pool", k_pool), ("v_pool", v_pool)):
+        _require(tensor.dtype == k.dtype, f"{name} must have the type of k")
+        _require(tensor.device == device, f"{name} must live on the same device as k")
+        _require(tensor.stride(-1) == 1 and all(s % 8 == 0 for s in tensor.stride()[:-1]) and tensor.data_ptr() % 16 == 0,
+                 f"{name} must be contiguous in its last dimension and 16-byte aligned in every row")
+    _require(slots.device == device, "slots must live on the same device as k")
+    index_source = index_pool = index_scales = None
+    index_stride = index_dtype = 0
+    if index_keys is not None:
+        _require(index_pools is not None, "index_keys need index_pools")
+        index_pool, index_scales = index_pools
+        index_source = index_keys
+        _require(index_keys.dtype in (torch.float32, torch.bfloat16) and tuple(index_keys.shape) == (tokens, _lib.HEAD_DIM),
+                 "index_keys must be float32 or bfloat16 [T, 128]")
+        _require((index_keys.stride(1) == 1) and index_keys.stride(0) % 8 == 0 and index_keys.data_ptr() % 16 == 0,
+                 "index_keys must be contiguous in the last dimension and 16-byte aligned in every row")
+        _require(index_pool.dtype == torch.float8_e4m3fn and tuple(index_pool.shape) == (pages, page_size, _lib.HEAD_DIM)
+                 and index_pool.is_contiguous(), "the index pool must be contiguous float8_e4m3fn [P, page_size, 128]")
+        _require(index_scales.dtype == torch.float32 and tuple(index_scales.shape) == (pages, page_size)
+                 and index_scales.is_contiguous(), "the index scales must be contiguous float32 [P, page_size]")
+        _require(index_keys.device == device and index_pool.device == device and index_scales.device == device,
+                 "index keys and pools must live on the same device as k")
+        index_stride, index_dtype = index_keys.stride(0), 1 if index_keys.dtype == torch.bfloat16 else 0
+    else:
+        _require(index_pools is None, "index_pools without index_keys")
+    args = _lib.AppendArgs(
+        slots.data_ptr(), k.data_ptr(), v.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), _lib.ptr(index_source),
+        _lib.ptr(index_pool), _lib.ptr(index_scales), *k.stride()[:2], *v.stride()[:2], *k_pool.stride()[:3],
+        *v_pool.stride()[:3], index_stride, index_dtype, tokens, heads, dim, pages, page_size)
+    with torch.cuda.device(device):
+        _lib.check(_lib.load_library().itk_append_tokens(ctypes.byref(args), _lib.current_stream(torch, device)))
+
+
+check_serving_status = _lib.check_serving_status
+
+__all__ = ["PagePlan", "append_tokens", "block_table_was_valid", "check_serving_status", "expand_block_table",
+           "fused_index_topk_paged", "make_page_plan", "plan_pages", "scatter_to_pages"]

@@ -338,6 +338,109 @@ int itk_quantize_rows_e4m3(const void* source, int source_dtype, const float* fo
 #define ITK_STATIC_MAX_ROWS 256
 int itk_fused_topk_static(const itk_fused_args* args, itk_stream_t stream);
 
+/* ------------------------------------------------------------------ serving step: pages, appends, attention
+ *
+ * The cache around the operator.  Keys and values (and the operator's index keys) live in pools of fixed-size
+ * pages; a step plans its pages, appends its tokens and attends.  No counterpart in the reference, which serves
+ * one contiguous sequence per call (src/fused_index_topk/inputs.py:31-32). */
+
+/* bits of the serving status word (one word per device context; the entries below only ever set bits) */
+#define ITK_SERVING_WAIT_EXPIRED 1     /* a bounded wait of the attention kernel ran out: its outputs are not valid */
+#define ITK_SERVING_BAD_LENGTHS 2      /* lengths that are negative, decrease or exceed their buffers; they were clamped */
+#define ITK_SERVING_BAD_PAGE 4         /* a page id or slot outside its pool; reads were clamped, writes skipped */
+#define ITK_SERVING_OUT_OF_PAGES 8     /* a page plan needed more pages than the free list or the block table holds */
+#define ITK_SERVING_BAD_SHARED_BASE 16 /* the shared-memory block is not 1 KB aligned; the kernel did nothing */
+
+/* Reads the current device's serving status word (synchronises the device); clears it when `clear` is set. */
+int itk_serving_status(int* status, int clear);
+
+/* Pages of one step.  For request b with old[b] tokens in the cache and fresh[b] new ones:
+ *   before = ceil(old / page_size), after = ceil((old + fresh) / page_size);
+ *   table[b, before:after] takes the next pages of free_pages in request order, table[b, after:] = -1;
+ *   cu_q = prefix sums of fresh [B+1], lengths = old + fresh;
+ *   row r of request b at position pos: slots[r] = table[b, pos / page_size] * page_size + pos % page_size;
+ *   flat = the used table entries of all requests one after another (0 behind them), and in that key space
+ *   k_start[r] = page_size * pages of the requests before b, k_end[r] = k_start[r] + pos + 1.
+ * Rows behind the last request: slot -1 and an empty range.  pages_needed[0] = pages taken from the free list. */
+typedef struct itk_page_plan_args {
+    int32_t* table;            /* int32 [requests, table_pages], row stride table_stride; updated in place */
+    const int32_t* old;        /* int32 [requests] */
+    const int32_t* fresh;      /* int32 [requests] */
+    const int32_t* free_pages; /* int32 [free_count] */
+    long long* slots;          /* int64 [rows] */
+    int32_t* cu_q;             /* int32 [requests + 1] */
+    int32_t* lengths;          /* int32 [requests] */
+    int32_t* flat;             /* int32 [requests * table_pages] */
+    int32_t* k_start;          /* int32 [rows] */
+    int32_t* k_end;            /* int32 [rows] */
+    int32_t* pages_needed;     /* int32 [1] */
+    long long table_stride;
+    int requests, table_pages, page_size, free_count, rows;
+} itk_page_plan_args;
+int itk_plan_pages(const itk_page_plan_args* args, itk_stream_t stream);
+
+#define ITK_MAX_PLAN_REQUESTS 16384
+#define ITK_ELEMENT_BF16 0
+#define ITK_ELEMENT_FP16 1
+
+/* pool[slots[t]] = token t for keys and values (16-bit elements, copied), and, when index_source is given, the
+ * e4m3 quantisation of token t's index key (the arithmetic of itk_quantize_rows_e4m3) with its scale.  Tokens with
+ * a negative slot are skipped.  Strides in elements; every row of a head starts on a 16-byte boundary. */
+typedef struct itk_append_args {
+    const long long* slots;    /* int64 [tokens] */
+    const void* k;             /* [tokens, kv_heads, dim] */
+    const void* v;
+    void* k_pool;              /* [pages, page_size, kv_heads, dim] */
+    void* v_pool;
+    const void* index_source;  /* [tokens, 128] fp32 or bf16, or null */
+    void* index_pool;          /* e4m3 [pages, page_size, 128], contiguous */
+    float* index_scales;       /* fp32 [pages, page_size], contiguous */
+    long long k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    long long k_page_stride, k_row_stride, k_pool_head_stride;
+    long long v_page_stride, v_row_stride, v_pool_head_stride;
+    long long index_stride;
+    int index_dtype;           /* ITK_SOURCE_F32 or ITK_SOURCE_BF16 */
+    int tokens, kv_heads, dim, pages, page_size;
+} itk_append_args;
+int itk_append_tokens(const itk_append_args* args, itk_stream_t stream);
+
+/* Keys and values of one segment: packed rows (table = null, one page of `page_size` rows) or a pool of pages
+ * read through a table.  Strides in elements. */
+typedef struct itk_kv_segment {
+    const void* k;
+    const void* v;
+    const int32_t* table;      /* int32 [requests, table_pages] (own keys) or [table_pages] (prefix), or null */
+    long long table_stride;
+    long long k_page_stride, k_row_stride, k_head_stride;
+    long long v_page_stride, v_row_stride, v_head_stride;
+    int pages, page_size, table_pages;
+} itk_kv_segment;
+
+/* out[t, h] = sum_j softmax_j(scale * q[t, h] . k_j) v_j over the prefix keys [0, prefix_keys) and the own keys of
+ * t's request; the request's rows are the LAST of its keys, and with `causal` row i of Q sees own keys
+ * j < N - Q + i + 1.  lse (optional) = natural logarithm of the sum of exponentials.  A row without a key gets
+ * out 0 and lse -inf.  Rows behind cu_q[requests] are left as they were, or zeroed with `clear_tail`. */
+typedef struct itk_attention_args {
+    const void* q;             /* [tokens, heads, dim] */
+    void* out;                 /* [tokens, heads, dim] */
+    float* lse;                /* [tokens, heads], contiguous, or null */
+    const int32_t* cu_q;       /* int32 [requests + 1] */
+    const int32_t* cu_k;       /* int32 [requests + 1]: packed own keys */
+    const int32_t* lens_k;     /* int32 [requests]: paged own keys */
+    void* workspace;
+    size_t workspace_bytes;
+    long long q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+    unsigned long long wait_limit_ns;   /* 0 = default */
+    itk_kv_segment own;
+    itk_kv_segment prefix;     /* k = null: no prefix */
+    float scale;
+    int element;               /* ITK_ELEMENT_* */
+    int tokens, heads, kv_heads, dim, requests, prefix_keys, causal, clear_tail;
+} itk_attention_args;
+int itk_attention(const itk_attention_args* args, itk_stream_t stream);
+/* Bytes of workspace a call with these sizes needs (the pointers are not looked at). */
+int itk_attention_workspace_bytes(const itk_attention_args* args, size_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,430 @@
+"""Attention over packed, paged and shared-prefix batches against the definition in 64 bits.
+
+Tolerance of an output, from the arithmetic (u = eps / 2 of the element type, e = 2^-24):
+* the weights may be rounded to the element type once: u * A with A = sum_j p_j |v_j|; fp16 weights (at most 1 after the row
+  maximum is taken off, so the sum is at least 1) may also lose 2^-25 each below the normal range: 2^-25 * sum_j |v_j|;
+* the output is rounded once: u * |out|;
+* a score is a sum of D products in fp32, scaled: ds = (D + 3) e * scale * max_j sum_i |q_i k_ji|, and the exponential of a
+  difference of two scores is off by 2 ds + 2^-20 relatively (the exponential itself is good to 2^-21);
+* sums over n keys add n e, joining partial results another 2^-20.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from fusedindextopk_b200 import _lib, attention
+from fusedindextopk_b200.build import build
+
+E = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def device():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    return torch.device("cuda:0")
+
+
+def sums(lengths, device):
+    return torch.tensor([0] + list(lengths), dtype=torch.int64).cumsum(0).to(torch.int32).to(device)
+
+
+def definition(q, keys, values, visible, scale):
+    """One request: rows [Q,Hq,D], keys [N,H,D]; row i sees the first visible[i] keys.  (out, lse, tol_out, tol_lse) in 64 bits."""
+
+    rows, heads, dim = q.shape
+    n, kv_heads = keys.shape[:2]
+    group = heads // kv_heads
+    u = torch.finfo(q.dtype).eps / 2
+    out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    lse = torch.full((rows, heads), -math.inf, dtype=torch.float64, device=q.device)
+    tol, tol_lse = torch.zeros_like(out), torch.zeros_like(lse)
+    if n == 0 or rows == 0:
+        return out, lse, tol, tol_lse
+    mask = torch.arange(n, device=q.device) >= visible.unsqueeze(1)
+    some = ~mask.all(dim=1)
+    for h in range(heads):
+        k, v = keys[:, h // group].double(), values[:, h // group].double()
+        x = q[:, h].double()
+        scores = ((x @ k.T) * scale).masked_fill(mask, -math.inf)
+        top = scores.amax(1, keepdim=True)
+        top = torch.where(top == -math.inf, torch.zeros_like(top), top)
+        weights = torch.exp(scores - top)
+        total = weights.sum(1, keepdim=True)
+        seen = (~mask).double()
+        o = torch.where(some.unsqueeze(1), (weights / total.clamp(min=1e-300)) @ v, torch.zeros((), dtype=torch.float64, device=q.device))
+        magnitude = torch.where(some.unsqueeze(1), (weights / total.clamp(min=1e-300)) @ v.abs(), torch.zeros_like(o))
+        ds = (dim + 3) * E * abs(scale) * ((x.abs() @ k.abs().T) * seen).amax(1, keepdim=True)
+        rel = 2 * ds + 2.0 ** -20 + n * E + 2.0 ** -20
+        extra = 2.0 ** -25 * (seen @ v.abs()) if q.dtype == torch.float16 else 0.0
+        tol[:, h] = (u + rel) * magnitude + u * o.abs() * 1.01 + extra + 1e-30
+        out[:, h] = o
+        lse[:, h] = torch.where(some, top.squeeze(1) + torch.log(total.squeeze(1)), torch.full_like(lse[:, h], -math.inf))
+        tol_lse[:, h] = ds.squeeze(1) + (2.0 ** -20 + n * E) + 4 * E * (lse[:, h].abs().nan_to_num(posinf=0.0) + top.squeeze(1).abs())
+    return out, lse, tol, tol_lse
+
+
+def expected(q, q_lens, requests, causal=True, scale=None):
+    """``requests``: (own keys [N,H,D], own values, prefix keys or None, prefix values) per request."""
+
+    scale = 1 / math.sqrt(q.shape[2]) if scale is None else scale
+    parts, row = [], 0
+    for count, (k, v, kp, vp) in zip(q_lens, requests):
+        prefix = 0
+        n = k.shape[0]
+        if kp is not None:
+            prefix = kp.shape[0]
+            k, v = torch.cat([kp, k]), torch.cat([vp, v])
+        own = n - count + 1 + torch.arange(count, device=q.device) if causal else torch.full((count,), n, device=q.device)
+        parts.append(definition(q[row:row + count], k, v, prefix + own.clamp(0, n), scale))
+        row += count
+    return tuple(torch.cat([p[i] for p in parts]) for i in range(4))
+
+
+def assert_close(got, lse, want):
+    out, want_lse, tol, tol_lse = want
+    off = (got[:out.shape[0]].double() - out).abs()
+    assert bool((off <= tol).all()), f"worst {float((off / tol).max()):.3f} of the tolerance at {int((off / tol).argmax())}"
+    if lse is not None:
+        lse = lse[:out.shape[0]].double()
+        assert torch.equal(lse == -math.inf, want_lse == -math.inf)
+        fine = want_lse > -math.inf
+        off = (lse - want_lse)[fine].abs()
+        assert bool((off <= tol_lse[fine]).all()), f"lse worst {float((off / tol_lse[fine]).max()):.3f} of the tolerance"
+
+
+def make(device, q_lens, k_lens, heads, kv_heads, dim, dtype, seed=0, spread=1.5):
+    g = torch.Generator(device=device).manual_seed(seed)
+    q = (torch.randn((sum(q_lens), heads, dim), generator=g, device=device) * spread).to(dtype)
+    k = torch.randn((sum(k_lens), kv_heads, dim), generator=g, device=device).to(dtype)
+    v = torch.randn((sum(k_lens), kv_heads, dim), generator=g, device=device).to(dtype)
+    return q, k, v
+
+
+def split(k, v, k_lens, kp=None, vp=None):
+    return [(a, b, kp, vp) for a, b in zip(k.split(k_lens), v.split(k_lens))]
+
+
+SHAPES = [
+    # q_lens, k_lens, heads, kv_heads, dim, dtype
+    ([1], [1], 1, 1, 128, torch.bfloat16),
+    ([1], [1], 8, 8, 64, torch.float16),
+    ([1], [129], 8, 1, 128, torch.bfloat16),
+    ([1], [8192], 32, 8, 128, torch.bfloat16),
+    ([1, 1, 1], [127, 128, 2000], 16, 2, 64, torch.bfloat16),
+    ([128], [128], 4, 4, 128, torch.bfloat16),
+    ([129, 0, 1, 300], [129, 0, 1, 300], 8, 2, 128, torch.float16),
+    ([257], [257], 2, 2, 64, torch.bfloat16),
+    ([100, 5, 64], [700, 5, 64], 12, 4, 128, torch.bfloat16),         # groups of 3
+    ([33, 70], [33, 1000], 10, 2, 64, torch.float16),                 # groups of 5
+    ([17, 1], [140, 555], 7, 1, 128, torch.bfloat16),                 # groups of 7
+    ([9, 2], [300, 77], 128, 1, 128, torch.bfloat16),                 # a group fills a tile
+    ([40], [400], 96, 1, 64, torch.bfloat16),                         # groups of 96: a tile holds one token
+    ([5, 3], [2, 0], 4, 2, 128, torch.bfloat16),                      # rows that see no key
+    ([600], [1300], 4, 1, 128, torch.float16),
+    ([1] * 40, list(range(1, 2400, 60)), 8, 2, 128, torch.bfloat16),
+    ([0, 0, 2], [5, 0, 500], 8, 8, 128, torch.bfloat16),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("q_lens,k_lens,heads,kv_heads,dim,dtype", SHAPES)
+def test_packed_batches_match_the_definition(device, q_lens, k_lens, heads, kv_heads, dim, dtype, causal):
+    q, k, v = make(device, q_lens, k_lens, heads, kv_heads, dim, dtype, seed=sum(k_lens))
+    got, lse = attention.attention_varlen(q, (k, v), sums(q_lens, device), sums(k_lens, device), causal=causal, return_lse=True)
+    attention.check_status(device)
+    assert_close(got, lse, expected(q, q_lens, split(k, v, k_lens), causal))
+
+
+def paged(k, v, k_lens, page_size, seed, layout="rows", fill=float("nan")):
+    """Scatter packed keys to random pages of pools full of NaN; returns (pools, table)."""
+
+    g = torch.Generator().manual_seed(seed)
+    need = [-(-n // page_size) for n in k_lens]
+    pages = sum(need) + 3
+    order = torch.randperm(pages, generator=g)
+    heads, dim = k.shape[1:]
+    table = torch.full((len(k_lens), max(max(need), 1)), -1, dtype=torch.int32)
+    pools = []
+    for x in (k, v):
+        pool = torch.full((pages, page_size, heads, dim), fill, dtype=k.dtype, device=k.device)
+        if layout == "heads":
+            pool = pool.transpose(1, 2).contiguous().transpose(1, 2)
+        at = 0
+        for b, part in enumerate(x.split(k_lens)):
+            for c in range(need[b]):
+                chunk = part[c * page_size:(c + 1) * page_size]
+                pool[int(order[at]), :chunk.shape[0]] = chunk
+                table[b, c] = order[at]
+                at += 1
+        pools.append(pool)
+    return tuple(pools), table.to(k.device)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page_size,layout", [(128, "rows"), (256, "heads"), (384, "rows")])
+@pytest.mark.parametrize("q_lens,k_lens,heads,kv_heads,dim,dtype", SHAPES[2:8:2] + SHAPES[8:17:3] + SHAPES[15:])
+def test_paged_batches_match_the_definition(device, q_lens, k_lens, heads, kv_heads, dim, dtype, page_size, layout):
+    q, k, v = make(device, q_lens, k_lens, heads, kv_heads, dim, dtype, seed=page_size)
+    pools, table = paged(k, v, k_lens, page_size, seed=sum(k_lens), layout=layout)
+    lens = torch.tensor(k_lens, dtype=torch.int32, device=device)
+    got, lse = attention.attention_paged(q, pools, table, sums(q_lens, device), lens, return_lse=True)
+    attention.check_status(device)
+    assert_close(got, lse, expected(q, q_lens, split(k, v, k_lens)))
+
+
+PREFIXES = [
+    # prefix, q_lens, k_lens, heads, kv_heads, dim, dtype
+    (1, [1], [1], 4, 2, 128, torch.bfloat16),
+    (300, [1, 1, 1], [5, 1, 140], 8, 2, 64, torch.float16),
+    (2048, [1, 2, 0, 3], [17, 128, 0, 300], 32, 8, 128, torch.bfloat16),
+    (129, [1] * 50, [3 + i for i in range(50)], 16, 2, 128, torch.bfloat16),
+    (1000, [70, 3, 130], [70, 40, 500], 6, 2, 128, torch.float16),
+    (5000, [1, 1], [0, 1], 8, 8, 64, torch.bfloat16),                 # a request without a key of its own
+    (0, [1, 9], [44, 9], 8, 2, 128, torch.bfloat16),                  # no prefix at all
+    (256, [4, 2], [2, 2], 16, 1, 128, torch.bfloat16),                # rows that see the prefix only
+    (4096, [3] * 30, [40 + 9 * i for i in range(30)], 28, 4, 128, torch.float16),   # groups of 7
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page_size", [0, 128, 256])
+@pytest.mark.parametrize("prefix,q_lens,k_lens,heads,kv_heads,dim,dtype", PREFIXES)
+def test_shared_prefixes_match_the_definition(device, prefix, q_lens, k_lens, heads, kv_heads, dim, dtype, page_size):
+    q, k, v = make(device, q_lens, [prefix] + k_lens, heads, kv_heads, dim, dtype, seed=prefix)
+    kp, vp, k_own, v_own = k[:prefix], v[:prefix], k[prefix:], v[prefix:]
+    if page_size == 0:
+        got, lse = attention.shared_prefix_attention(q, (kp, vp), (k_own, v_own), sums(q_lens, device), sums(k_lens, device),
+                                                     return_lse=True)
+    else:
+        pools, table = paged(k, v, [prefix] + k_lens, page_size, seed=prefix)
+        lens = torch.tensor(k_lens, dtype=torch.int32, device=device)
+        prefix_table = table[0, :-(-prefix // page_size)].contiguous()
+        got, lse = attention.shared_prefix_attention_paged(q, pools, prefix_table, prefix, table[1:], sums(q_lens, device), lens,
+                                                           return_lse=True)
+    attention.check_status(device)
+    assert_close(got, lse, expected(q, q_lens, split(k_own, v_own, k_lens, kp, vp)))
+
+
+@pytest.mark.gpu
+def test_slices_of_one_projection_and_a_strided_output(device):
+    q_lens, k_lens, heads, kv_heads, dim = [100, 30], [100, 30], 8, 2, 128
+    g = torch.Generator(device=device).manual_seed(3)
+    fused = torch.randn((130, heads + 2 * kv_heads, dim), generator=g, device=device).to(torch.bfloat16)
+    q, k, v = fused.split([heads, kv_heads, kv_heads], dim=1)
+    wide = torch.full((130, heads, 2 * dim), 7.0, dtype=torch.bfloat16, device=device)
+    out = wide[:, :, :dim]
+    got = attention.attention_varlen(q, (k, v), sums(q_lens, device), sums(k_lens, device), out=out, scale=0.3)
+    assert got is out
+    assert_close(out, None, expected(q, q_lens, split(k, v, k_lens), scale=0.3))
+    assert bool((wide[:, :, dim:] == 7.0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q_len,k_len", [(1, 70), (40, 200), (300, 300)])
+def test_rows_behind_the_last_request(device, q_len, k_len):
+    q, k, v = make(device, [q_len + 37], [k_len + 50], 8, 2, 128, torch.bfloat16)
+    k[k_len:], v[k_len:] = float("nan"), float("inf")
+    q[q_len:] = float("nan")
+    cu_q, cu_k = sums([q_len], device), sums([k_len], device)
+    want = expected(q[:q_len], [q_len], [(k[:k_len], v[:k_len], None, None)])
+    got, lse = attention.attention_varlen(q, (k, v), cu_q, cu_k, return_lse=True)
+    assert_close(got, lse, want)
+    assert bool((got[q_len:] == 0).all()) and bool((lse[q_len:] == -math.inf).all())
+    out = torch.full_like(q, 5.0)
+    attention.attention_varlen(q, (k, v), cu_q, cu_k, out=out)
+    assert_close(out, None, want)
+    assert bool((out[q_len:] == 5.0).all()), "rows behind the last request were written"
+    attention.check_status(device)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 128), (16, 2, 64)])
+def test_what_a_row_does_not_see_does_not_reach_it(device, bad, heads, kv_heads, dim):
+    """Keys and values behind a row's last visible key may hold anything; the rows that see them get it."""
+
+    n, at = 500, 317
+    q, k, v = make(device, [n], [n], heads, kv_heads, dim, torch.bfloat16, seed=1)
+    clean = expected(q, [n], [(k, v, None, None)])
+    k_bad, v_bad = k.clone(), v.clone()
+    v_bad[at, 0, 3] = bad
+    got, lse = attention.attention_varlen(q, (k, v_bad), sums([n], device), sums([n], device), return_lse=True)
+    group = heads // kv_heads
+    touched = torch.zeros_like(q, dtype=torch.bool)
+    touched[at:, :group, 3] = True
+    assert_close(torch.where(touched, clean[0].to(q.dtype), got), lse, clean)
+    assert not bool(got[touched].isfinite().any())
+    if not math.isnan(bad):
+        assert bool((got[touched] == bad).all())
+    k_bad[at, 0, 3] = float("nan")
+    got, lse = attention.attention_varlen(q, (k_bad, v), sums([n], device), sums([n], device), return_lse=True)
+    touched = torch.zeros((n, heads), dtype=torch.bool, device=device)
+    touched[at:, :group] = True
+    assert bool(lse[touched].isnan().all()) and bool(got[touched].isnan().all())
+    assert_close(torch.where(touched.unsqueeze(2), clean[0].to(q.dtype), got), torch.where(touched, clean[1].float(), lse), clean)
+
+
+@pytest.mark.gpu
+def test_scores_far_from_zero(device):
+    """Row maxima that keep growing along the keys, up to scores of several hundred."""
+
+    q, k, v = make(device, [64], [2000], 4, 2, 128, torch.bfloat16, seed=2)
+    ramp = torch.linspace(0.0, 3.0, 2000, device=device)[:, None, None]
+    q = q.abs()
+    k = (ramp * k.abs()).to(torch.bfloat16)
+    for sign in (1, -1):
+        got, lse = attention.attention_varlen(q, (sign * k, v), sums([64], device), sums([2000], device), return_lse=True)
+        assert_close(got, lse, expected(q, [64], [(sign * k, v, None, None)]))
+
+
+@pytest.mark.gpu
+def test_a_captured_call_follows_its_buffers(device):
+    """Two graphs of the same tensors, replayed with other lengths in place, next to an eager call on another stream."""
+
+    q, k, v = make(device, [300], [4000], 8, 2, 128, torch.bfloat16, seed=4)
+    cu_q, cu_k = sums([100, 200], device), sums([1000, 3000], device)
+    stream = torch.cuda.Stream(device)
+    stream.wait_stream(torch.cuda.current_stream(device))
+    with torch.cuda.stream(stream):
+        attention.attention_varlen(q, (k, v), cu_q, cu_k)
+    torch.cuda.current_stream(device).wait_stream(stream)
+    graphs = []
+    for causal in (True, False):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = attention.attention_varlen(q, (k, v), cu_q, cu_k, causal=causal, return_lse=True)
+        graphs.append((graph, held, causal))
+    for q_lens, k_lens in (([100, 200], [1000, 3000]), ([1, 250], [2500, 700]), ([0, 1], [0, 4000])):
+        cu_q.copy_(sums(q_lens, device))
+        cu_k.copy_(sums(k_lens, device))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            eager = attention.attention_varlen(q, (k, v), cu_q, cu_k, return_lse=True)
+        for graph, _, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        total_q, total_k = sum(q_lens), sum(k_lens)
+        parts = split(k[:total_k], v[:total_k], k_lens)
+        for _, held, causal in graphs:
+            assert_close(held[0], held[1], expected(q[:total_q], q_lens, parts, causal))
+        assert_close(eager[0], eager[1], expected(q[:total_q], q_lens, parts))
+    attention.check_status(device)
+
+
+@pytest.mark.gpu
+def test_calls_repeat_to_the_bit(device):
+    q_lens, k_lens = [1, 300, 2, 1], [5000, 300, 900, 1]
+    q, k, v = make(device, q_lens, k_lens, 16, 2, 128, torch.bfloat16, seed=5)
+    cu_q, cu_k = sums(q_lens, device), sums(k_lens, device)
+    first = attention.attention_varlen(q, (k, v), cu_q, cu_k, return_lse=True)
+    for _ in range(5):
+        again = attention.attention_varlen(q, (k, v), cu_q, cu_k, return_lse=True)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+@pytest.mark.gpu
+def test_bad_lengths_and_pages_are_clamped_and_reported(device):
+    q, k, v = make(device, [4], [300], 4, 2, 128, torch.bfloat16)
+    cu = torch.tensor([0, 9], dtype=torch.int32, device=device)             # more rows than q has
+    attention.attention_varlen(q, (k, v), cu, sums([300], device))
+    with pytest.raises(_lib.ItkError, match="lengths"):
+        attention.check_status(device)
+    attention.check_status(device)                                          # reported once
+    pools, table = paged(k, v, [300], 128, seed=1, fill=0.0)
+    lens = torch.tensor([300], dtype=torch.int32, device=device)
+    for page in (-1, 1000):
+        table[0, 1] = page
+        attention.attention_paged(q, pools, table, sums([4], device), lens)
+        with pytest.raises(_lib.ItkError, match="page"):
+            attention.check_status(device)
+    attention.attention_paged(q, pools, table[:, :1], sums([4], device), lens)   # 300 keys on one page of 128
+    with pytest.raises(_lib.ItkError, match="lengths"):
+        attention.check_status(device)
+
+
+@pytest.mark.gpu
+def test_refusals(device):
+    q, k, v = make(device, [4], [30], 4, 2, 128, torch.bfloat16)
+    cu_q, cu_k = sums([4], device), sums([30], device)
+
+    def refused(match, *args, call=attention.attention_varlen, **kwargs):
+        with pytest.raises(ValueError, match=match):
+            call(*args, **kwargs)
+
+    refused("CUDA", q.cpu(), (k, v), cu_q, cu_k)
+    refused("bfloat16 or float16", q.float(), (k, v), cu_q, cu_k)
+    refused("64 or 128", q[..., :96], (k[..., :96], v[..., :96]), cu_q, cu_k)
+    refused("type of q", q, (k.half(), v.half()), cu_q, cu_k)
+    refused("multiple of", q[:, :3], (k, v), cu_q, cu_k)
+    refused("shape", q, (k, v[:20]), cu_q, cu_k)
+    refused("int32", q, (k, v), cu_q.long(), cu_k)
+    refused("entries", q, (k, v), cu_q, sums([10, 20], device))
+    refused("B >= 1", q, (k, v), cu_q[:1], cu_k[:1])
+    refused("aligned", torch.empty(4, 4, 132, dtype=q.dtype, device=device)[..., 4:], (k, v), cu_q, cu_k)
+    refused("last dimension", q.transpose(1, 2).contiguous().transpose(1, 2), (k, v), cu_q, cu_k)
+    refused("out must", q, (k, v), cu_q, cu_k, out=torch.empty(4, 4, 64, dtype=q.dtype, device=device))
+    refused("overlap", q, (k, v), cu_q, cu_k, out=torch.empty(4, 4, 128, dtype=q.dtype, device=device)[:1].expand(4, 4, 128))
+    refused("finite", q, (k, v), cu_q, cu_k, scale=float("inf"))
+    pools, table = paged(k, v, [30], 128, seed=1)
+    lens = torch.tensor([30], dtype=torch.int32, device=device)
+    refused("multiple of 128", q, tuple(p[:, :64] for p in pools), table, cu_q, lens, call=attention.attention_paged)
+    refused("one row per request", q, pools, table.repeat(2, 1), cu_q, lens, call=attention.attention_paged)
+    refused("int32", q, pools, table.long(), cu_q, lens, call=attention.attention_paged)
+    refused("cover", q, pools, table[0], 129, table, cu_q, lens, call=attention.shared_prefix_attention_paged)
+    refused("same heads", q, (k[:, :1], v[:, :1]), (k, v), cu_q, cu_k, call=attention.shared_prefix_attention)
+    empty = attention.attention_varlen(q[:0], (k, v), sums([0], device), cu_k)
+    assert empty.shape == (0, 4, 128)
+
+
+def test_c_entry_refuses_before_any_launch():
+    build()
+    library = _lib.load_library()
+    args = _lib.AttentionArgs()
+    assert library.itk_attention(None, None) == -1
+    assert library.itk_attention(ctypes.byref(args), None) == -1
+    args.heads, args.kv_heads, args.dim, args.tokens = 8, 3, 128, 5
+    assert library.itk_attention(ctypes.byref(args), None) == -1
+    assert b"multiple of kv_heads" in library.itk_last_error()
+    args.kv_heads, args.dim = 2, 96
+    assert library.itk_attention(ctypes.byref(args), None) == -1
+    assert b"64 or 128" in library.itk_last_error()
+    args.dim = 128
+    assert library.itk_attention(ctypes.byref(args), None) == -1
+    assert b"at least one request" in library.itk_last_error()
+    args.requests = 1
+    assert library.itk_attention(ctypes.byref(args), None) == -1
+    assert b"must not be null" in library.itk_last_error()
+    args.q = args.out = args.cu_q = args.lens_k = 1 << 20
+    args.own.k = args.own.v = args.own.table = 1 << 20
+    args.own.pages, args.own.page_size = 4, 96
+    assert library.itk_attention(ctypes.byref(args), None) == -1
+    assert b"multiple of 128" in library.itk_last_error()
+    args.own.pages, args.own.page_size = 1 << 24, 128
+    assert library.itk_attention(ctypes.byref(args), None) == -1
+    assert b"2^31" in library.itk_last_error()
+    args.own.pages, args.own.k_row_stride = 4, 12
+    assert library.itk_attention(ctypes.byref(args), None) == -1
+    assert b"multiples of 8" in library.itk_last_error()
+    args.tokens = 0
+    args.own.k_row_stride = 16
+    assert library.itk_attention(ctypes.byref(args), None) == 0      # nothing to do
+
+
+def test_argument_structs_match_the_header():
+    import re
+    from pathlib import Path
+
+    text = (Path(__file__).resolve().parents[1] / "include" / "itk_b200.h").read_text()
+    for name, mirror in (("itk_attention_args", _lib.AttentionArgs), ("itk_kv_segment", _lib.KvSegment),
+                         ("itk_append_args", _lib.AppendArgs), ("itk_page_plan_args", _lib.PagePlanArgs)):
+        body = text[text.index(f"typedef struct {name} {{"):text.index(f"}} {name};")]
+        body = re.sub(r"/\*.*?\*/", "", body, flags=re.S).split("{", 1)[1]
+        fields = [re.sub(r"[\s*]", " ", f).split()[-1] for line in body.split(";") for f in line.split(",") if f.strip()]
+        assert fields == [field for field, _ in mirror._fields_]

@@ -1,0 +1,261 @@
+"""Page plans and token appends: block tables, slots and ranges against a plain loop, pools against torch."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from fusedindextopk_b200 import _lib, paged
+from fusedindextopk_b200.build import build
+
+
+@pytest.fixture(scope="module")
+def device():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    return torch.device("cuda:0")
+
+
+def plain_plan(table, old, new, free, page, rows):
+    """The definition, one token at a time."""
+
+    table = [list(r) for r in table]
+    columns = len(table[0])
+    slots, starts, ends, cu, lengths, flat, taken = [], [], [], [0], [], [], 0
+    for b, (o, n) in enumerate(zip(old, new)):
+        before, after = -(-o // page), -(-(o + n) // page)
+        for c in range(before, columns):
+            if c < after:
+                table[b][c] = free[taken]
+                taken += 1
+            else:
+                table[b][c] = -1
+        first = len(flat)
+        flat += table[b][:after]
+        for position in range(o, o + n):
+            slots.append(table[b][position // page] * page + position % page)
+            starts.append(first * page)
+            ends.append(first * page + position + 1)
+        cu.append(cu[-1] + n)
+        lengths.append(o + n)
+    padding = rows - len(slots)
+    flat += [0] * (len(table) * columns - len(flat))
+    return table, slots + [-1] * padding, cu, lengths, flat, starts + [0] * padding, ends + [0] * padding, taken
+
+
+def make(seed, requests, columns, page, new_max, spare=2):
+    g = torch.Generator().manual_seed(seed)
+    new = torch.randint(0, new_max + 1, (requests,), generator=g)
+    old = torch.randint(0, columns * page - new_max + 1, (requests,), generator=g)
+    old[torch.rand(requests, generator=g) < 0.3] = 0
+    before = -(-old // page)
+    need = int((-(-(old + new) // page) - before).sum())
+    order = torch.randperm(int(before.sum()) + need + spare, generator=g).tolist()
+    table = [[-7] * columns for _ in range(requests)]
+    for b in range(requests):
+        for c in range(int(before[b])):
+            table[b][c] = order.pop()
+    return table, old.tolist(), new.tolist(), order
+
+
+def gpu(values, device):
+    return torch.tensor(values, dtype=torch.int32, device=device)
+
+
+CASES = [(1, 1, 128, 1, 0), (1, 40, 128, 300, 5), (8, 16, 128, 1, 0), (7, 5, 256, 400, 100), (600, 9, 128, 200, 3),
+         (513, 3, 384, 2, 17), (3000, 4, 128, 1, 0)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("requests,columns,page,new_max,spare_rows", CASES)
+def test_page_plans_match_the_definition(device, requests, columns, page, new_max, spare_rows):
+    table, old, new, free = make(requests, requests, columns, page, new_max)
+    rows = sum(new) + spare_rows
+    want = plain_plan(table, old, new, free, page, rows)
+    plan = paged.make_page_plan(requests, columns, rows, page_size=page, device=device)
+    wide = torch.full((requests, columns + 3), 99, dtype=torch.int32, device=device)
+    block_table = wide[:, :columns]
+    block_table.copy_(gpu(table, device))
+    for _ in range(2):                                       # the same step twice gives the same plan
+        got = paged.plan_pages(plan, block_table, gpu(old, device), gpu(new, device), gpu(free, device))
+        assert got.block_table is block_table
+        assert block_table.tolist() == want[0]
+        assert got.slots.tolist() == want[1]
+        assert got.cu_seqlens_q.tolist() == want[2]
+        assert got.lengths.tolist() == want[3]
+        assert got.flat_table.tolist() == want[4]
+        assert got.k_start.tolist() == want[5]
+        assert got.k_end.tolist() == want[6]
+        assert got.pages_needed.tolist() == [want[7]]
+    assert bool((wide[:, columns:] == 99).all())
+    paged.check_serving_status(device)
+
+
+@pytest.mark.gpu
+def test_a_captured_plan_follows_its_lengths(device):
+    requests, columns, page, rows = 5, 6, 128, 40
+    plan = paged.make_page_plan(requests, columns, rows, page_size=page, device=device)
+    block_table = torch.full((requests, columns), -1, dtype=torch.int32, device=device)
+    old, new, free = gpu([0] * 5, device), gpu([0] * 5, device), gpu(list(range(30)), device)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        paged.plan_pages(plan, block_table, old, new, free)
+    held, used = [0] * requests, 0
+    for step in ([8, 0, 1, 30, 1], [1, 1, 1, 1, 1], [0, 0, 0, 0, 40], [7, 9, 0, 0, 0]):
+        table = block_table.tolist()
+        pool = list(range(used, 30))
+        want = plain_plan(table, held, step, pool, page, rows)
+        old.copy_(gpu(held, device))
+        new.copy_(gpu(step, device))
+        free[:len(pool)] = gpu(pool, device)
+        graph.replay()
+        assert block_table.tolist() == want[0] and plan.slots.tolist() == want[1] and plan.flat_table.tolist() == want[4]
+        held, used = want[3], used + want[7]
+    paged.check_serving_status(device)
+
+
+@pytest.mark.gpu
+def test_plans_that_do_not_fit_are_reported_and_stay_in_their_buffers(device):
+    page = 128
+    plan = paged.make_page_plan(2, 2, 300, page_size=page, device=device)
+    table = torch.full((2, 2), -1, dtype=torch.int32, device=device)
+    # three pages wanted, two there
+    got = paged.plan_pages(plan, table, gpu([0, 0], device), gpu([200, 100], device), gpu([4, 9], device))
+    assert table.tolist() == [[4, 9], [-1, -1]] and got.pages_needed.tolist() == [3]
+    assert got.slots[:200].tolist() == [4 * page + i for i in range(128)] + [9 * page + i for i in range(72)]
+    assert bool((got.slots[200:] == -1).all())
+    with pytest.raises(_lib.ItkError, match="out of pages"):
+        paged.check_serving_status(device)
+    # a request that outgrows its table row
+    got = paged.plan_pages(plan, table, gpu([200, 0], device), gpu([100, 0], device), gpu([5, 6], device))
+    assert got.lengths.tolist() == [256, 0] and bool((got.slots[56:] == -1).all()) and bool((got.slots[:56] >= 0).all())
+    with pytest.raises(_lib.ItkError, match="out of pages"):
+        paged.check_serving_status(device)
+    # more new tokens than rows, and a negative length
+    got = paged.plan_pages(plan, table, gpu([-5, 0], device), gpu([200, 200], device), gpu([1, 2, 3, 4], device))
+    assert got.cu_seqlens_q.tolist() == [0, 200, 300]
+    with pytest.raises(_lib.ItkError, match="lengths"):
+        paged.check_serving_status(device)
+    huge = 2 ** 31 - 1
+    paged.plan_pages(plan, table, gpu([huge, huge], device), gpu([huge, huge], device), gpu([1], device))
+    with pytest.raises(_lib.ItkError):
+        paged.check_serving_status(device)
+
+
+def plain_append(slots, k, v, pools, index=None, index_pools=None):
+    kept = slots >= 0
+    at = slots[kept]
+    for x, pool in ((k, pools[0]), (v, pools[1])):
+        flat = pool.reshape(-1, *pool.shape[2:]).clone()
+        flat[at] = x[kept]
+        pool.copy_(flat.view(pool.shape))
+    if index is not None:
+        x = index[kept].float()
+        amax = x.abs().amax(-1).clamp(min=1e-4)
+        scales = amax / torch.full_like(amax, 448.0)       # by a tensor: a true division, not a product with 1/448
+        index_pools[0].view(torch.uint8).view(-1, 128)[at] = (x / scales.unsqueeze(1)).to(torch.float8_e4m3fn).view(torch.uint8)
+        index_pools[1].view(-1)[at] = scales
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,heads,dim,page,layout,index_dtype", [
+    (1, 1, 64, 128, "rows", torch.bfloat16), (5, 3, 128, 128, "rows", None), (64, 8, 128, 256, "heads", torch.float32),
+    (1000, 2, 64, 100, "rows", torch.bfloat16), (333, 40, 128, 128, "heads", torch.bfloat16), (0, 2, 64, 128, "rows", None)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_appends_match_torch(device, tokens, heads, dim, page, layout, index_dtype, dtype):
+    g = torch.Generator(device=device).manual_seed(tokens)
+    pages = tokens // page + 3
+    fused = torch.randn((tokens, 3 * heads, dim), generator=g, device=device).to(dtype)
+    k, v = fused[:, :heads], fused[:, 2 * heads:]
+    pools = [torch.randn((pages, page, heads, dim), generator=g, device=device).to(dtype) for _ in range(2)]
+    if layout == "heads":
+        pools = [p.transpose(1, 2).contiguous().transpose(1, 2) for p in pools]
+    slots = torch.randperm(pages * page, generator=torch.Generator().manual_seed(tokens))[:tokens].to(device)
+    slots[::7] = -1
+    index = index_pools = want_index = None
+    if index_dtype is not None:
+        index = torch.randn((tokens, 128), generator=g, device=device).to(index_dtype)
+        index[: tokens // 3] *= 1e-6                                       # below the amax floor
+        index_pools = (torch.randn((pages, page, 128), generator=g, device=device).to(torch.float8_e4m3fn),
+                       torch.rand((pages, page), generator=g, device=device))
+        want_index = tuple(p.clone() for p in index_pools)
+    want = [p.clone() for p in pools]
+    plain_append(slots, k, v, want, index, want_index)
+    paged.append_tokens(slots, (k, v), tuple(pools), index_keys=index, index_pools=index_pools)
+    assert torch.equal(pools[0], want[0]) and torch.equal(pools[1], want[1])
+    if index is not None:
+        assert torch.equal(index_pools[0].view(torch.uint8), want_index[0].view(torch.uint8))
+        assert bool((index_pools[1] == want_index[1]).all())
+    paged.check_serving_status(device)
+
+
+@pytest.mark.gpu
+def test_slots_behind_the_pool_are_skipped_and_reported(device):
+    k = torch.ones((3, 2, 64), dtype=torch.bfloat16, device=device)
+    pools = [torch.zeros((2, 128, 2, 64), dtype=torch.bfloat16, device=device) for _ in range(2)]
+    slots = torch.tensor([256, 3, 1 << 40], dtype=torch.int64, device=device)
+    paged.append_tokens(slots, (k, k), tuple(pools))
+    assert int(pools[0].sum()) == 128 and bool((pools[0][0, 3] == 1).all())
+    with pytest.raises(_lib.ItkError, match="page or slot"):
+        paged.check_serving_status(device)
+
+
+@pytest.mark.gpu
+def test_append_refusals(device):
+    k = torch.ones((3, 2, 64), dtype=torch.bfloat16, device=device)
+    pool = torch.zeros((2, 128, 2, 64), dtype=torch.bfloat16, device=device)
+    slots = torch.arange(3, device=device)
+
+    def refused(match, *args, **kwargs):
+        with pytest.raises(ValueError, match=match):
+            paged.append_tokens(*args, **kwargs)
+
+    refused("CUDA", slots, (k.cpu(), k.cpu()), (pool, pool))
+    refused("shape", slots, (k, k[:2]), (pool, pool))
+    refused("type of k", slots, (k, k), (pool.half(), pool))
+    refused("int64", slots.int(), (k, k), (pool, pool))
+    refused("64 or 128", slots, (k[..., :32], k[..., :32]), (pool[..., :32], pool[..., :32]))
+    refused("index_pools", slots, (k, k), (pool, pool), index_keys=torch.zeros((3, 128), device=device))
+    refused("aligned", slots, (torch.ones((3, 2, 68), dtype=k.dtype, device=device)[..., 4:], k), (pool, pool))
+    plan = paged.make_page_plan(2, 4, 10, page_size=128, device=device)
+    table, ints = torch.zeros((2, 4), dtype=torch.int32, device=device), gpu([1, 2], device)
+    for bad in ((table[:1], ints, ints, ints), (table.long(), ints, ints, ints), (table, ints[:1], ints, ints),
+                (table, ints, ints.long(), ints), (table, ints, ints, ints.cpu()), (table[:1].expand(2, 4), ints, ints, ints)):
+        with pytest.raises(ValueError):
+            paged.plan_pages(plan, *bad)
+
+
+def test_page_plan_sizes_are_refused_without_a_gpu():
+    for kwargs in (dict(requests=0), dict(requests=20000), dict(table_pages=0), dict(page_size=100), dict(rows=-1),
+                   dict(requests=16384, table_pages=1024), dict(device="cpu")):
+        size = dict(requests=4, table_pages=4, rows=4, page_size=128, device="cuda") | kwargs
+        with pytest.raises(ValueError):
+            paged.make_page_plan(size.pop("requests"), size.pop("table_pages"), size.pop("rows"), **size)
+
+
+def test_c_entries_refuse_before_any_launch():
+    build()
+    library = _lib.load_library()
+    plan, append = _lib.PagePlanArgs(), _lib.AppendArgs()
+    assert library.itk_plan_pages(None, None) == -1
+    assert library.itk_plan_pages(ctypes.byref(plan), None) == -1
+    plan.requests, plan.table_pages, plan.page_size, plan.table_stride = 16384, 1024, 128, 1024
+    assert library.itk_plan_pages(ctypes.byref(plan), None) == -1
+    assert b"2^31" in library.itk_last_error()
+    plan.requests = 4
+    assert library.itk_plan_pages(ctypes.byref(plan), None) == -1
+    assert b"must not be null" in library.itk_last_error()
+    assert library.itk_append_tokens(None, None) == -1
+    assert library.itk_append_tokens(ctypes.byref(append), None) == -1
+    append.tokens, append.kv_heads, append.dim, append.pages, append.page_size = 3, 2, 128, 2, 128
+    assert library.itk_append_tokens(ctypes.byref(append), None) == -1
+    assert b"must not be null" in library.itk_last_error()
+    append.slots = append.k = append.v = append.k_pool = append.v_pool = 1 << 20
+    append.k_row_stride = 4
+    assert library.itk_append_tokens(ctypes.byref(append), None) == -1
+    assert b"multiples of 8" in library.itk_last_error()
+    append.k_row_stride, append.v = 8, (1 << 20) + 8
+    assert library.itk_append_tokens(ctypes.byref(append), None) == -1
+    assert b"aligned" in library.itk_last_error()

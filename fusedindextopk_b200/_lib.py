@@ -117,7 +117,7 @@ class AttentionArgs(ctypes.Structure):
         ("out_token_stride", c_longlong), ("out_head_stride", c_longlong), ("wait_limit_ns", ctypes.c_ulonglong),
         ("own", KvSegment), ("prefix", KvSegment), ("scale", ctypes.c_float), ("element", c_int),
         ("tokens", c_int), ("heads", c_int), ("kv_heads", c_int), ("dim", c_int), ("requests", c_int),
-        ("prefix_keys", c_int), ("causal", c_int), ("clear_tail", c_int),
+        ("prefix_keys", c_int), ("causal", c_int), ("clear_tail", c_int), ("withhold_loads", c_int),
     ]
 
 

@@ -101,12 +101,12 @@ def _attend(torch: Any, q: Any, kv_heads: int, own: Any, prefix: Any, prefix_key
     lse = torch.empty((tokens, heads), dtype=torch.float32, device=device) if return_lse else None
     if tokens:
         scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
-        _require(math.isfinite(scale), "scale must be finite")
+        _require(0.0 < scale < 1e38, "scale must be positive and finite")
         args = _lib.AttentionArgs(
             q.data_ptr(), out.data_ptr(), _lib.ptr(lse), cu_seqlens_q.data_ptr(), _lib.ptr(cu_seqlens_k), _lib.ptr(lengths),
             None, 0, q.stride(0), q.stride(1), out.stride(0), out.stride(1), 0, own, prefix, scale,
             _lib.ELEMENT_BF16 if q.dtype == torch.bfloat16 else _lib.ELEMENT_FP16, tokens, heads, kv_heads, dim, requests,
-            prefix_keys, int(causal), int(clear_tail))
+            prefix_keys, int(causal), int(clear_tail), 0)
         library = _lib.load_library()
         needed = ctypes.c_size_t(0)
         _lib.check(library.itk_attention_workspace_bytes(ctypes.byref(args), ctypes.byref(needed)))
@@ -132,8 +132,8 @@ def attention_varlen(q: Any, kv: tuple[Any, Any], cu_seqlens_q: Any, cu_seqlens_
 
     ``q`` is ``[T, Hq, D]``, ``kv = (k, v)`` both ``[N, H, D]``; request ``b`` owns rows
     ``cu_seqlens_q[b]:cu_seqlens_q[b+1]`` and keys ``cu_seqlens_k[b]:cu_seqlens_k[b+1]`` (int32 ``[B+1]`` each, lengths of
-    zero allowed).  With ``causal`` row i of its Q sees its first ``N - Q + i + 1`` keys, else all N.  ``scale`` defaults to
-    ``D ** -0.5``.  Rows behind the last request are zero (log-sum-exp ``-inf``), or left as they were in a given ``out``.
+    zero allowed).  With ``causal`` row i of its Q sees its first ``N - Q + i + 1`` keys, else all N.  ``scale`` (positive)
+    defaults to ``D ** -0.5``.  Rows behind the last request are zero (log-sum-exp ``-inf``), or left as they were in a given ``out``.
     """
 
     import torch

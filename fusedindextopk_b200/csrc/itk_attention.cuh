@@ -1,9 +1,35 @@
-// Attention of packed, paged and shared-prefix batches.
+// Attention of packed, paged and shared-prefix batches on the tensor cores.
 //
 //     s_j = scale * q . k_j,   m = max_j s_j,   l = sum_j exp(s_j - m),   out = sum_j exp(s_j - m) v_j / l
 //
 // over the prefix keys (all of them) and the request's own keys (the first min(N, N - Q + i + 1) of them for row i
 // of Q when causal).  Scores, statistics and sums are fp32.
+//
+// Rows.  The G = heads / kv_heads query heads of a key head share its keys, so one 128-row tile holds TT = 128 / G
+// consecutive tokens x G heads (row r = token r / G, head r % G): a single token of a decode step fills G rows of a
+// tile instead of one, and a prompt's tile needs its diagonal mask on few key tiles.
+//
+// Units.  An item is one key head, up to 2 TT tokens and a range of 128-key tiles.
+//   pair mode  (more than TT tokens): two row tiles A and B walk the same key tiles; every key tile read from L2
+//              serves 256 rows;
+//   split mode (at most TT tokens): one row tile; even key tiles go to lane A, odd ones to lane B, which are then two
+//              independent softmax states over the same rows, joined like any two partial results.  The tensor work
+//              and the softmax of one lane overlap the other's although there is one row tile only.
+// A plan kernel (one CTA) turns the lengths on the device into a list of items, longest first, cuts long ones into
+// chunks of keys when there are too few to fill the SMs, and lays out the partial results; the attention kernel
+// walks the list; a third kernel joins the partial results.  No length is read by the host.
+//
+// Attention kernel, one CTA per SM, 11 warps: 0-3 softmax of lane A, 4-7 softmax of lane B (one row per thread),
+// 8 UMMA issuer and TMEM owner, 9 TMA producer, 10 guard.  TMEM: S_A, S_B (128 columns each; the weights P overwrite
+// the first half of S as 16-bit pairs and are the A operand of P V from there), O_A, O_B.  The row maximum is only
+// moved when it grows by more than 2^8 (kLazy): until then weights are at most 2^8 and O needs no rescaling; when it
+// does, the row's own softmax warp rescales O in TMEM, which is safe because S of a tile is complete only after P V
+// of the tile before it.
+//
+// Masked places.  Scores behind a row's last key are replaced, not added to, so keys may hold anything there.  A value
+// row that some row of the item does not see could still reach it as 0 * inf: the guard warp zeroes value rows
+// behind the request's end in shared memory and, on the tiles where rows differ in what they see, zeroes non-finite
+// values and reports them, and the epilogue adds them back to the rows that do see them.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -14,32 +40,195 @@
 
 namespace itk {
 
-constexpr int kRowsKernelThreads = 128;
+constexpr int kAttnTile = 128;                 // rows of a row tile, keys of a key tile
+constexpr int kAttnThreads = 352;
+constexpr int kAttnSoftmaxWarps = 4;           // per lane
+constexpr int kAttnMmaWarp = 8, kAttnLoadWarp = 9, kAttnGuardWarp = 10;
+constexpr int kAttnTmemColumns = 512;
+constexpr int kAttnColumnS = 0, kAttnColumnO = 256;   // lane B: + 128
+constexpr int kAttnMaxStages = 10;
+constexpr int kAttnPoison = 16;                // items the guard may be ahead of an epilogue, with room to spare
+constexpr float kAttnLazy = 8.0f;              // log2 of how far weights may exceed 1 before the maximum moves
+constexpr float kLn2 = 0.69314718055994530942f;
+constexpr float kLog2e = 1.44269504088896340736f;
+
+template <int DIM>
+struct AttnShape {
+    static constexpr int kChunks = DIM / 64;                    // 128-byte wide column chunks
+    static constexpr int kTileBytes = kAttnTile * DIM * 2;
+    static constexpr int kStages = DIM == 128 ? 5 : 10;         // 160 KB of key and value tiles in flight
+    static constexpr int kSmemTiles = (2 + kStages) * kTileBytes;
+    static constexpr int kSmemBytes = kSmemTiles + 1024;
+};
+
+// One unit of work for every key head.
+struct AttnItem {
+    int q_first, tokens;      // packed row tokens [q_first, q_first + tokens)
+    int tile_begin, tiles;    // 128-key tiles of the segment
+    int keys;                 // keys of the segment that any row of the item may see
+    int visible, slope;       // token i sees min(keys, visible + slope * i) of them
+    int request;              // whose block table row to use; -1: the prefix
+    int k_first;              // first row of packed own keys
+    int partial, slot, slots; // row of the partial results of the whole entry (-1: write the output), first slot, slots
+};
+
+struct AttnCombine {
+    int q_first, tokens;
+    int partial, slots;       // own partial results
+};
+
+struct AttnCounters {
+    int items, combines, partial_rows, rows_end;
+};
+
+struct AttnWorkspace {
+    AttnCounters* counters;
+    int* entry_first;         // [requests + 1] own entries before a request
+    int2* prefix_slots;       // per prefix entry: first partial row, slots
+    AttnItem* items;
+    AttnCombine* combines;
+    float* partial_lse;       // log2 of the sum of exponentials of a partial row
+    float* partial_out;       // [partial_rows, DIM], normalised
+    int max_items, max_combines, max_partial_rows;
+};
+
+struct AttnParams {
+    CUtensorMap map_q, map_k, map_v, map_k_prefix, map_v_prefix;
+    itk_attention_args a;
+    AttnWorkspace w;
+    int* status;
+    int group, tile_tokens, sm_count, withhold_loads;
+    float scale_log2;
+    unsigned long long wait_limit_ns;
+};
+
+// ------------------------------------------------------------------ PTX
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2, int c3) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+        ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+        : "memory");
+}
+
+// 16-bit floating-point operands, fp32 accumulator, M = 128.
+__host__ __device__ constexpr uint32_t umma_idesc_16bit(bool bf16, int n, bool b_mn_major) {
+    return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_mn_major ? 1u : 0u) << 16) |
+           ((static_cast<uint32_t>(n) >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+// MN-major operand (rows of the tile are the K dimension), 128-byte swizzle: 64-column chunks are `chunk_bytes` apart,
+// eight-row groups 1024 bytes.
+__device__ __forceinline__ uint64_t umma_desc_sw128_mnmajor(uint32_t smem_address, uint32_t chunk_bytes) {
+    uint64_t desc = 0;
+    desc |= static_cast<uint64_t>((smem_address & 0x3FFFFu) >> 4);
+    desc |= static_cast<uint64_t>(chunk_bytes >> 4) << 16;
+    desc |= static_cast<uint64_t>(1024 >> 4) << 32;
+    desc |= static_cast<uint64_t>(1) << 46;
+    desc |= static_cast<uint64_t>(2) << 61;
+    return desc;
+}
+
+__device__ __forceinline__ void umma_16bit_ss(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void umma_16bit_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_store_16(uint32_t tmem_address, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(tmem_address), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_load_8(uint32_t tmem_address, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(tmem_address)
+                 : "memory");
+}
+
+__device__ __forceinline__ void tmem_load_wait8(uint32_t (&r)[8]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
+                 :
+                 : "memory");
+}
+
+__device__ __forceinline__ void tmem_store_8(uint32_t tmem_address, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(tmem_address), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 template <typename T>
-__device__ __forceinline__ float to_float(T x);
+struct Element;
+
 template <>
-__device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+struct Element<__nv_bfloat16> {
+    static constexpr bool kBf16 = true;
+    static constexpr uint32_t kExponent = 0x7f80u;
+    static __device__ __forceinline__ uint32_t pack(float low, float high) {
+        uint32_t r;
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(high), "f"(low));
+        return r;
+    }
+    static __device__ __forceinline__ float value(uint32_t bits) { return __uint_as_float(bits << 16); }
+};
+
 template <>
-__device__ __forceinline__ float to_float<__half>(__half x) { return __half2float(x); }
-template <typename T>
-__device__ __forceinline__ T from_float(float x);
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-template <>
-__device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+struct Element<__half> {
+    static constexpr bool kBf16 = false;
+    static constexpr uint32_t kExponent = 0x7c00u;
+    static __device__ __forceinline__ uint32_t pack(float low, float high) {
+        uint32_t r;
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(high), "f"(low));
+        return r;
+    }
+    static __device__ __forceinline__ float value(uint32_t bits) { return __half2float(__ushort_as_half(static_cast<unsigned short>(bits))); }
+};
+
+// ------------------------------------------------------------------ plan
 
 // Lengths of one request, clamped to the buffers they index.
-struct AttentionRequest {
+struct AttnRequest {
     int q_first, q_count, k_first, k_count;
 };
 
-__device__ __forceinline__ AttentionRequest attention_request(const itk_attention_args& p, int b, int* status) {
-    AttentionRequest r;
+__device__ __forceinline__ AttnRequest attn_request(const itk_attention_args& p, int b, bool& bad) {
+    AttnRequest r;
     const int q0 = p.cu_q[b], q1 = p.cu_q[b + 1];
     r.q_first = min(max(q0, 0), p.tokens);
     r.q_count = max(min(max(q1, 0), p.tokens) - r.q_first, 0);
-    bool bad = q0 != r.q_first || q1 != r.q_first + r.q_count;
+    bad |= q0 != r.q_first || q1 != r.q_first + r.q_count;
     if (p.cu_k != nullptr) {
         const int k0 = p.cu_k[b], k1 = p.cu_k[b + 1];
         r.k_first = min(max(k0, 0), p.own.page_size);
@@ -52,101 +241,831 @@ __device__ __forceinline__ AttentionRequest attention_request(const itk_attentio
         r.k_count = static_cast<int>(min(static_cast<long long>(max(n, 0)), room));
         bad |= n != r.k_count;
     }
-    if (bad) atomicOr(status, ITK_SERVING_BAD_LENGTHS);
     return r;
 }
 
-// One warp per (row, head): the plainest form.  32 keys at a time, a lane scores one of them; the weighted values
-// are added with every lane owning dim / 32 columns.
-template <typename T, int DIM>
-__global__ void __launch_bounds__(kRowsKernelThreads) itk_attention_rows_kernel(const itk_attention_args p, int* status) {
-    constexpr int kOwn = DIM / 32;
-    __shared__ float q_rows[kRowsKernelThreads / 32][DIM];
-    const int lane = threadIdx.x & 31;
-    float* q_row = q_rows[threadIdx.x >> 5];
-    const long long work = static_cast<long long>(blockIdx.x) * (kRowsKernelThreads / 32) + (threadIdx.x >> 5);
-    if (work >= static_cast<long long>(p.tokens) * p.heads) return;
-    const int token = static_cast<int>(work / p.heads), head = static_cast<int>(work - static_cast<long long>(token) * p.heads);
-    const int kv_head = head / (p.heads / p.kv_heads);
-    T* out = static_cast<T*>(p.out) + token * p.out_token_stride + head * p.out_head_stride;
+constexpr int kAttnPlanThreads = 1024;
+constexpr int kAttnBins = 256;
+constexpr int kAttnTries = 8;
+constexpr int kAttnMinChunk = 2;    // key tiles of a chunk at least: below that a chunk's fixed cost outweighs its keys
+static_assert(kAttnMinChunk >= 2, "a split item of one tile is its entry's only item: it has one slot and no lane B");
+// Relative cost of a key tile: a pair tile is bound by tensor and exponential work for 256 rows, a split tile by
+// the time its keys take to arrive.
+constexpr int kAttnPairCost = 4, kAttnSplitCost = 3;
 
-    int low = 0, high = p.requests;
-    while (high - low > 1) {
-        const int middle = (low + high) >> 1;
-        if (p.cu_q[middle] <= token) {
-            low = middle;
+struct AttnEntry {
+    AttnItem item;
+    int tiles, unit;          // key tiles, cost of one
+    bool pair, prefix;
+};
+
+// Entry e of the list "prefix entries, then the entries of request 0, 1, ...": up to 2 TT consecutive tokens of one
+// request (of any requests for the prefix, which they all see).
+__device__ __forceinline__ AttnEntry attn_entry(const AttnParams& p, int e, int prefix_entries, int rows_end) {
+    const int span = 2 * p.tile_tokens;
+    AttnEntry r;
+    r.prefix = e < prefix_entries;
+    if (r.prefix) {
+        r.item.q_first = e * span;
+        r.item.tokens = min(span, rows_end - e * span);
+        r.item.keys = p.a.prefix_keys;
+        r.item.visible = p.a.prefix_keys;
+        r.item.slope = 0;
+        r.item.request = -1;
+        r.item.k_first = 0;
+    } else {
+        const int own = e - prefix_entries;
+        int low = 0, high = p.a.requests;       // entry_first[low] <= own < entry_first[high]
+        while (high - low > 1) {
+            const int middle = (low + high) >> 1;
+            if (p.w.entry_first[middle] <= own) {
+                low = middle;
+            } else {
+                high = middle;
+            }
+        }
+        bool bad = false;
+        const AttnRequest q = attn_request(p.a, low, bad);
+        const int first = (own - p.w.entry_first[low]) * span;
+        r.item.q_first = q.q_first + first;
+        r.item.tokens = min(span, q.q_count - first);
+        r.item.request = low;
+        r.item.k_first = q.k_first;
+        if (p.a.causal) {
+            r.item.visible = q.k_count - q.q_count + first + 1;
+            r.item.slope = 1;
+            r.item.keys = max(0, min(q.k_count, r.item.visible + r.item.tokens - 1));
         } else {
-            high = middle;
+            r.item.visible = r.item.keys = q.k_count;
+            r.item.slope = 0;
         }
     }
-    const AttentionRequest r = attention_request(p, low, status);
-    if (token < r.q_first || token >= r.q_first + r.q_count) {
-        if (p.clear_tail) {
-            for (int c = lane; c < DIM; c += 32) out[c] = from_float<T>(0.0f);
-            if (lane == 0 && p.lse != nullptr) p.lse[work] = -INFINITY;
+    r.tiles = (r.item.keys + kAttnTile - 1) / kAttnTile;
+    r.pair = r.item.tokens > p.tile_tokens;
+    r.unit = r.pair ? kAttnPairCost : kAttnSplitCost;
+    return r;
+}
+
+__device__ __forceinline__ int attn_chunks(const AttnEntry& e, long long cost) {
+    const long long per = max(static_cast<long long>(kAttnMinChunk), (cost + e.unit - 1) / e.unit);
+    return static_cast<int>((e.tiles + per - 1) / per);
+}
+
+__global__ void __launch_bounds__(kAttnPlanThreads) itk_attention_plan_kernel(const __grid_constant__ AttnParams p) {
+    __shared__ int warp_sums[kAttnPlanThreads / 32];
+    __shared__ int carry, rows_end;
+    __shared__ unsigned long long total_cost;
+    __shared__ int counts[kAttnTries], longest, item_count, combine_count, partial_rows;
+    __shared__ int bins[kAttnBins];
+    const int tx = threadIdx.x, lane = tx & 31, warp = tx >> 5;
+    const int span = 2 * p.tile_tokens, kv_heads = p.a.kv_heads;
+    if (tx == 0) {
+        carry = 0;
+        total_cost = 0;
+        longest = item_count = combine_count = partial_rows = 0;
+        rows_end = min(max(p.a.cu_q[p.a.requests], 0), p.a.tokens);
+    }
+    if (tx < kAttnTries) counts[tx] = 0;
+    if (tx < kAttnBins) bins[tx] = 0;
+    __syncthreads();
+
+    // own entries before every request
+    bool bad = false;
+    for (int base = 0; base < p.a.requests; base += kAttnPlanThreads) {
+        const int b = base + tx;
+        int mine = 0;
+        if (b < p.a.requests) mine = (attn_request(p.a, b, bad).q_count + span - 1) / span;
+        int upto = mine;
+#pragma unroll
+        for (int step = 1; step < 32; step <<= 1) {
+            const int other = __shfl_up_sync(0xffffffffu, upto, step);
+            if (lane >= step) upto += other;
         }
+        if (lane == 31) warp_sums[warp] = upto;
+        __syncthreads();
+        int before = carry;
+        for (int w = 0; w < warp; ++w) before += warp_sums[w];
+        if (b < p.a.requests) p.w.entry_first[b] = before + upto - mine;
+        __syncthreads();
+        if (tx == kAttnPlanThreads - 1) carry = before + upto;
+        __syncthreads();
+    }
+    if (bad) atomicOr(p.status, ITK_SERVING_BAD_LENGTHS);
+    const int prefix_entries = p.a.prefix_keys > 0 ? (rows_end + span - 1) / span : 0;
+    const int own_entries = min(carry, p.w.max_combines);
+    const int entries = prefix_entries + own_entries;
+    if (tx == 0) p.w.entry_first[p.a.requests] = own_entries;
+    __syncthreads();
+
+    // the chunk length that spreads the work over the SMs in one wave, if there is one
+    unsigned long long cost = 0;
+    for (int e = tx; e < entries; e += kAttnPlanThreads) {
+        const AttnEntry entry = attn_entry(p, e, prefix_entries, rows_end);
+        cost += static_cast<unsigned long long>(entry.tiles) * entry.unit;
+    }
+    atomicAdd(&total_cost, cost);
+    __syncthreads();
+    const long long share = max(1ll, (static_cast<long long>(total_cost) * kv_heads + p.sm_count - 1) / p.sm_count);
+    int mine[kAttnTries] = {};
+    for (int e = tx; e < entries; e += kAttnPlanThreads) {
+        const AttnEntry entry = attn_entry(p, e, prefix_entries, rows_end);
+#pragma unroll
+        for (int k = 0; k < kAttnTries; ++k) mine[k] += attn_chunks(entry, share + share * k / kAttnTries);
+    }
+#pragma unroll
+    for (int k = 0; k < kAttnTries; ++k)
+        if (mine[k] != 0) atomicAdd(&counts[k], mine[k]);
+    __syncthreads();
+    long long chunk = share;
+    for (int k = kAttnTries - 1; k >= 0; --k)
+        if (static_cast<long long>(counts[k]) * kv_heads <= p.sm_count) chunk = share + share * k / kAttnTries;
+
+    // items by cost, the costliest first: a counting sort over 256 cost classes
+    for (int e = tx; e < entries; e += kAttnPlanThreads) {
+        const AttnEntry entry = attn_entry(p, e, prefix_entries, rows_end);
+        const int chunks = max(1, attn_chunks(entry, chunk));
+        atomicMax(&longest, (entry.tiles + chunks - 1) / chunks * entry.unit);
+    }
+    __syncthreads();
+    const int top = max(longest, 1);
+    for (int e = tx; e < entries; e += kAttnPlanThreads) {
+        const AttnEntry entry = attn_entry(p, e, prefix_entries, rows_end);
+        const int chunks = max(1, attn_chunks(entry, chunk));
+        const int item_cost = (entry.tiles + chunks - 1) / chunks * entry.unit;
+        const int bin = kAttnBins - 1 - static_cast<int>(static_cast<long long>(item_cost) * (kAttnBins - 1) / top);
+        atomicAdd(&bins[bin], chunks);
+    }
+    __syncthreads();
+    if (warp == 0) {
+        int sum = 0, held[kAttnBins / 32];
+#pragma unroll
+        for (int i = 0; i < kAttnBins / 32; ++i) {
+            held[i] = bins[lane * (kAttnBins / 32) + i];
+            sum += held[i];
+        }
+        int upto = sum;
+#pragma unroll
+        for (int step = 1; step < 32; step <<= 1) {
+            const int other = __shfl_up_sync(0xffffffffu, upto, step);
+            if (lane >= step) upto += other;
+        }
+        int before = upto - sum;
+#pragma unroll
+        for (int i = 0; i < kAttnBins / 32; ++i) {
+            bins[lane * (kAttnBins / 32) + i] = before;
+            before += held[i];
+        }
+        if (lane == 31) item_count = before;
+    }
+    __syncthreads();
+    for (int e = tx; e < entries; e += kAttnPlanThreads) {
+        AttnEntry entry = attn_entry(p, e, prefix_entries, rows_end);
+        const int chunks = attn_chunks(entry, chunk);               // 0: no key at all
+        const int longest_chunk = chunks > 0 ? (entry.tiles + chunks - 1) / chunks : 0;
+        const int lanes = !entry.pair && longest_chunk > 1 ? 2 : 1;
+        entry.item.slots = chunks * lanes;
+        entry.item.partial = -1;
+        const bool joined = p.a.prefix_keys > 0 || entry.item.slots > 1;
+        if (joined && entry.item.slots > 0) {
+            const int rows = entry.item.slots * entry.item.tokens * p.group * kv_heads;
+            const int first = atomicAdd(&partial_rows, rows);
+            // (the host sizes the buffer so that this always fits; nothing is written behind it if it did not)
+            entry.item.partial = first + rows <= p.w.max_partial_rows ? first : -2;
+            if (entry.item.partial == -2) atomicOr(p.status, ITK_SERVING_BAD_LENGTHS);
+        }
+        if (entry.prefix) {
+            p.w.prefix_slots[e] = make_int2(entry.item.partial, entry.item.partial < 0 ? 0 : entry.item.slots);
+        } else if (joined) {
+            const int at = atomicAdd(&combine_count, 1);
+            p.w.combines[at] = AttnCombine{entry.item.q_first, entry.item.tokens, entry.item.partial,
+                                           entry.item.partial < 0 ? 0 : entry.item.slots};
+        }
+        if (chunks == 0 && joined) {        // the prefix alone: a place in the list, but nothing to do
+            entry.item.tokens = 0;
+        }
+        const int count = max(1, chunks);
+        const int item_cost = (entry.tiles + count - 1) / count * entry.unit;
+        const int bin = kAttnBins - 1 - static_cast<int>(static_cast<long long>(item_cost) * (kAttnBins - 1) / top);
+        const int place = atomicAdd(&bins[bin], count);
+        for (int c = 0; c < count; ++c) {
+            const long long lo = static_cast<long long>(entry.tiles) * c / count, hi = static_cast<long long>(entry.tiles) * (c + 1) / count;
+            entry.item.tile_begin = static_cast<int>(lo);
+            entry.item.tiles = static_cast<int>(hi - lo);
+            entry.item.slot = c * lanes;
+            if (place + c < p.w.max_items) p.w.items[place + c] = entry.item;
+        }
+    }
+    __syncthreads();
+    if (tx == 0) *p.w.counters = AttnCounters{min(item_count, p.w.max_items), combine_count, partial_rows, rows_end};
+}
+
+// ------------------------------------------------------------------ attention
+
+struct AttnShared {
+    uint64_t q_full[2], q_empty[2];
+    uint64_t kv_full[kAttnMaxStages], kv_empty[kAttnMaxStages], guard_full[kAttnMaxStages];
+    uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
+    int poison[kAttnPoison];
+    uint32_t tmem_base;
+    int abort;
+};
+static_assert(sizeof(AttnShared) <= 1024, "barriers fit the tail of the shared-memory block");
+
+// What an item means for one lane.
+struct AttnLanes {
+    bool pair;
+    int first_visible;        // keys that every row sees
+    int tiles[2];             // key tiles of lane A, B
+};
+
+__device__ __forceinline__ AttnLanes attn_lanes(const AttnItem& item, int tile_tokens) {
+    AttnLanes r;
+    r.pair = item.tokens > tile_tokens;
+    r.first_visible = max(0, min(item.visible, item.keys));
+    r.tiles[0] = r.pair ? item.tiles : (item.tiles + 1) / 2;
+    r.tiles[1] = r.pair ? item.tiles : item.tiles / 2;
+    return r;
+}
+
+// Walks this CTA's share of the list: item k of every wave, the waves in alternating direction so that the CTA with
+// the longest item of one wave has the shortest of the next.
+struct AttnWalk {
+    int wave = 0, total, heads;
+    __device__ __forceinline__ AttnWalk(const AttnParams& p) : total(p.w.counters->items * p.a.kv_heads), heads(p.a.kv_heads) {}
+    __device__ __forceinline__ bool next(const AttnParams& p, AttnItem& item, int& head) {
+        for (;;) {
+            const int grid = static_cast<int>(gridDim.x), me = static_cast<int>(blockIdx.x);
+            const long long at = static_cast<long long>(wave) * grid + ((wave & 1) ? grid - 1 - me : me);
+            if (static_cast<long long>(wave) * grid >= total) return false;
+            ++wave;
+            if (at >= total) continue;
+            const int index = static_cast<int>(at) / heads;
+            head = static_cast<int>(at) - index * heads;
+            const int4* source = reinterpret_cast<const int4*>(p.w.items + index);
+            const int4 a = source[0], b = source[1], c = source[2];
+            item = AttnItem{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, c.x, c.y, c.z, c.w};
+            if (item.tokens > 0) return true;
+        }
+    }
+};
+static_assert(sizeof(AttnItem) == 48, "items are read as three 16-byte vectors");
+
+// Where key tile t of a segment lies.
+__device__ __forceinline__ int attn_page(const AttnParams& p, const AttnItem& item, int t) {
+    const itk_kv_segment& seg = item.request < 0 ? p.a.prefix : p.a.own;
+    if (seg.table == nullptr) return 0;
+    const int32_t* table = seg.table + (item.request < 0 ? 0 : item.request * seg.table_stride);
+    const int page = table[t / (seg.page_size / kAttnTile)];
+    if (page < 0 || page >= seg.pages) {
+        atomicOr(p.status, ITK_SERVING_BAD_PAGE);
+        return page < 0 ? 0 : seg.pages - 1;
+    }
+    return page;
+}
+
+template <typename T>
+__device__ __forceinline__ const T* attn_value_row(const AttnParams& p, const AttnItem& item, int head, int key) {
+    const itk_kv_segment& seg = item.request < 0 ? p.a.prefix : p.a.own;
+    long long row = item.k_first + key;
+    long long page = 0;
+    if (seg.table != nullptr) {
+        page = attn_page(p, item, key / kAttnTile);
+        row = key % seg.page_size;
+    }
+    return static_cast<const T*>(seg.v) + page * seg.v_page_stride + row * seg.v_row_stride + head * seg.v_head_stride;
+}
+
+// Ring position of the key and value tile of step t of an item.  Pair: K0 V0 K1 V1 ...  Split (the lanes take turns and
+// each is one key tile ahead of its values): K0 K1 V0 K2 V1 K3 ... V(n-1).
+__device__ __forceinline__ int ring_key(bool pair, int t) { return pair ? 2 * t : (t < 2 ? t : 2 * t - 1); }
+__device__ __forceinline__ int ring_value(bool pair, int t, int tiles) {
+    return pair ? 2 * t + 1 : min(2 * t + 2, 2 * tiles - 1);
+}
+
+template <typename T, int DIM>
+__global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __grid_constant__ AttnParams p) {
+    using Shape = AttnShape<DIM>;
+    constexpr int kStages = Shape::kStages;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t* smem_q = smem;
+    uint8_t* smem_kv = smem + 2 * Shape::kTileBytes;
+    AttnShared& sh = *reinterpret_cast<AttnShared*>(smem + Shape::kSmemTiles);
+    const int warp = static_cast<int>(threadIdx.x) >> 5;
+    const int lane = static_cast<int>(threadIdx.x) & 31;
+
+    if ((smem_u32(smem) & 1023u) != 0u) {   // the same in every thread
+        if (threadIdx.x == 0) atomicOr(p.status, ITK_SERVING_BAD_SHARED_BASE);
         return;
     }
-    const int visible = p.causal ? min(r.k_count, r.k_count - r.q_count + (token - r.q_first) + 1) : r.k_count;
-    const T* q = static_cast<const T*>(p.q) + token * p.q_token_stride + head * p.q_head_stride;
-    for (int c = lane; c < DIM; c += 32) q_row[c] = to_float<T>(q[c]);
-    __syncwarp();
+    if (static_cast<int>(blockIdx.x) >= p.w.counters->items * p.a.kv_heads) return;   // more CTAs than work
 
-    float top = -INFINITY, total = 0.0f, sums[kOwn] = {};
-    for (int part = 0; part < 2; ++part) {
-        const itk_kv_segment& seg = part == 0 ? p.prefix : p.own;
-        const int keys = part == 0 ? (p.prefix.k != nullptr ? p.prefix_keys : 0) : visible;
-        const int first = part == 0 ? 0 : r.k_first;
-        const int32_t* table = seg.table == nullptr ? nullptr : seg.table + (part == 0 ? 0 : low * seg.table_stride);
-        for (int base = 0; base < keys; base += 32) {
-            const int key = base + lane;
-            float score = -INFINITY;
-            const T* v_row = nullptr;
-            if (key < keys) {
-                long long page = 0, row = first + key;
-                if (table != nullptr) {
-                    page = table[key / seg.page_size];
-                    row = key % seg.page_size;
-                    if (page < 0 || page >= seg.pages) {
-                        atomicOr(status, ITK_SERVING_BAD_PAGE);
-                        page = page < 0 ? 0 : seg.pages - 1;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh.q_full[i], 1);
+            mbar_init(&sh.q_empty[i], 1);
+            mbar_init(&sh.s_full[i], 1);
+            mbar_init(&sh.p_full[i], kAttnSoftmaxWarps);
+            mbar_init(&sh.o_full[i], 1);
+            mbar_init(&sh.o_empty[i], kAttnSoftmaxWarps);
+        }
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(&sh.kv_full[i], 1);
+            mbar_init(&sh.kv_empty[i], 1);
+            mbar_init(&sh.guard_full[i], 1);
+        }
+        for (int i = 0; i < kAttnPoison; ++i) sh.poison[i] = 0;
+        sh.abort = 0;
+        fence_mbar_init();
+        prefetch_tensormap(&p.map_q);
+        prefetch_tensormap(&p.map_k);
+        prefetch_tensormap(&p.map_v);
+    }
+    if (warp == kAttnMmaWarp) {
+        tmem_alloc(&sh.tmem_base, kAttnTmemColumns);
+        tmem_relinquish_alloc_permit();
+    }
+    tcgen05_fence_before_sync();
+    __syncthreads();
+    tcgen05_fence_after_sync();
+    const uint32_t tmem = sh.tmem_base;
+    volatile int* abort_flag = &sh.abort;
+    // a wait of the whole warp: its lanes leave together
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.wait_limit_ns)) != 0;
+    };
+    bool ok = true;
+    AttnItem item;
+    int head;
+    AttnWalk walk(p);
+
+    if (warp == kAttnLoadWarp) {
+        // ============================================================ TMA producer
+        int ring = 0;                 // tiles loaded so far
+        int q_uses[2] = {0, 0};
+        const int q_bytes = Shape::kChunks * p.tile_tokens * p.group * 128;
+        while (ok && p.withhold_loads == 0 && walk.next(p, item, head)) {
+            const AttnLanes l = attn_lanes(item, p.tile_tokens);
+            if (item.tiles == 0) continue;
+            for (int tile = 0; ok && tile < (l.pair ? 2 : 1); ++tile) {
+                ok = wait(&sh.q_empty[tile], (q_uses[tile] & 1) ^ 1);
+                ++q_uses[tile];
+                if (ok && lane == 0) {
+                    mbar_arrive_expect_tx(&sh.q_full[tile], q_bytes);
+                    for (int c = 0; c < Shape::kChunks; ++c)
+                        tma_load_3d(smem_q + tile * Shape::kTileBytes + c * (kAttnTile * 128), &p.map_q, &sh.q_full[tile], c * 64,
+                                    head * p.group, item.q_first + tile * p.tile_tokens);
+                }
+            }
+            const itk_kv_segment& seg = item.request < 0 ? p.a.prefix : p.a.own;
+            const CUtensorMap* map_k = item.request < 0 ? &p.map_k_prefix : &p.map_k;
+            const CUtensorMap* map_v = item.request < 0 ? &p.map_v_prefix : &p.map_v;
+            const bool table = seg.table != nullptr;
+            const int steps = 2 * item.tiles;
+            int k_next = 0, v_next = 0;
+            int k_pages = 0, v_pages = 0;       // pages of 32 key (value) tiles, one per lane
+            for (int s = 0; ok && s < steps; ++s) {
+                // pair: K V K V; split: K K V K V K ... V V
+                const bool key_tile = l.pair ? (s & 1) == 0 : (s < 2 ? s < item.tiles : (k_next < item.tiles && (s & 1) != 0));
+                const int t = key_tile ? k_next++ : v_next++;
+                int& pages = key_tile ? k_pages : v_pages;
+                if (table && (t & 31) == 0) pages = t + lane < item.tiles ? attn_page(p, item, item.tile_begin + t + lane) : 0;
+                const int page = table ? __shfl_sync(0xffffffffu, pages, t & 31) : 0;
+                const int key = (item.tile_begin + t) * kAttnTile;
+                const int row = table ? key % seg.page_size : item.k_first + key;
+                const int stage = ring % kStages;
+                ok = wait(&sh.kv_empty[stage], ((ring / kStages) & 1) ^ 1);
+                ++ring;
+                if (ok && lane == 0) {
+                    // a value tile that the guard has to look at reaches the issuer through the guard
+                    const bool guarded = !key_tile && key + kAttnTile > l.first_visible;
+                    uint64_t* full = guarded ? &sh.guard_full[stage] : &sh.kv_full[stage];
+                    mbar_arrive_expect_tx(full, Shape::kTileBytes);
+                    for (int c = 0; c < Shape::kChunks; ++c)
+                        tma_load_4d(smem_kv + stage * Shape::kTileBytes + c * (kAttnTile * 128), key_tile ? map_k : map_v,
+                                    full, c * 64, head, row, page);
+                }
+            }
+        }
+    } else if (warp == kAttnMmaWarp) {
+        // ============================================================ UMMA issuer
+        constexpr uint32_t kIdescS = umma_idesc_16bit(Element<T>::kBf16, kAttnTile, false);
+        constexpr uint32_t kIdescO = umma_idesc_16bit(Element<T>::kBf16, DIM, true);
+        int ring = 0, items_of[2] = {0, 0}, steps_of[2] = {0, 0}, q_uses[2] = {0, 0};
+        while (ok && walk.next(p, item, head)) {
+            const AttnLanes l = attn_lanes(item, p.tile_tokens);
+            if (item.tiles == 0) continue;
+            for (int tile = 0; ok && tile < (l.pair ? 2 : 1); ++tile) {
+                ok = wait(&sh.q_full[tile], q_uses[tile] & 1);
+                ++q_uses[tile];
+            }
+            // S of lane x for its key tile j; the key tile is released when its last reader has been issued
+            auto scores = [&](int x, int j) {
+                const int t = l.pair ? j : 2 * j + x;
+                const int at = ring + ring_key(l.pair, t);
+                const int stage = at % kStages;
+                ok = ok && wait(&sh.kv_full[stage], (at / kStages) & 1);
+                if (!ok) return;
+                tcgen05_fence_after_sync();
+                if (lane == 0) {
+                    const uint32_t a = smem_u32(smem_q + (l.pair ? x : 0) * Shape::kTileBytes);
+                    const uint32_t b = smem_u32(smem_kv + stage * Shape::kTileBytes);
+#pragma unroll
+                    for (int k = 0; k < DIM / 16; ++k) {
+                        const uint32_t offset = (k / 4) * (kAttnTile * 128) + (k % 4) * 32;
+                        umma_16bit_ss(tmem + kAttnColumnS + x * 128, umma_desc_sw128_kmajor(a + offset),
+                                      umma_desc_sw128_kmajor(b + offset), kIdescS, k > 0);
+                    }
+                    if (!l.pair || x == 1) umma_commit(&sh.kv_empty[stage]);
+                    umma_commit(&sh.s_full[x]);
+                    // the last scores of a row tile: its rows may be replaced
+                    if (t + 1 == item.tiles) umma_commit(&sh.q_empty[l.pair ? x : 0]);
+                }
+                __syncwarp();
+            };
+            scores(0, 0);
+            if (l.tiles[1] > 0) scores(1, 0);
+            for (int j = 0; ok && j < l.tiles[0]; ++j) {
+                for (int x = 0; ok && x < 2; ++x) {
+                    if (j >= l.tiles[x]) break;
+                    const int t = l.pair ? j : 2 * j + x;
+                    const int at = ring + ring_value(l.pair, t, item.tiles);
+                    const int stage = at % kStages;
+                    ok = wait(&sh.kv_full[stage], (at / kStages) & 1);
+                    if (ok && j == 0) ok = wait(&sh.o_empty[x], (items_of[x] & 1) ^ 1);
+                    if (ok) ok = wait(&sh.p_full[x], steps_of[x] & 1);
+                    ++steps_of[x];
+                    if (!ok) break;
+                    tcgen05_fence_after_sync();
+                    if (lane == 0) {
+                        const uint32_t a = tmem + kAttnColumnS + x * 128;
+                        const uint32_t b = smem_u32(smem_kv + stage * Shape::kTileBytes);
+#pragma unroll
+                        for (int k = 0; k < kAttnTile / 16; ++k)
+                            umma_16bit_ts(tmem + kAttnColumnO + x * 128, a + k * 8,
+                                          umma_desc_sw128_mnmajor(b + k * 2048, kAttnTile * 128), kIdescO, j > 0 || k > 0);
+                        if (!l.pair || x == 1) umma_commit(&sh.kv_empty[stage]);
+                        if (j + 1 == l.tiles[x]) umma_commit(&sh.o_full[x]);
+                    }
+                    __syncwarp();
+                    if (j + 1 == l.tiles[x]) ++items_of[x];
+                    if (j + 1 < l.tiles[x]) scores(x, j + 1);
+                }
+            }
+            ring += 2 * item.tiles;
+        }
+    } else if (warp == kAttnGuardWarp) {
+        // ============================================================ guard
+        int ring = 0, sequence = 0;
+        uint32_t phases = 0;          // of guard_full: a stage's flips with every tile the guard takes from it
+        while (ok && p.withhold_loads == 0 && walk.next(p, item, head)) {
+            const AttnLanes l = attn_lanes(item, p.tile_tokens);
+            ++sequence;
+            if (item.tiles == 0) continue;
+            const int first = max(0, l.first_visible / kAttnTile - item.tile_begin);
+            for (int t = first; ok && t < item.tiles; ++t) {
+                const int at = ring + ring_value(l.pair, t, item.tiles);
+                const int stage = at % kStages;
+                ok = wait(&sh.guard_full[stage], (phases >> stage) & 1);
+                phases ^= 1u << stage;
+                if (!ok) break;
+                const int base = (item.tile_begin + t) * kAttnTile;
+                const int shared_rows = max(0, l.first_visible - base), end = min(kAttnTile, item.keys - base);
+                uint8_t* tile = smem_kv + stage * Shape::kTileBytes;
+                bool found = false;
+                constexpr int kVectors = DIM / 8;
+                for (int i = shared_rows * kVectors + lane; i < kAttnTile * kVectors; i += 32) {
+                    const int row = i / kVectors, vector = i % kVectors;
+                    uint4* place = reinterpret_cast<uint4*>(tile + (vector / 8) * (kAttnTile * 128) + row * 128 + (vector % 8) * 16);
+                    if (row >= end) {
+                        *place = make_uint4(0, 0, 0, 0);
+                        continue;
+                    }
+                    uint4 v = *place;
+                    uint32_t words[4] = {v.x, v.y, v.z, v.w};
+                    bool hit = false;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        constexpr uint32_t kExp = Element<T>::kExponent;
+                        if ((words[w] & kExp) == kExp) {
+                            words[w] &= 0xffff0000u;
+                            hit = true;
+                        }
+                        if ((words[w] & (kExp << 16)) == (kExp << 16)) {
+                            words[w] &= 0x0000ffffu;
+                            hit = true;
+                        }
+                    }
+                    if (hit) *place = make_uint4(words[0], words[1], words[2], words[3]);
+                    found |= hit;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                found = __any_sync(0xffffffffu, found) != 0;
+                if (lane == 0) {
+                    if (found) *reinterpret_cast<volatile int*>(&sh.poison[sequence % kAttnPoison]) = sequence;
+                    mbar_arrive(&sh.kv_full[stage]);
+                }
+                __syncwarp();
+            }
+            ring += 2 * item.tiles;
+        }
+    } else {
+        // ============================================================ softmax
+        const int x = warp >> 2;                      // lane A or B
+        const int row = (warp & 3) * 32 + lane;
+        const int token_of_row = row / p.group, head_of_row = row - token_of_row * p.group;
+        const uint32_t tmem_row = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+        const uint32_t tmem_s = tmem_row + kAttnColumnS + x * 128;
+        const uint32_t tmem_o = tmem_row + kAttnColumnO + x * 128;
+        const float scale = p.scale_log2;
+        const float lazy = kAttnLazy / scale;
+        int steps = 0, items = 0, sequence = 0;
+        while (ok && walk.next(p, item, head)) {
+            const AttnLanes l = attn_lanes(item, p.tile_tokens);
+            ++sequence;
+            const int token = token_of_row + (l.pair ? x * p.tile_tokens : 0);      // of the item
+            const bool valid = token_of_row < p.tile_tokens && token < item.tokens;
+            const bool active = __any_sync(0xffffffffu, valid) != 0;
+            const int visible = max(0, min(item.keys, item.visible + item.slope * token));
+            const int tiles = l.tiles[x];
+            float top = -INFINITY, base = 0.0f, total = 0.0f;     // raw maximum in use, the same scaled, sum of weights
+            for (int j = 0; j < tiles; ++j) {
+                ok = wait(&sh.s_full[x], steps & 1);
+                ++steps;
+                if (!ok) break;
+                tcgen05_fence_after_sync();
+                if (active) {
+                    const int t = item.tile_begin + (l.pair ? j : 2 * j + x);
+                    const int limit = visible - t * kAttnTile;
+                    uint32_t s[4][32];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tmem_load_32(tmem_s + c * 32, s[c]);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tmem_load_wait(s[c]);
+                    if (__any_sync(0xffffffffu, limit < kAttnTile)) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (c * 32 + i >= limit) s[c][i] = 0xff800000u;
+                    }
+                    float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) most[c] = fmaxf(most[c], __uint_as_float(s[c][i]));
+                    const float tile_top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+                    if (j == 0) {
+                        top = tile_top;
+                        base = top == -INFINITY ? 0.0f : top * scale;
+                    } else {
+                        const bool moves = tile_top > top + lazy;
+                        if (__any_sync(0xffffffffu, moves)) {
+                            float shrink = 1.0f;
+                            if (moves) {
+                                const float new_base = tile_top * scale;
+                                shrink = top == -INFINITY ? 0.0f : exp2_fast(base - new_base);
+                                top = tile_top;
+                                base = new_base;
+                                total *= shrink;
+                            }
+#pragma unroll 1
+                            for (int c = 0; c < DIM; c += 8) {      // in small pieces: S sits in 128 registers
+                                uint32_t o[8];
+                                tmem_load_8(tmem_o + c, o);
+                                tmem_load_wait8(o);
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * shrink);
+                                tmem_store_8(tmem_o + c, o);
+                            }
+                        }
+                    }
+                    const float2 scale2 = make_float2(scale, scale), base2 = make_float2(-base, -base);
+                    float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t packed[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const float2 z = fma2(make_float2(__uint_as_float(s[c][2 * i]), __uint_as_float(s[c][2 * i + 1])), scale2, base2);
+                            const float low = exp2_fast(z.x), high = exp2_fast(z.y);
+                            sums[(i & 1) * 2] += low;
+                            sums[(i & 1) * 2 + 1] += high;
+                            packed[i] = Element<T>::pack(low, high);
+                        }
+                        tmem_store_16(tmem_s + c * 16, packed);
+                    }
+                    total += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+                    tmem_store_wait();
+                }
+                tcgen05_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.p_full[x]);
+            }
+            if (!ok) break;
+
+            // ------------------------------------------------------ epilogue
+            if (tiles > 0) {
+                ok = wait(&sh.o_full[x], items & 1);
+                ++items;
+                if (!ok) break;
+                tcgen05_fence_after_sync();
+            }
+            const bool direct = item.partial < 0;
+            // lane B of a split item has rows of its own only among partial results
+            const bool writes = active && item.partial != -2 && (l.pair || x == 0 || (!direct && item.slots > 1));
+            const int head_index = head * p.group + head_of_row;
+            const long long out_token = item.q_first + token;
+            const bool empty = total == 0.0f;
+            const float inverse = empty ? 0.0f : 1.0f / total;
+            long long partial_row = 0;
+            bool stores = valid && writes;
+            if (!direct) {
+                const int rows = item.tokens * p.group;
+                const int slot = item.slot + (l.pair ? 0 : x);
+                // a split entry of single-tile chunks has one slot per chunk: lane A's
+                if (!l.pair && x == 1 && slot >= item.slots) stores = false;
+                partial_row = item.partial + (static_cast<long long>(head) * item.slots + slot) * rows + token * p.group + head_of_row;
+            }
+            const bool poisoned = tiles > 0 && *reinterpret_cast<volatile int*>(&sh.poison[sequence % kAttnPoison]) == sequence;
+            if (writes) {
+#pragma unroll 1
+                for (int c = 0; c < DIM / 32; ++c) {
+                    uint32_t o[32];
+                    if (tiles > 0) {
+                        tmem_load_32(tmem_o + c * 32, o);
+                        tmem_load_wait(o);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = empty ? 0u : __float_as_uint(__uint_as_float(o[i]) * inverse);
+                    if (poisoned && valid) {
+                        const int from = max(l.first_visible, item.tile_begin * kAttnTile);
+                        const int to = min(visible, (item.tile_begin + item.tiles) * kAttnTile);
+#pragma unroll 1
+                        for (int key = from; key < to; ++key) {
+                            if (!l.pair && (((key / kAttnTile - item.tile_begin) & 1) != x)) continue;
+                            const uint32_t* source = reinterpret_cast<const uint32_t*>(attn_value_row<T>(p, item, head, key) + c * 32);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const uint32_t word = source[i];
+                                constexpr uint32_t kExp = Element<T>::kExponent;
+                                if ((word & kExp) == kExp) o[2 * i] = __float_as_uint(__uint_as_float(o[2 * i]) + Element<T>::value(word & 0xffffu));
+                                if ((word >> 16 & kExp) == kExp)
+                                    o[2 * i + 1] = __float_as_uint(__uint_as_float(o[2 * i + 1]) + Element<T>::value(word >> 16));
+                            }
+                        }
+                    }
+                    if (stores && direct) {
+                        T* out = static_cast<T*>(p.a.out) + out_token * p.a.out_token_stride + head_index * p.a.out_head_stride + c * 32;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                w[k] = Element<T>::pack(__uint_as_float(o[8 * i + 2 * k]), __uint_as_float(o[8 * i + 2 * k + 1]));
+                            reinterpret_cast<uint4*>(out)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    } else if (stores && !empty) {
+                        uint4* out = reinterpret_cast<uint4*>(p.w.partial_out + partial_row * DIM + c * 32);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) out[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                     }
                 }
-                const T* k_row = static_cast<const T*>(seg.k) + page * seg.k_page_stride + row * seg.k_row_stride + kv_head * seg.k_head_stride;
-                v_row = static_cast<const T*>(seg.v) + page * seg.v_page_stride + row * seg.v_row_stride + kv_head * seg.v_head_stride;
-                float dot = 0.0f;
-                for (int c = 0; c < DIM; c += 8) {
-                    const uint4 raw = *reinterpret_cast<const uint4*>(k_row + c);
-                    const T* x = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) dot = fmaf(q_row[c + i], to_float<T>(x[i]), dot);
+                if (stores) {
+                    const float lse2 = empty ? -INFINITY : base + log2f(total);
+                    if (!direct) {
+                        p.w.partial_lse[partial_row] = lse2;
+                    } else if (p.a.lse != nullptr) {
+                        p.a.lse[out_token * p.a.heads + head_index] = lse2 * kLn2;
+                    }
                 }
-                score = dot * p.scale;
             }
-            float tile_top = score;
-            for (int step = 16; step > 0; step >>= 1) tile_top = fmaxf(tile_top, __shfl_xor_sync(0xffffffffu, tile_top, step));
-            const float new_top = fmaxf(top, tile_top);
-            const float base_top = new_top == -INFINITY ? 0.0f : new_top;
-            const float shrink = expf(top - base_top);
-            const float weight = key < keys ? expf(score - base_top) : 0.0f;
-            top = new_top;
-            total = total * shrink + weight;
-#pragma unroll
-            for (int i = 0; i < kOwn; ++i) sums[i] *= shrink;
-            const int count = min(32, keys - base);
-            for (int j = 0; j < count; ++j) {
-                const float w = __shfl_sync(0xffffffffu, weight, j);
-                const T* row = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(v_row), j));
-#pragma unroll
-                for (int i = 0; i < kOwn; ++i) sums[i] = fmaf(w, to_float<T>(row[lane + 32 * i]), sums[i]);
+            if (tiles > 0) {
+                tcgen05_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.o_empty[x]);
             }
         }
     }
-    for (int step = 16; step > 0; step >>= 1) total += __shfl_xor_sync(0xffffffffu, total, step);
-    const bool empty = total == 0.0f;
+    if (!ok && lane == 0) {
+        sh.abort = 1;
+        atomicOr(p.status, ITK_SERVING_WAIT_EXPIRED);
+    }
+
+    // ---------------------------------------------------------------- teardown
+    __syncwarp();
+    tcgen05_fence_before_sync();
+    __syncthreads();
+    if (warp == kAttnMmaWarp) {
+        if (sh.abort != 0) {
+            // a wait expired: copies and UMMAs issued before that may still be in flight; neither shared
+            // memory nor TMEM is given up under them
+            const uint64_t until = global_timer_ns() + 2000000ull;
+            while (global_timer_ns() < until) {
+            }
+        }
+        __syncwarp();
+        tcgen05_fence_after_sync();
+        tmem_dealloc(tmem, kAttnTmemColumns);
+    }
+}
+
+// ------------------------------------------------------------------ join
+
+constexpr int kJoinThreads = 256;
+
+// out = sum_c 2^(lse_c - lse) out_c over the slots of a row (own ones, then the prefix's), in slot order.  One warp
+// per row; also clears the rows behind the last request when asked to.
+template <typename T, int DIM>
+__global__ void __launch_bounds__(kJoinThreads) itk_attention_join_kernel(const __grid_constant__ AttnParams p) {
+    constexpr int kOwn = DIM / 32;
+    const AttnCounters counters = *p.w.counters;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int span = 2 * p.tile_tokens;
+    const int heads = p.a.kv_heads;
+    for (int work = blockIdx.x; work < counters.combines * heads; work += gridDim.x) {
+        const AttnCombine entry = p.w.combines[work / heads];
+        const int head = work % heads;
+        const int rows = entry.tokens * p.group;
+        for (int r = warp; r < rows; r += kJoinThreads / 32) {
+            const int token = entry.q_first + r / p.group;
+            const int head_index = head * p.group + r % p.group;
+            // two runs of partial rows: first row, distance, count
+            long long first[2] = {entry.partial + static_cast<long long>(head) * entry.slots * rows + r, 0};
+            int step[2] = {rows, 0}, count[2] = {entry.slots, 0};
+            if (p.a.prefix_keys > 0) {
+                const int e = token / span;
+                const int2 slots = p.w.prefix_slots[e];
+                const int prefix_rows = min(span, counters.rows_end - e * span) * p.group;
+                first[1] = slots.x + static_cast<long long>(head) * slots.y * prefix_rows + (token - e * span) * p.group + r % p.group;
+                step[1] = prefix_rows;
+                count[1] = slots.y;
+            }
+            float top = -INFINITY;
+            bool broken = false;
+            for (int run = 0; run < 2; ++run)
+                for (int c = lane; c < count[run]; c += 32) {
+                    const float lse = p.w.partial_lse[first[run] + static_cast<long long>(c) * step[run]];
+                    broken |= lse != lse;
+                    top = fmaxf(top, lse);
+                }
 #pragma unroll
-    for (int i = 0; i < kOwn; ++i) out[lane + 32 * i] = from_float<T>(empty ? 0.0f : sums[i] / total);
-    if (lane == 0 && p.lse != nullptr) p.lse[work] = empty ? -INFINITY : top + logf(total);
+            for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            broken = __any_sync(0xffffffffu, broken) != 0;
+            float total = 0.0f, sums[kOwn] = {};
+            if (top > -INFINITY) {
+                for (int run = 0; run < 2; ++run)
+                    for (int base = 0; base < count[run]; base += 32) {
+                        float weight = 0.0f;
+                        if (base + lane < count[run])
+                            weight = exp2_fast(p.w.partial_lse[first[run] + static_cast<long long>(base + lane) * step[run]] - top);
+                        const int here = min(32, count[run] - base);
+#pragma unroll 4
+                        for (int c = 0; c < here; ++c) {
+                            const float w = __shfl_sync(0xffffffffu, weight, c);
+                            if (w == 0.0f) continue;       // an empty slot holds no values
+                            const float* source = p.w.partial_out + (first[run] + static_cast<long long>(base + c) * step[run]) * DIM + lane * kOwn;
+                            float held[kOwn];
+                            if constexpr (kOwn == 4) {
+                                *reinterpret_cast<float4*>(held) = *reinterpret_cast<const float4*>(source);
+                            } else {
+                                *reinterpret_cast<float2*>(held) = *reinterpret_cast<const float2*>(source);
+                            }
+                            total += w;
+#pragma unroll
+                            for (int i = 0; i < kOwn; ++i) sums[i] = fmaf(w, held[i], sums[i]);
+                        }
+                    }
+            }
+            const bool empty = total == 0.0f && !broken;
+            const float nan = __int_as_float(0x7fffffff);
+            const float inverse = broken ? nan : (empty ? 0.0f : 1.0f / total);
+            uint32_t packed[kOwn / 2];
+#pragma unroll
+            for (int i = 0; i < kOwn / 2; ++i) packed[i] = Element<T>::pack(sums[2 * i] * inverse, sums[2 * i + 1] * inverse);
+            T* out = static_cast<T*>(p.a.out) + token * p.a.out_token_stride + head_index * p.a.out_head_stride + lane * kOwn;
+            if constexpr (kOwn == 4) {
+                *reinterpret_cast<uint2*>(out) = make_uint2(packed[0], packed[1]);
+            } else {
+                *reinterpret_cast<uint32_t*>(out) = packed[0];
+            }
+            if (lane == 0 && p.a.lse != nullptr)
+                p.a.lse[static_cast<long long>(token) * p.a.heads + head_index] = broken ? nan : (empty ? -INFINITY : (top + log2f(total)) * kLn2);
+        }
+    }
+    if (p.a.clear_tail) {
+        const long long begin = static_cast<long long>(counters.rows_end) * p.a.heads, end = static_cast<long long>(p.a.tokens) * p.a.heads;
+        for (long long r = begin + static_cast<long long>(blockIdx.x) * (kJoinThreads / 32) + warp; r < end;
+             r += static_cast<long long>(gridDim.x) * (kJoinThreads / 32)) {
+            const long long token = r / p.a.heads, head = r - token * p.a.heads;
+            T* out = static_cast<T*>(p.a.out) + token * p.a.out_token_stride + head * p.a.out_head_stride + lane * kOwn;
+            if constexpr (kOwn == 4) {
+                *reinterpret_cast<uint2*>(out) = make_uint2(0u, 0u);
+            } else {
+                *reinterpret_cast<uint32_t*>(out) = 0u;
+            }
+            if (lane == 0 && p.a.lse != nullptr) p.a.lse[r] = -INFINITY;
+        }
+    }
 }
 
 }  // namespace itk

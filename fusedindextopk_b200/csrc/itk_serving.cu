@@ -25,6 +25,11 @@ struct DeviceState {
 std::mutex g_device_mutex;
 DeviceState g_devices[kMaxDevices];
 
+template <typename Kernel>
+cudaError_t raise_smem(Kernel kernel, int bytes) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
 int current_device(DeviceState* state) {
     int device = 0;
     ITK_CUDA(cudaGetDevice(&device));
@@ -41,6 +46,10 @@ int current_device(DeviceState* state) {
         d.status = static_cast<int*>(address);
         ITK_CUDA(cudaFuncSetAttribute(itk_plan_pages_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (3 * ITK_MAX_PLAN_REQUESTS + 1) * static_cast<int>(sizeof(int))));
+        ITK_CUDA(raise_smem(itk_attention_kernel<__nv_bfloat16, 128>, AttnShape<128>::kSmemBytes));
+        ITK_CUDA(raise_smem(itk_attention_kernel<__nv_bfloat16, 64>, AttnShape<64>::kSmemBytes));
+        ITK_CUDA(raise_smem(itk_attention_kernel<__half, 128>, AttnShape<128>::kSmemBytes));
+        ITK_CUDA(raise_smem(itk_attention_kernel<__half, 64>, AttnShape<64>::kSmemBytes));
         d.ready = true;
     }
     *state = d;
@@ -85,6 +94,74 @@ int check_attention(const itk_attention_args& a) {
     ITK_REQUIRE(a.element == ITK_ELEMENT_BF16 || a.element == ITK_ELEMENT_FP16, "element must be bf16 or fp16");
     ITK_REQUIRE(static_cast<long long>(a.tokens) * a.heads < (1ll << 31), "tokens * heads must stay below 2^31");
     return ITK_OK;
+}
+
+constexpr int kAttnMaxSms = 256;     // the workspace is sized for any device the library runs on
+
+// Workspace of a call: what the plan kernel can write at most.  With T tokens, B requests and 2 TT tokens per entry
+// there are at most T / (2 TT) + B own entries; the prefix has T / (2 TT) + 1.  Chunking adds at most one item per SM
+// (a chunk costs at least a fair share of the work).  Partial rows: a split entry (at most one per request, at most
+// 128 rows per key head) has two lanes; chunks add at most two row tiles per SM and as many again for the rounding of
+// entries that are cut; with a prefix every own row and every prefix row has one more, two in split entries.
+int attention_workspace(const itk_attention_args& a, AttnWorkspace* w, size_t* bytes) {
+    const long long tile_tokens = kAttnTile / (a.heads / a.kv_heads), span = 2 * tile_tokens;
+    const long long rows = static_cast<long long>(a.tokens) * a.heads;
+    const long long own = a.tokens / span + a.requests, prefix = a.prefix_keys > 0 ? a.tokens / span + 1 : 0;
+    long long partial = 2 * std::min(rows, static_cast<long long>(a.requests) * kAttnTile * a.kv_heads) + 2ll * kAttnMaxSms * 2 * kAttnTile;
+    if (prefix > 0) partial += 3 * rows;
+    ITK_REQUIRE(partial < (1ll << 31) - 1 && own + prefix < (1ll << 28), "the batch is too large for one call");
+    size_t at = 0;
+    auto take = [&](size_t size) {
+        const size_t offset = at;
+        at += (size + 255) / 256 * 256;
+        return static_cast<char*>(a.workspace) + offset;
+    };
+    w->max_combines = static_cast<int>(own);
+    w->max_items = static_cast<int>(own + prefix + kAttnMaxSms);
+    w->max_partial_rows = static_cast<int>(partial);
+    w->counters = reinterpret_cast<AttnCounters*>(take(sizeof(AttnCounters)));
+    w->entry_first = reinterpret_cast<int*>(take((static_cast<size_t>(a.requests) + 1) * sizeof(int)));
+    w->prefix_slots = reinterpret_cast<int2*>(take(static_cast<size_t>(prefix) * sizeof(int2)));
+    w->items = reinterpret_cast<AttnItem*>(take(static_cast<size_t>(w->max_items) * sizeof(AttnItem)));
+    w->combines = reinterpret_cast<AttnCombine*>(take(static_cast<size_t>(own) * sizeof(AttnCombine)));
+    w->partial_lse = reinterpret_cast<float*>(take(static_cast<size_t>(partial) * sizeof(float)));
+    w->partial_out = reinterpret_cast<float*>(take(static_cast<size_t>(partial) * a.dim * sizeof(float)));
+    *bytes = at;
+    return ITK_OK;
+}
+
+int encode_map(CUtensorMap* map, int element, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
+               const cuuint32_t* box) {
+    EncodeTiled encode = encode_tiled_entry();
+    if (encode == nullptr) return fail(ITK_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint32_t ones[4] = {1, 1, 1, 1};
+    const CUresult result = encode(
+        map, element == ITK_ELEMENT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+        static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (result != CUDA_SUCCESS) return fail(ITK_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", int(result));
+    return ITK_OK;
+}
+
+// Bytes between the entries of a dimension; one with a single entry may carry any stride, which nothing steps over.
+cuuint64_t map_stride(long long elements, long long count) { return count > 1 || elements > 0 ? elements * 2 : 16; }
+
+// [pages, page_size, kv_heads, dim] in any order of strides; a box is 128 rows of 64 columns of one head.
+int segment_map(CUtensorMap* map, const itk_attention_args& a, const itk_kv_segment& s, const void* base, long long page_stride,
+                long long row_stride, long long head_stride) {
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.dim), static_cast<cuuint64_t>(a.kv_heads),
+                                static_cast<cuuint64_t>(s.page_size), static_cast<cuuint64_t>(s.pages)};
+    const cuuint64_t strides[3] = {map_stride(head_stride, a.kv_heads), map_stride(row_stride, s.page_size), map_stride(page_stride, s.pages)};
+    const cuuint32_t box[4] = {64, 1, kAttnTile, 1};
+    return encode_map(map, a.element, 4, base, dims, strides, box);
+}
+
+template <typename T, int DIM>
+int launch_attention(const AttnParams& params, cudaStream_t stream) {
+    itk_attention_plan_kernel<<<1, kAttnPlanThreads, 0, stream>>>(params);
+    itk_attention_kernel<T, DIM><<<params.sm_count, kAttnThreads, AttnShape<DIM>::kSmemBytes, stream>>>(params);
+    itk_attention_join_kernel<T, DIM><<<4 * params.sm_count, kJoinThreads, 0, stream>>>(params);
+    return launched("itk_attention_kernel");
 }
 
 }  // namespace
@@ -159,8 +236,8 @@ int itk_attention_workspace_bytes(const itk_attention_args* args, size_t* bytes)
     ITK_REQUIRE(args != nullptr && bytes != nullptr, "args and bytes must not be null");
     const int rc = check_attention(*args);
     if (rc != ITK_OK) return rc;
-    *bytes = 0;
-    return ITK_OK;
+    AttnWorkspace ignored;
+    return attention_workspace(*args, &ignored, bytes);
 }
 
 int itk_attention(const itk_attention_args* args, itk_stream_t stream) {
@@ -185,19 +262,49 @@ int itk_attention(const itk_attention_args* args, itk_stream_t stream) {
         if ((rc = check_segment(a.prefix, "prefix keys")) != ITK_OK) return rc;
         const long long room = a.prefix.table != nullptr ? static_cast<long long>(a.prefix.table_pages) * a.prefix.page_size : a.prefix.page_size;
         ITK_REQUIRE(a.prefix_keys <= room, "prefix_keys exceeds the prefix");
+    } else {
+        ITK_REQUIRE(a.prefix_keys == 0, "prefix keys: keys and values must not be null");
     }
+    ITK_REQUIRE(a.scale > 0.0f && a.scale * kLog2e <= 3.0e38f, "scale must be positive and finite");
     DeviceState device;
     if ((rc = current_device(&device)) != ITK_OK) return rc;
-    const long long rows = static_cast<long long>(a.tokens) * a.heads;
-    const unsigned grid = static_cast<unsigned>((rows + 3) / 4);
-    if (a.element == ITK_ELEMENT_BF16) {
-        if (a.dim == 128) itk_attention_rows_kernel<__nv_bfloat16, 128><<<grid, kRowsKernelThreads, 0, stream>>>(a, device.status);
-        else itk_attention_rows_kernel<__nv_bfloat16, 64><<<grid, kRowsKernelThreads, 0, stream>>>(a, device.status);
-    } else {
-        if (a.dim == 128) itk_attention_rows_kernel<__half, 128><<<grid, kRowsKernelThreads, 0, stream>>>(a, device.status);
-        else itk_attention_rows_kernel<__half, 64><<<grid, kRowsKernelThreads, 0, stream>>>(a, device.status);
+    AttnParams params;
+    size_t needed = 0;
+    if ((rc = attention_workspace(a, &params.w, &needed)) != ITK_OK) return rc;
+    ITK_REQUIRE(a.workspace != nullptr && (reinterpret_cast<uintptr_t>(a.workspace) & 255u) == 0 && a.workspace_bytes >= needed,
+                "the workspace must be 256-byte aligned and hold %zu bytes", needed);
+    params.a = a;
+    params.status = device.status;
+    params.group = a.heads / a.kv_heads;
+    params.tile_tokens = kAttnTile / params.group;
+    params.sm_count = std::min(device.sm_count, kAttnMaxSms);
+    params.withhold_loads = a.withhold_loads;
+    params.scale_log2 = a.scale * kLog2e;
+    params.wait_limit_ns = a.wait_limit_ns != 0 ? a.wait_limit_ns : kWaitLimitNs;
+    {
+        const cuuint64_t dims[3] = {static_cast<cuuint64_t>(a.dim), static_cast<cuuint64_t>(a.heads), static_cast<cuuint64_t>(a.tokens)};
+        const cuuint64_t strides[2] = {map_stride(a.q_head_stride, a.heads), map_stride(a.q_token_stride, a.tokens)};
+        const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(params.group), static_cast<cuuint32_t>(params.tile_tokens)};
+        if ((rc = encode_map(&params.map_q, a.element, 3, a.q, dims, strides, box)) != ITK_OK) return rc;
     }
-    return launched("itk_attention_rows_kernel");
+    if (a.own.k != nullptr) {
+        const itk_kv_segment& s = a.own;
+        if ((rc = segment_map(&params.map_k, a, s, s.k, s.k_page_stride, s.k_row_stride, s.k_head_stride)) != ITK_OK) return rc;
+        if ((rc = segment_map(&params.map_v, a, s, s.v, s.v_page_stride, s.v_row_stride, s.v_head_stride)) != ITK_OK) return rc;
+    } else {        // no own key: no item loads through these
+        params.map_k = params.map_v = params.map_q;
+    }
+    if (a.prefix_keys > 0) {
+        const itk_kv_segment& s = a.prefix;
+        if ((rc = segment_map(&params.map_k_prefix, a, s, s.k, s.k_page_stride, s.k_row_stride, s.k_head_stride)) != ITK_OK) return rc;
+        if ((rc = segment_map(&params.map_v_prefix, a, s, s.v, s.v_page_stride, s.v_row_stride, s.v_head_stride)) != ITK_OK) return rc;
+    } else {
+        params.map_k_prefix = params.map_k;
+        params.map_v_prefix = params.map_v;
+    }
+    if (a.element == ITK_ELEMENT_BF16)
+        return a.dim == 128 ? launch_attention<__nv_bfloat16, 128>(params, stream) : launch_attention<__nv_bfloat16, 64>(params, stream);
+    return a.dim == 128 ? launch_attention<__half, 128>(params, stream) : launch_attention<__half, 64>(params, stream);
 }
 
 }  // extern "C"

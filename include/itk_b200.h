@@ -430,12 +430,13 @@ typedef struct itk_attention_args {
     void* workspace;
     size_t workspace_bytes;
     long long q_token_stride, q_head_stride, out_token_stride, out_head_stride;
-    unsigned long long wait_limit_ns;   /* 0 = default */
+    unsigned long long wait_limit_ns;   /* 0 = default (2 s) */
     itk_kv_segment own;
     itk_kv_segment prefix;     /* k = null: no prefix */
     float scale;
     int element;               /* ITK_ELEMENT_* */
     int tokens, heads, kv_heads, dim, requests, prefix_keys, causal, clear_tail;
+    int withhold_loads;        /* test only: the producer loads nothing, so that a wait expires */
 } itk_attention_args;
 int itk_attention(const itk_attention_args* args, itk_stream_t stream);
 /* Bytes of workspace a call with these sizes needs (the pointers are not looked at). */

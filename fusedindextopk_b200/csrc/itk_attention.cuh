@@ -45,7 +45,8 @@ constexpr int kAttnThreads = 352;
 constexpr int kAttnSoftmaxWarps = 4;           // per lane
 constexpr int kAttnMmaWarp = 8, kAttnLoadWarp = 9, kAttnGuardWarp = 10;
 constexpr int kAttnTmemColumns = 512;
-constexpr int kAttnColumnS = 0, kAttnColumnO = 256;   // lane B: + 128
+constexpr int kAttnHalf = 64;                  // keys of a step: half a tile
+constexpr int kAttnColumnS = 0, kAttnColumnO = 256;   // lane B: + 128; step i of a lane uses S columns 64 * (i % 2)
 constexpr int kAttnMaxStages = 10;
 constexpr int kAttnPoison = 16;                // items the guard may be ahead of an epilogue, with room to spare
 constexpr float kAttnLazy = 8.0f;              // log2 of how far weights may exceed 1 before the maximum moves
@@ -104,6 +105,17 @@ struct AttnParams {
 
 // ------------------------------------------------------------------ PTX
 
+// True in one thread of the warp, always the same one.  The tcgen05 instructions take their operands from uniform
+// registers: under this predicate, with operands that come out of a broadcast, they are moved there once; under a
+// comparison with the lane id every issue paid about 100 cycles (4 UMMAs and two commits: 590 cycles).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t elected;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
+    return elected != 0;
+}
+
+__device__ __forceinline__ int uniform(int value) { return __shfl_sync(0xffffffffu, value, 0); }
+
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
@@ -152,36 +164,36 @@ __device__ __forceinline__ void umma_16bit_ts(uint32_t tmem_d, uint32_t tmem_a, 
         : "memory");
 }
 
-__device__ __forceinline__ void tmem_store_16(uint32_t tmem_address, const uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_store_32(uint32_t tmem_address, const uint32_t (&r)[32]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
         ::"r"(tmem_address), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+          "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]),
+          "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
 
-__device__ __forceinline__ void tmem_load_8(uint32_t tmem_address, uint32_t (&r)[8]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                 : "r"(tmem_address)
-                 : "memory");
-}
-
-__device__ __forceinline__ void tmem_load_wait8(uint32_t (&r)[8]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
-                 :
-                 : "memory");
-}
-
-__device__ __forceinline__ void tmem_store_8(uint32_t tmem_address, const uint32_t (&r)[8]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-                 ::"r"(tmem_address), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-                 : "memory");
-}
-
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Maximum of three; a NaN among them is passed over.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t ra, rb, rd;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(ra) : "f"(a.x), "f"(a.y));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(rb) : "f"(b.x), "f"(b.y));
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(rd) : "l"(ra), "l"(rb));
+    float2 d;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(rd));
+    return d;
+}
 
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
@@ -464,7 +476,8 @@ __global__ void __launch_bounds__(kAttnPlanThreads) itk_attention_plan_kernel(co
 struct AttnShared {
     uint64_t q_full[2], q_empty[2];
     uint64_t kv_full[kAttnMaxStages], kv_empty[kAttnMaxStages], guard_full[kAttnMaxStages];
-    uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
+    uint64_t s_full[2][2], p_full[2][2];      // lane, step parity
+    uint64_t pv_done[2], o_full[2], o_empty[2];
     int poison[kAttnPoison];
     uint32_t tmem_base;
     int abort;
@@ -550,7 +563,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
     uint8_t* smem_q = smem;
     uint8_t* smem_kv = smem + 2 * Shape::kTileBytes;
     AttnShared& sh = *reinterpret_cast<AttnShared*>(smem + Shape::kSmemTiles);
-    const int warp = static_cast<int>(threadIdx.x) >> 5;
+    const int warp = uniform(static_cast<int>(threadIdx.x) >> 5);
     const int lane = static_cast<int>(threadIdx.x) & 31;
 
     if ((smem_u32(smem) & 1023u) != 0u) {   // the same in every thread
@@ -563,8 +576,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh.q_full[i], 1);
             mbar_init(&sh.q_empty[i], 1);
-            mbar_init(&sh.s_full[i], 1);
-            mbar_init(&sh.p_full[i], kAttnSoftmaxWarps);
+            for (int h = 0; h < 2; ++h) {
+                mbar_init(&sh.s_full[i][h], 1);
+                mbar_init(&sh.p_full[i][h], kAttnSoftmaxWarps);
+            }
+            mbar_init(&sh.pv_done[i], 1);
             mbar_init(&sh.o_full[i], 1);
             mbar_init(&sh.o_empty[i], kAttnSoftmaxWarps);
         }
@@ -587,11 +603,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
     tcgen05_fence_before_sync();
     __syncthreads();
     tcgen05_fence_after_sync();
-    const uint32_t tmem = sh.tmem_base;
+    const uint32_t tmem = static_cast<uint32_t>(uniform(static_cast<int>(sh.tmem_base)));
     volatile int* abort_flag = &sh.abort;
     // a wait of the whole warp: its lanes leave together
     auto wait = [&](uint64_t* bar, uint32_t parity) {
         return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.wait_limit_ns)) != 0;
+    };
+    auto hot_wait = [&](uint64_t* bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, mbar_wait<kHotWait>(bar, parity, abort_flag, p.wait_limit_ns)) != 0;
     };
     bool ok = true;
     AttnItem item;
@@ -648,70 +667,78 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
         }
     } else if (warp == kAttnMmaWarp) {
         // ============================================================ UMMA issuer
-        constexpr uint32_t kIdescS = umma_idesc_16bit(Element<T>::kBf16, kAttnTile, false);
+        constexpr uint32_t kIdescS = umma_idesc_16bit(Element<T>::kBf16, kAttnHalf, false);
         constexpr uint32_t kIdescO = umma_idesc_16bit(Element<T>::kBf16, DIM, true);
-        int ring = 0, items_of[2] = {0, 0}, steps_of[2] = {0, 0}, q_uses[2] = {0, 0};
+        int ring = 0, items_of[2] = {0, 0}, q_uses[2] = {0, 0};
+        const uint32_t q_base = smem_u32(smem_q), kv_base = smem_u32(smem_kv);
+        uint32_t p_phases = 0;        // bit 2 x + h: parity of the next P of lane x, buffer h
         while (ok && walk.next(p, item, head)) {
             const AttnLanes l = attn_lanes(item, p.tile_tokens);
             if (item.tiles == 0) continue;
             for (int tile = 0; ok && tile < (l.pair ? 2 : 1); ++tile) {
-                ok = wait(&sh.q_full[tile], q_uses[tile] & 1);
+                ok = hot_wait(&sh.q_full[tile], q_uses[tile] & 1);
                 ++q_uses[tile];
             }
-            // S of lane x for its key tile j; the key tile is released when its last reader has been issued
-            auto scores = [&](int x, int j) {
-                const int t = l.pair ? j : 2 * j + x;
-                const int at = ring + ring_key(l.pair, t);
+            const bool pair = uniform(l.pair) != 0;
+            const int tiles = uniform(item.tiles);
+            const int steps[2] = {uniform(2 * l.tiles[0]), uniform(2 * l.tiles[1])};
+            // S of lane x for its step i; the key tile is released when its last reader has been issued
+            auto scores = [&](int x, int i) {
+                const int t = pair ? i >> 1 : 2 * (i >> 1) + x, h = i & 1;
+                const int at = ring + ring_key(pair, t);
                 const int stage = at % kStages;
-                ok = ok && wait(&sh.kv_full[stage], (at / kStages) & 1);
+                ok = ok && hot_wait(&sh.kv_full[stage], (at / kStages) & 1);
                 if (!ok) return;
                 tcgen05_fence_after_sync();
-                if (lane == 0) {
-                    const uint32_t a = smem_u32(smem_q + (l.pair ? x : 0) * Shape::kTileBytes);
-                    const uint32_t b = smem_u32(smem_kv + stage * Shape::kTileBytes);
+                const uint64_t a = umma_desc_sw128_kmajor(q_base + (pair ? x : 0) * Shape::kTileBytes);
+                const uint64_t b = umma_desc_sw128_kmajor(kv_base + stage * Shape::kTileBytes + h * (kAttnHalf * 128));
+                if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < DIM / 16; ++k) {
-                        const uint32_t offset = (k / 4) * (kAttnTile * 128) + (k % 4) * 32;
-                        umma_16bit_ss(tmem + kAttnColumnS + x * 128, umma_desc_sw128_kmajor(a + offset),
-                                      umma_desc_sw128_kmajor(b + offset), kIdescS, k > 0);
+                        constexpr int kChunkStep = (kAttnTile * 128) >> 4;
+                        const int offset = (k / 4) * kChunkStep + (k % 4) * 2;      // 16-byte units: 32 bytes per K step
+                        umma_16bit_ss(tmem + kAttnColumnS + x * 128 + h * kAttnHalf, a + offset, b + offset, kIdescS, k > 0);
                     }
-                    if (!l.pair || x == 1) umma_commit(&sh.kv_empty[stage]);
-                    umma_commit(&sh.s_full[x]);
-                    // the last scores of a row tile: its rows may be replaced
-                    if (t + 1 == item.tiles) umma_commit(&sh.q_empty[l.pair ? x : 0]);
+                    umma_commit(&sh.s_full[x][h]);
+                    if (h == 1) {
+                        if (!pair || x == 1) umma_commit(&sh.kv_empty[stage]);
+                        // the last scores of a row tile: its rows may be replaced
+                        if (t + 1 == tiles) umma_commit(&sh.q_empty[pair ? x : 0]);
+                    }
                 }
                 __syncwarp();
             };
-            scores(0, 0);
-            if (l.tiles[1] > 0) scores(1, 0);
-            for (int j = 0; ok && j < l.tiles[0]; ++j) {
+            for (int i = 0; i < 2; ++i)
+                for (int x = 0; x < 2; ++x)
+                    if (steps[x] > 0) scores(x, i);
+            for (int i = 0; ok && i < steps[0]; ++i) {
                 for (int x = 0; ok && x < 2; ++x) {
-                    if (j >= l.tiles[x]) break;
-                    const int t = l.pair ? j : 2 * j + x;
-                    const int at = ring + ring_value(l.pair, t, item.tiles);
+                    if (i >= steps[x]) break;
+                    const int t = pair ? i >> 1 : 2 * (i >> 1) + x, h = i & 1;
+                    const int at = ring + ring_value(pair, t, tiles);
                     const int stage = at % kStages;
-                    ok = wait(&sh.kv_full[stage], (at / kStages) & 1);
-                    if (ok && j == 0) ok = wait(&sh.o_empty[x], (items_of[x] & 1) ^ 1);
-                    if (ok) ok = wait(&sh.p_full[x], steps_of[x] & 1);
-                    ++steps_of[x];
+                    ok = hot_wait(&sh.kv_full[stage], (at / kStages) & 1);
+                    if (ok && i == 0) ok = hot_wait(&sh.o_empty[x], (items_of[x] & 1) ^ 1);
+                    if (ok) ok = hot_wait(&sh.p_full[x][h], (p_phases >> (2 * x + h)) & 1);
+                    p_phases ^= 1u << (2 * x + h);
                     if (!ok) break;
                     tcgen05_fence_after_sync();
-                    if (lane == 0) {
-                        const uint32_t a = tmem + kAttnColumnS + x * 128;
-                        const uint32_t b = smem_u32(smem_kv + stage * Shape::kTileBytes);
+                    const uint32_t a = tmem + kAttnColumnS + x * 128 + h * kAttnHalf;
+                    const uint64_t b = umma_desc_sw128_mnmajor(kv_base + stage * Shape::kTileBytes + h * (kAttnHalf * 128), kAttnTile * 128);
+                    if (elect_one()) {
 #pragma unroll
-                        for (int k = 0; k < kAttnTile / 16; ++k)
-                            umma_16bit_ts(tmem + kAttnColumnO + x * 128, a + k * 8,
-                                          umma_desc_sw128_mnmajor(b + k * 2048, kAttnTile * 128), kIdescO, j > 0 || k > 0);
-                        if (!l.pair || x == 1) umma_commit(&sh.kv_empty[stage]);
-                        if (j + 1 == l.tiles[x]) umma_commit(&sh.o_full[x]);
+                        for (int k = 0; k < kAttnHalf / 16; ++k)
+                            umma_16bit_ts(tmem + kAttnColumnO + x * 128, a + k * 8, b + k * (2048 >> 4), kIdescO, i > 0 || k > 0);
+                        umma_commit(&sh.pv_done[x]);
+                        if (i + 1 == steps[x]) umma_commit(&sh.o_full[x]);
+                        if (h == 1 && (!pair || x == 1)) umma_commit(&sh.kv_empty[stage]);
                     }
                     __syncwarp();
-                    if (j + 1 == l.tiles[x]) ++items_of[x];
-                    if (j + 1 < l.tiles[x]) scores(x, j + 1);
+                    if (i + 1 == steps[x]) ++items_of[x];
+                    if (i + 2 < steps[x]) scores(x, i + 2);
                 }
             }
-            ring += 2 * item.tiles;
+            ring += 2 * tiles;
         }
     } else if (warp == kAttnGuardWarp) {
         // ============================================================ guard
@@ -778,7 +805,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
         const uint32_t tmem_o = tmem_row + kAttnColumnO + x * 128;
         const float scale = p.scale_log2;
         const float lazy = kAttnLazy / scale;
-        int steps = 0, items = 0, sequence = 0;
+        int steps = 0, items = 0, sequence = 0;       // steps and items with keys of this lane, items of the walk
         while (ok && walk.next(p, item, head)) {
             const AttnLanes l = attn_lanes(item, p.tile_tokens);
             ++sequence;
@@ -787,96 +814,105 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
             const bool active = __any_sync(0xffffffffu, valid) != 0;
             const int visible = max(0, min(item.keys, item.visible + item.slope * token));
             const int tiles = l.tiles[x];
-            float top = -INFINITY, base = 0.0f, total = 0.0f;     // raw maximum in use, the same scaled, sum of weights
-            for (int j = 0; j < tiles; ++j) {
-                ok = wait(&sh.s_full[x], steps & 1);
-                ++steps;
+            float top = -INFINITY, base = 0.0f;           // raw maximum in use, the same scaled
+            float2 total = make_float2(0.0f, 0.0f);       // sum of weights
+            for (int i = 0; i < 2 * tiles; ++i, ++steps) {
+                const int h = i & 1;
+                ok = hot_wait(&sh.s_full[x][h], (steps >> 1) & 1);
                 if (!ok) break;
                 tcgen05_fence_after_sync();
                 if (active) {
-                    const int t = item.tile_begin + (l.pair ? j : 2 * j + x);
-                    const int limit = visible - t * kAttnTile;
-                    uint32_t s[4][32];
+                    const int t = item.tile_begin + (l.pair ? i >> 1 : 2 * (i >> 1) + x);
+                    const int limit = visible - t * kAttnTile - h * kAttnHalf;
+                    const uint32_t tmem_step = tmem_s + h * kAttnHalf;
+                    uint32_t s[2][32];
+                    tmem_load_32(tmem_step, s[0]);
+                    tmem_load_32(tmem_step + 32, s[1]);
+                    tmem_load_wait(s[0]);
+                    tmem_load_wait(s[1]);
+                    if (__any_sync(0xffffffffu, limit < kAttnHalf)) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) tmem_load_32(tmem_s + c * 32, s[c]);
+                        for (int c = 0; c < 2; ++c)
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) tmem_load_wait(s[c]);
-                    if (__any_sync(0xffffffffu, limit < kAttnTile)) {
-#pragma unroll
-                        for (int c = 0; c < 4; ++c)
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (c * 32 + i >= limit) s[c][i] = 0xff800000u;
+                            for (int k = 0; k < 32; ++k)
+                                if (c * 32 + k >= limit) s[c][k] = 0xff800000u;
                     }
-                    float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    float most[4];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
+                    for (int c = 0; c < 4; ++c) {
+                        const uint32_t* part = &s[c >> 1][(c & 1) * 16];
+                        most[c] = fmaxf(__uint_as_float(part[0]), __uint_as_float(part[1]));
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) most[c] = fmaxf(most[c], __uint_as_float(s[c][i]));
-                    const float tile_top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-                    if (j == 0) {
-                        top = tile_top;
+                        for (int k = 2; k < 16; k += 2) most[c] = max3(most[c], __uint_as_float(part[k]), __uint_as_float(part[k + 1]));
+                    }
+                    const float step_top = max3(fmaxf(most[0], most[1]), most[2], most[3]);
+                    if (i == 0) {
+                        top = fmaxf(step_top, -INFINITY);       // a NaN is no maximum; its weight is NaN all the same
                         base = top == -INFINITY ? 0.0f : top * scale;
                     } else {
-                        const bool moves = tile_top > top + lazy;
+                        const bool moves = step_top > top + lazy;
                         if (__any_sync(0xffffffffu, moves)) {
                             float shrink = 1.0f;
                             if (moves) {
-                                const float new_base = tile_top * scale;
+                                const float new_base = step_top * scale;
                                 shrink = top == -INFINITY ? 0.0f : exp2_fast(base - new_base);
-                                top = tile_top;
+                                top = step_top;
                                 base = new_base;
-                                total *= shrink;
+                                total.x *= shrink;
+                                total.y *= shrink;
                             }
+                            // O has to hold the steps up to the one before (S of this step implies all but that one);
+                            // the next P V waits for this step's weights
+                            ok = hot_wait(&sh.pv_done[x], (steps + 1) & 1);
+                            if (!ok) break;
+                            tcgen05_fence_after_sync();
 #pragma unroll 1
-                            for (int c = 0; c < DIM; c += 8) {      // in small pieces: S sits in 128 registers
-                                uint32_t o[8];
-                                tmem_load_8(tmem_o + c, o);
-                                tmem_load_wait8(o);
+                            for (int c = 0; c < DIM; c += 32) {
+                                uint32_t o[32];
+                                tmem_load_32(tmem_o + c, o);
+                                tmem_load_wait(o);
 #pragma unroll
-                                for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * shrink);
-                                tmem_store_8(tmem_o + c, o);
+                                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * shrink);
+                                tmem_store_32(tmem_o + c, o);
                             }
                         }
                     }
                     const float2 scale2 = make_float2(scale, scale), base2 = make_float2(-base, -base);
-                    float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    float2 sums[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                    uint32_t packed[32];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t packed[16];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const float2 z = fma2(make_float2(__uint_as_float(s[c][2 * i]), __uint_as_float(s[c][2 * i + 1])), scale2, base2);
-                            const float low = exp2_fast(z.x), high = exp2_fast(z.y);
-                            sums[(i & 1) * 2] += low;
-                            sums[(i & 1) * 2 + 1] += high;
-                            packed[i] = Element<T>::pack(low, high);
-                        }
-                        tmem_store_16(tmem_s + c * 16, packed);
+                    for (int k = 0; k < 32; ++k) {
+                        const uint32_t* pair = &s[k >> 4][(k & 15) * 2];
+                        const float2 z = fma2(make_float2(__uint_as_float(pair[0]), __uint_as_float(pair[1])), scale2, base2);
+                        const float2 w = make_float2(exp2_fast(z.x), exp2_fast(z.y));
+                        sums[k & 1] = add2(sums[k & 1], w);
+                        packed[k] = Element<T>::pack(w.x, w.y);
                     }
-                    total += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+                    tmem_store_32(tmem_step, packed);
+                    total = add2(total, add2(sums[0], sums[1]));
                     tmem_store_wait();
                 }
                 tcgen05_fence_before_sync();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.p_full[x]);
+                if (lane == 0) mbar_arrive(&sh.p_full[x][h]);
             }
             if (!ok) break;
 
             // ------------------------------------------------------ epilogue
             if (tiles > 0) {
-                ok = wait(&sh.o_full[x], items & 1);
+                ok = hot_wait(&sh.o_full[x], items & 1);
                 ++items;
                 if (!ok) break;
                 tcgen05_fence_after_sync();
             }
+            const float sum = total.x + total.y;
             const bool direct = item.partial < 0;
             // lane B of a split item has rows of its own only among partial results
             const bool writes = active && item.partial != -2 && (l.pair || x == 0 || (!direct && item.slots > 1));
             const int head_index = head * p.group + head_of_row;
             const long long out_token = item.q_first + token;
-            const bool empty = total == 0.0f;
-            const float inverse = empty ? 0.0f : 1.0f / total;
+            const bool empty = sum == 0.0f;
+            const float inverse = empty ? 0.0f : 1.0f / sum;
             long long partial_row = 0;
             bool stores = valid && writes;
             if (!direct) {
@@ -931,7 +967,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
                     }
                 }
                 if (stores) {
-                    const float lse2 = empty ? -INFINITY : base + log2f(total);
+                    const float lse2 = empty ? -INFINITY : base + log2f(sum);
                     if (!direct) {
                         p.w.partial_lse[partial_row] = lse2;
                     } else if (p.a.lse != nullptr) {

@@ -671,7 +671,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
         constexpr uint32_t kIdescO = umma_idesc_16bit(Element<T>::kBf16, DIM, true);
         int ring = 0, items_of[2] = {0, 0}, q_uses[2] = {0, 0};
         const uint32_t q_base = smem_u32(smem_q), kv_base = smem_u32(smem_kv);
-        uint32_t p_phases = 0;        // bit 2 x + h: parity of the next P of lane x, buffer h
+        uint32_t p_phase[2] = {0, 0};       // parity of a lane's next weights; both buffers' turn over with a tile
         while (ok && walk.next(p, item, head)) {
             const AttnLanes l = attn_lanes(item, p.tile_tokens);
             if (item.tiles == 0) continue;
@@ -681,17 +681,22 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
             }
             const bool pair = uniform(l.pair) != 0;
             const int tiles = uniform(item.tiles);
-            const int steps[2] = {uniform(2 * l.tiles[0]), uniform(2 * l.tiles[1])};
-            // S of lane x for its step i; the key tile is released when its last reader has been issued
-            auto scores = [&](int x, int i) {
-                const int t = pair ? i >> 1 : 2 * (i >> 1) + x, h = i & 1;
-                const int at = ring + ring_key(pair, t);
-                const int stage = at % kStages;
-                ok = ok && hot_wait(&sh.kv_full[stage], (at / kStages) & 1);
-                if (!ok) return;
-                tcgen05_fence_after_sync();
+            const int lane_tiles[2] = {uniform(l.tiles[0]), uniform(l.tiles[1])};
+            // tile j of lane x: the lane's 2 j + h-th step works on half h of it
+            auto key_tile = [&](int x, int j) { return pair ? j : 2 * j + x; };
+            uint32_t k_tile[2] = {0, 0}, v_tile[2] = {0, 0};       // shared-memory address of the lanes' current tiles
+            int k_stage[2] = {0, 0}, v_stage[2] = {0, 0};
+            // S of lane x for half h of its tile j; the key tile is released when its last reader has been issued
+            auto scores = [&](int x, int j, int h) {
+                if (h == 0) {
+                    const int at = ring + ring_key(pair, key_tile(x, j));
+                    k_stage[x] = at % kStages;
+                    k_tile[x] = kv_base + k_stage[x] * Shape::kTileBytes;
+                    ok = ok && hot_wait(&sh.kv_full[k_stage[x]], (at / kStages) & 1);
+                    if (!ok) return;
+                }
                 const uint64_t a = umma_desc_sw128_kmajor(q_base + (pair ? x : 0) * Shape::kTileBytes);
-                const uint64_t b = umma_desc_sw128_kmajor(kv_base + stage * Shape::kTileBytes + h * (kAttnHalf * 128));
+                const uint64_t b = umma_desc_sw128_kmajor(k_tile[x] + h * (kAttnHalf * 128));
                 if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < DIM / 16; ++k) {
@@ -701,41 +706,53 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
                     }
                     umma_commit(&sh.s_full[x][h]);
                     if (h == 1) {
-                        if (!pair || x == 1) umma_commit(&sh.kv_empty[stage]);
+                        if (!pair || x == 1) umma_commit(&sh.kv_empty[k_stage[x]]);
                         // the last scores of a row tile: its rows may be replaced
-                        if (t + 1 == tiles) umma_commit(&sh.q_empty[pair ? x : 0]);
+                        if (key_tile(x, j) + 1 == tiles) umma_commit(&sh.q_empty[pair ? x : 0]);
                     }
                 }
                 __syncwarp();
             };
-            for (int i = 0; i < 2; ++i)
-                for (int x = 0; x < 2; ++x)
-                    if (steps[x] > 0) scores(x, i);
-            for (int i = 0; ok && i < steps[0]; ++i) {
-                for (int x = 0; ok && x < 2; ++x) {
-                    if (i >= steps[x]) break;
-                    const int t = pair ? i >> 1 : 2 * (i >> 1) + x, h = i & 1;
-                    const int at = ring + ring_value(pair, t, tiles);
-                    const int stage = at % kStages;
-                    ok = hot_wait(&sh.kv_full[stage], (at / kStages) & 1);
-                    if (ok && i == 0) ok = hot_wait(&sh.o_empty[x], (items_of[x] & 1) ^ 1);
-                    if (ok) ok = hot_wait(&sh.p_full[x][h], (p_phases >> (2 * x + h)) & 1);
-                    p_phases ^= 1u << (2 * x + h);
-                    if (!ok) break;
-                    tcgen05_fence_after_sync();
-                    const uint32_t a = tmem + kAttnColumnS + x * 128 + h * kAttnHalf;
-                    const uint64_t b = umma_desc_sw128_mnmajor(kv_base + stage * Shape::kTileBytes + h * (kAttnHalf * 128), kAttnTile * 128);
-                    if (elect_one()) {
 #pragma unroll
-                        for (int k = 0; k < kAttnHalf / 16; ++k)
-                            umma_16bit_ts(tmem + kAttnColumnO + x * 128, a + k * 8, b + k * (2048 >> 4), kIdescO, i > 0 || k > 0);
-                        umma_commit(&sh.pv_done[x]);
-                        if (i + 1 == steps[x]) umma_commit(&sh.o_full[x]);
-                        if (h == 1 && (!pair || x == 1)) umma_commit(&sh.kv_empty[stage]);
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+                    if (x == 0 || lane_tiles[1] > 0) scores(x, 0, h);
+            for (int j = 0; ok && j < lane_tiles[0]; ++j) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        if (!ok || (x == 1 && j >= lane_tiles[1])) continue;
+                        if (h == 0) {
+                            const int at = ring + ring_value(pair, key_tile(x, j), tiles);
+                            v_stage[x] = at % kStages;
+                            v_tile[x] = kv_base + v_stage[x] * Shape::kTileBytes;
+                            ok = hot_wait(&sh.kv_full[v_stage[x]], (at / kStages) & 1);
+                            if (ok && j == 0) ok = hot_wait(&sh.o_empty[x], (items_of[x] & 1) ^ 1);
+                        }
+                        if (ok) ok = hot_wait(&sh.p_full[x][h], p_phase[x]);
+                        if (!ok) continue;
+                        tcgen05_fence_after_sync();
+                        const uint32_t a = tmem + kAttnColumnS + x * 128 + h * kAttnHalf;
+                        const uint64_t b = umma_desc_sw128_mnmajor(v_tile[x] + h * (kAttnHalf * 128), kAttnTile * 128);
+                        if (elect_one()) {
+#pragma unroll
+                            for (int k = 0; k < kAttnHalf / 16; ++k)
+                                umma_16bit_ts(tmem + kAttnColumnO + x * 128, a + k * 8, b + k * (2048 >> 4), kIdescO, j > 0 || h > 0 || k > 0);
+                            umma_commit(&sh.pv_done[x]);
+                            if (h == 1) {
+                                if (j + 1 == lane_tiles[x]) umma_commit(&sh.o_full[x]);
+                                if (!pair || x == 1) umma_commit(&sh.kv_empty[v_stage[x]]);
+                            }
+                        }
+                        __syncwarp();
+                        if (j + 1 < lane_tiles[x]) scores(x, j + 1, h);
+                        if (h == 1) {
+                            p_phase[x] ^= 1u;
+                            if (j + 1 == lane_tiles[x]) ++items_of[x];
+                        }
                     }
-                    __syncwarp();
-                    if (i + 1 == steps[x]) ++items_of[x];
-                    if (i + 2 < steps[x]) scores(x, i + 2);
                 }
             }
             ring += 2 * tiles;

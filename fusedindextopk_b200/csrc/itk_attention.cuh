@@ -19,8 +19,8 @@
 // chunks of keys when there are too few to fill the SMs, and lays out the partial results; the attention kernel
 // walks the list; a third kernel joins the partial results.  No length is read by the host.
 //
-// Attention kernel, one CTA per SM, 11 warps: 0-3 softmax of lane A, 4-7 softmax of lane B (one row per thread),
-// 8 UMMA issuer and TMEM owner, 9 TMA producer, 10 guard.  TMEM: S_A, S_B (128 columns each; the weights P overwrite
+// Attention kernel, one CTA per SM, 12 warps: 0-3 softmax of lane A, 4-7 softmax of lane B (one row per thread),
+// 8 and 9 UMMA issuers of lane A and B, 10 TMA producer, 11 guard.  TMEM: S_A, S_B (128 columns each; the weights P overwrite
 // the first half of S as 16-bit pairs and are the A operand of P V from there), O_A, O_B.  The row maximum is only
 // moved when it grows by more than 2^8 (kLazy): until then weights are at most 2^8 and O needs no rescaling; when it
 // does, the row's own softmax warp rescales O in TMEM, which is safe because S of a tile is complete only after P V
@@ -41,9 +41,9 @@
 namespace itk {
 
 constexpr int kAttnTile = 128;                 // rows of a row tile, keys of a key tile
-constexpr int kAttnThreads = 352;
+constexpr int kAttnThreads = 384;
 constexpr int kAttnSoftmaxWarps = 4;           // per lane
-constexpr int kAttnMmaWarp = 8, kAttnLoadWarp = 9, kAttnGuardWarp = 10;
+constexpr int kAttnMmaWarp = 8, kAttnLoadWarp = 10, kAttnGuardWarp = 11;   // kAttnMmaWarp + x issues for lane x
 constexpr int kAttnTmemColumns = 512;
 constexpr int kAttnHalf = 64;                  // keys of a step: half a tile
 constexpr int kAttnColumnS = 0, kAttnColumnO = 256;   // lane B: + 128; step i of a lane uses S columns 64 * (i % 2)
@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh.q_full[i], 1);
-            mbar_init(&sh.q_empty[i], 1);
+            mbar_init(&sh.q_empty[i], 2);       // both issuers, or the only one that reads it twice
             for (int h = 0; h < 2; ++h) {
                 mbar_init(&sh.s_full[i][h], 1);
                 mbar_init(&sh.p_full[i][h], kAttnSoftmaxWarps);
@@ -586,7 +586,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
         }
         for (int i = 0; i < kStages; ++i) {
             mbar_init(&sh.kv_full[i], 1);
-            mbar_init(&sh.kv_empty[i], 1);
+            mbar_init(&sh.kv_empty[i], 2);
             mbar_init(&sh.guard_full[i], 1);
         }
         for (int i = 0; i < kAttnPoison; ++i) sh.poison[i] = 0;
@@ -596,7 +596,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
         prefetch_tensormap(&p.map_k);
         prefetch_tensormap(&p.map_v);
     }
-    if (warp == kAttnMmaWarp) {
+    if (warp == kAttnMmaWarp) {          // the first issuer owns TMEM
         tmem_alloc(&sh.tmem_base, kAttnTmemColumns);
         tmem_relinquish_alloc_permit();
     }
@@ -665,95 +665,94 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
                 }
             }
         }
-    } else if (warp == kAttnMmaWarp) {
-        // ============================================================ UMMA issuer
+    } else if (warp == kAttnMmaWarp || warp == kAttnMmaWarp + 1) {
+        // ============================================================ UMMA issuer of lane x
+        // One warp per lane: while one waits for its weights the other keeps the tensor pipe fed.
         constexpr uint32_t kIdescS = umma_idesc_16bit(Element<T>::kBf16, kAttnHalf, false);
         constexpr uint32_t kIdescO = umma_idesc_16bit(Element<T>::kBf16, DIM, true);
-        int ring = 0, items_of[2] = {0, 0}, q_uses[2] = {0, 0};
+        const int x = warp - kAttnMmaWarp;
+        const uint32_t tmem_s = tmem + kAttnColumnS + x * 128, tmem_o = tmem + kAttnColumnO + x * 128;
         const uint32_t q_base = smem_u32(smem_q), kv_base = smem_u32(smem_kv);
-        uint32_t p_phase[2] = {0, 0};       // parity of a lane's next weights; both buffers' turn over with a tile
+        int ring = 0, items = 0, q_uses[2] = {0, 0};
+        uint32_t p_phase = 0;               // parity of the next weights; both buffers' turn over with a tile
         while (ok && walk.next(p, item, head)) {
             const AttnLanes l = attn_lanes(item, p.tile_tokens);
-            if (item.tiles == 0) continue;
-            for (int tile = 0; ok && tile < (l.pair ? 2 : 1); ++tile) {
-                ok = hot_wait(&sh.q_full[tile], q_uses[tile] & 1);
-                ++q_uses[tile];
-            }
             const bool pair = uniform(l.pair) != 0;
-            const int tiles = uniform(item.tiles);
-            const int lane_tiles[2] = {uniform(l.tiles[0]), uniform(l.tiles[1])};
-            // tile j of lane x: the lane's 2 j + h-th step works on half h of it
-            auto key_tile = [&](int x, int j) { return pair ? j : 2 * j + x; };
-            uint32_t k_tile[2] = {0, 0}, v_tile[2] = {0, 0};       // shared-memory address of the lanes' current tiles
-            int k_stage[2] = {0, 0}, v_stage[2] = {0, 0};
-            // S of lane x for half h of its tile j; the key tile is released when its last reader has been issued
-            auto scores = [&](int x, int j, int h) {
-                if (h == 0) {
-                    const int at = ring + ring_key(pair, key_tile(x, j));
-                    k_stage[x] = at % kStages;
-                    k_tile[x] = kv_base + k_stage[x] * Shape::kTileBytes;
-                    ok = ok && hot_wait(&sh.kv_full[k_stage[x]], (at / kStages) & 1);
-                    if (!ok) return;
-                }
-                const uint64_t a = umma_desc_sw128_kmajor(q_base + (pair ? x : 0) * Shape::kTileBytes);
-                const uint64_t b = umma_desc_sw128_kmajor(k_tile[x] + h * (kAttnHalf * 128));
-                if (elect_one()) {
-#pragma unroll
-                    for (int k = 0; k < DIM / 16; ++k) {
-                        constexpr int kChunkStep = (kAttnTile * 128) >> 4;
-                        const int offset = (k / 4) * kChunkStep + (k % 4) * 2;      // 16-byte units: 32 bytes per K step
-                        umma_16bit_ss(tmem + kAttnColumnS + x * 128 + h * kAttnHalf, a + offset, b + offset, kIdescS, k > 0);
+            const int tiles = uniform(item.tiles), mine = uniform(l.tiles[x]);
+            const int q_tile = pair ? x : 0;
+            const uint32_t q_phase = q_uses[q_tile] & 1;
+            if (tiles > 0) {
+                ++q_uses[0];
+                if (pair) ++q_uses[1];
+            }
+            if (mine > 0) {
+                ok = hot_wait(&sh.q_full[q_tile], q_phase);
+                // tiles of a split item alternate between the lanes; each lane's reader count is made up to two
+                const bool twice = !pair;
+                auto key_tile = [&](int j) { return pair ? j : 2 * j + x; };
+                uint32_t k_tile = 0;
+                int k_stage = 0;
+                const uint64_t q_desc = umma_desc_sw128_kmajor(q_base + q_tile * Shape::kTileBytes);
+                // S for half h of the lane's tile j; the key tile is released when its last half has been issued
+                auto scores = [&](int j, int h) {
+                    if (h == 0) {
+                        const int at = ring + ring_key(pair, key_tile(j));
+                        k_stage = at % kStages;
+                        k_tile = kv_base + k_stage * Shape::kTileBytes;
+                        ok = ok && hot_wait(&sh.kv_full[k_stage], (at / kStages) & 1);
+                        if (!ok) return;
                     }
-                    umma_commit(&sh.s_full[x][h]);
-                    if (h == 1) {
-                        if (!pair || x == 1) umma_commit(&sh.kv_empty[k_stage[x]]);
-                        // the last scores of a row tile: its rows may be replaced
-                        if (key_tile(x, j) + 1 == tiles) umma_commit(&sh.q_empty[pair ? x : 0]);
-                    }
-                }
-                __syncwarp();
-            };
+                    const uint64_t b = umma_desc_sw128_kmajor(k_tile + h * (kAttnHalf * 128));
+                    if (elect_one()) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int x = 0; x < 2; ++x)
-                    if (x == 0 || lane_tiles[1] > 0) scores(x, 0, h);
-            for (int j = 0; ok && j < lane_tiles[0]; ++j) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        if (!ok || (x == 1 && j >= lane_tiles[1])) continue;
-                        if (h == 0) {
-                            const int at = ring + ring_value(pair, key_tile(x, j), tiles);
-                            v_stage[x] = at % kStages;
-                            v_tile[x] = kv_base + v_stage[x] * Shape::kTileBytes;
-                            ok = hot_wait(&sh.kv_full[v_stage[x]], (at / kStages) & 1);
-                            if (ok && j == 0) ok = hot_wait(&sh.o_empty[x], (items_of[x] & 1) ^ 1);
+                        for (int k = 0; k < DIM / 16; ++k) {
+                            constexpr int kChunkStep = (kAttnTile * 128) >> 4;
+                            const int offset = (k / 4) * kChunkStep + (k % 4) * 2;      // 16-byte units: 32 bytes per K step
+                            umma_16bit_ss(tmem_s + h * kAttnHalf, q_desc + offset, b + offset, kIdescS, k > 0);
                         }
-                        if (ok) ok = hot_wait(&sh.p_full[x][h], p_phase[x]);
+                        umma_commit(&sh.s_full[x][h]);
+                        if (h == 1) {
+                            umma_commit(&sh.kv_empty[k_stage]);
+                            if (twice) umma_commit(&sh.kv_empty[k_stage]);
+                            if (j + 1 == mine) {       // the last scores of the row tile: its rows may be replaced
+                                umma_commit(&sh.q_empty[q_tile]);
+                                if (pair || tiles == 1) umma_commit(&sh.q_empty[q_tile]);
+                            }
+                        }
+                    }
+                    __syncwarp();
+                };
+                scores(0, 0);
+                scores(0, 1);
+                for (int j = 0; ok && j < mine; ++j) {
+                    const int at = ring + ring_value(pair, key_tile(j), tiles);
+                    const int v_stage = at % kStages;
+                    const uint64_t v_desc = umma_desc_sw128_mnmajor(kv_base + v_stage * Shape::kTileBytes, kAttnTile * 128);
+                    ok = hot_wait(&sh.kv_full[v_stage], (at / kStages) & 1);
+                    if (ok && j == 0) ok = hot_wait(&sh.o_empty[x], (items & 1) ^ 1);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (ok) ok = hot_wait(&sh.p_full[x][h], p_phase);
                         if (!ok) continue;
                         tcgen05_fence_after_sync();
-                        const uint32_t a = tmem + kAttnColumnS + x * 128 + h * kAttnHalf;
-                        const uint64_t b = umma_desc_sw128_mnmajor(v_tile[x] + h * (kAttnHalf * 128), kAttnTile * 128);
                         if (elect_one()) {
 #pragma unroll
                             for (int k = 0; k < kAttnHalf / 16; ++k)
-                                umma_16bit_ts(tmem + kAttnColumnO + x * 128, a + k * 8, b + k * (2048 >> 4), kIdescO, j > 0 || h > 0 || k > 0);
+                                umma_16bit_ts(tmem_o, tmem_s + h * kAttnHalf + k * 8, v_desc + (h * (kAttnHalf * 128) + k * 2048) / 16,
+                                              kIdescO, j > 0 || h > 0 || k > 0);
                             umma_commit(&sh.pv_done[x]);
                             if (h == 1) {
-                                if (j + 1 == lane_tiles[x]) umma_commit(&sh.o_full[x]);
-                                if (!pair || x == 1) umma_commit(&sh.kv_empty[v_stage[x]]);
+                                if (j + 1 == mine) umma_commit(&sh.o_full[x]);
+                                umma_commit(&sh.kv_empty[v_stage]);
+                                if (twice) umma_commit(&sh.kv_empty[v_stage]);
                             }
                         }
                         __syncwarp();
-                        if (j + 1 < lane_tiles[x]) scores(x, j + 1, h);
-                        if (h == 1) {
-                            p_phase[x] ^= 1u;
-                            if (j + 1 == lane_tiles[x]) ++items_of[x];
-                        }
+                        if (j + 1 < mine) scores(j + 1, h);
                     }
+                    p_phase ^= 1u;
                 }
+                ++items;
             }
             ring += 2 * tiles;
         }

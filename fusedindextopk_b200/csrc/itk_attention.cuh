@@ -105,6 +105,11 @@ struct AttnParams {
 
 // ------------------------------------------------------------------ PTX
 
+// Programmatic dependent launch: the next kernel of the stream may start its prologue; what it reads of this one it
+// reads behind grid_wait, which returns when this one has completed.
+__device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // True in one thread of the warp, always the same one.  The tcgen05 instructions take their operands from uniform
 // registers: under this predicate, with operands that come out of a broadcast, they are moved there once; under a
 // comparison with the lane id every issue paid about 100 cycles (4 UMMAs and two commits: 590 cycles).
@@ -265,15 +270,24 @@ static_assert(kAttnMinChunk >= 2, "a split item of one tile is its entry's only 
 // the time its keys take to arrive.
 constexpr int kAttnPairCost = 4, kAttnSplitCost = 3;
 
+constexpr int kAttnCached = 1024;   // requests whose lengths the plan keeps in shared memory
+
 struct AttnEntry {
     AttnItem item;
     int tiles, unit;          // key tiles, cost of one
     bool pair, prefix;
 };
 
+// Lengths and first entries of the requests: in shared memory for batches that fit it, else from global memory.
+struct AttnRequests {
+    const AttnRequest* cached;
+    const int* first;         // [requests + 1] own entries before a request
+    bool is_cached;
+};
+
 // Entry e of the list "prefix entries, then the entries of request 0, 1, ...": up to 2 TT consecutive tokens of one
 // request (of any requests for the prefix, which they all see).
-__device__ __forceinline__ AttnEntry attn_entry(const AttnParams& p, int e, int prefix_entries, int rows_end) {
+__device__ __forceinline__ AttnEntry attn_entry(const AttnParams& p, const AttnRequests& requests, int e, int prefix_entries, int rows_end) {
     const int span = 2 * p.tile_tokens;
     AttnEntry r;
     r.prefix = e < prefix_entries;
@@ -287,18 +301,18 @@ __device__ __forceinline__ AttnEntry attn_entry(const AttnParams& p, int e, int 
         r.item.k_first = 0;
     } else {
         const int own = e - prefix_entries;
-        int low = 0, high = p.a.requests;       // entry_first[low] <= own < entry_first[high]
+        int low = 0, high = p.a.requests;       // first[low] <= own < first[high]
         while (high - low > 1) {
             const int middle = (low + high) >> 1;
-            if (p.w.entry_first[middle] <= own) {
+            if (requests.first[middle] <= own) {
                 low = middle;
             } else {
                 high = middle;
             }
         }
         bool bad = false;
-        const AttnRequest q = attn_request(p.a, low, bad);
-        const int first = (own - p.w.entry_first[low]) * span;
+        const AttnRequest q = requests.is_cached ? requests.cached[low] : attn_request(p.a, low, bad);
+        const int first = (own - requests.first[low]) * span;
         r.item.q_first = q.q_first + first;
         r.item.tokens = min(span, q.q_count - first);
         r.item.request = low;
@@ -329,24 +343,34 @@ __global__ void __launch_bounds__(kAttnPlanThreads) itk_attention_plan_kernel(co
     __shared__ unsigned long long total_cost;
     __shared__ int counts[kAttnTries], longest, item_count, combine_count, partial_rows;
     __shared__ int bins[kAttnBins];
+    __shared__ AttnRequest cache[kAttnCached];
+    __shared__ int cached_first[kAttnCached + 1];
+    const bool is_cached = p.a.requests <= kAttnCached;
+    int* entry_first = is_cached ? cached_first : p.w.entry_first;
+    const AttnRequests requests{cache, entry_first, is_cached};
     const int tx = threadIdx.x, lane = tx & 31, warp = tx >> 5;
     const int span = 2 * p.tile_tokens, kv_heads = p.a.kv_heads;
+    grid_launch_dependents();
     if (tx == 0) {
         carry = 0;
         total_cost = 0;
         longest = item_count = combine_count = partial_rows = 0;
-        rows_end = min(max(p.a.cu_q[p.a.requests], 0), p.a.tokens);
     }
+    if (tx == 32) rows_end = min(max(p.a.cu_q[p.a.requests], 0), p.a.tokens);
     if (tx < kAttnTries) counts[tx] = 0;
     if (tx < kAttnBins) bins[tx] = 0;
-    __syncthreads();
+    // (the barriers of the first pass below stand between these and their first readers: there is at least one request)
 
     // own entries before every request
     bool bad = false;
     for (int base = 0; base < p.a.requests; base += kAttnPlanThreads) {
         const int b = base + tx;
         int mine = 0;
-        if (b < p.a.requests) mine = (attn_request(p.a, b, bad).q_count + span - 1) / span;
+        if (b < p.a.requests) {
+            const AttnRequest request = attn_request(p.a, b, bad);
+            if (is_cached) cache[b] = request;
+            mine = (request.q_count + span - 1) / span;
+        }
         int upto = mine;
 #pragma unroll
         for (int step = 1; step < 32; step <<= 1) {
@@ -357,7 +381,7 @@ __global__ void __launch_bounds__(kAttnPlanThreads) itk_attention_plan_kernel(co
         __syncthreads();
         int before = carry;
         for (int w = 0; w < warp; ++w) before += warp_sums[w];
-        if (b < p.a.requests) p.w.entry_first[b] = before + upto - mine;
+        if (b < p.a.requests) entry_first[b] = before + upto - mine;
         __syncthreads();
         if (tx == kAttnPlanThreads - 1) carry = before + upto;
         __syncthreads();
@@ -366,21 +390,26 @@ __global__ void __launch_bounds__(kAttnPlanThreads) itk_attention_plan_kernel(co
     const int prefix_entries = p.a.prefix_keys > 0 ? (rows_end + span - 1) / span : 0;
     const int own_entries = min(carry, p.w.max_combines);
     const int entries = prefix_entries + own_entries;
-    if (tx == 0) p.w.entry_first[p.a.requests] = own_entries;
+    if (tx == 0) entry_first[p.a.requests] = own_entries;
     __syncthreads();
+
+    // every thread keeps its first entry; batches of more than 1024 entries work the others out again in every pass
+    AttnEntry kept;
+    if (tx < entries) kept = attn_entry(p, requests, tx, prefix_entries, rows_end);
+    auto entry_at = [&](int e) { return e == tx ? kept : attn_entry(p, requests, e, prefix_entries, rows_end); };
 
     // the chunk length that spreads the work over the SMs in one wave, if there is one
     unsigned long long cost = 0;
     for (int e = tx; e < entries; e += kAttnPlanThreads) {
-        const AttnEntry entry = attn_entry(p, e, prefix_entries, rows_end);
+        const AttnEntry entry = entry_at(e);
         cost += static_cast<unsigned long long>(entry.tiles) * entry.unit;
     }
-    atomicAdd(&total_cost, cost);
+    if (cost != 0) atomicAdd(&total_cost, cost);
     __syncthreads();
     const long long share = max(1ll, (static_cast<long long>(total_cost) * kv_heads + p.sm_count - 1) / p.sm_count);
     int mine[kAttnTries] = {};
     for (int e = tx; e < entries; e += kAttnPlanThreads) {
-        const AttnEntry entry = attn_entry(p, e, prefix_entries, rows_end);
+        const AttnEntry entry = entry_at(e);
 #pragma unroll
         for (int k = 0; k < kAttnTries; ++k) mine[k] += attn_chunks(entry, share + share * k / kAttnTries);
     }
@@ -394,14 +423,14 @@ __global__ void __launch_bounds__(kAttnPlanThreads) itk_attention_plan_kernel(co
 
     // items by cost, the costliest first: a counting sort over 256 cost classes
     for (int e = tx; e < entries; e += kAttnPlanThreads) {
-        const AttnEntry entry = attn_entry(p, e, prefix_entries, rows_end);
+        const AttnEntry entry = entry_at(e);
         const int chunks = max(1, attn_chunks(entry, chunk));
         atomicMax(&longest, (entry.tiles + chunks - 1) / chunks * entry.unit);
     }
     __syncthreads();
     const int top = max(longest, 1);
     for (int e = tx; e < entries; e += kAttnPlanThreads) {
-        const AttnEntry entry = attn_entry(p, e, prefix_entries, rows_end);
+        const AttnEntry entry = entry_at(e);
         const int chunks = max(1, attn_chunks(entry, chunk));
         const int item_cost = (entry.tiles + chunks - 1) / chunks * entry.unit;
         const int bin = kAttnBins - 1 - static_cast<int>(static_cast<long long>(item_cost) * (kAttnBins - 1) / top);
@@ -431,7 +460,7 @@ __global__ void __launch_bounds__(kAttnPlanThreads) itk_attention_plan_kernel(co
     }
     __syncthreads();
     for (int e = tx; e < entries; e += kAttnPlanThreads) {
-        AttnEntry entry = attn_entry(p, e, prefix_entries, rows_end);
+        AttnEntry entry = entry_at(e);
         const int chunks = attn_chunks(entry, chunk);               // 0: no key at all
         const int longest_chunk = chunks > 0 ? (entry.tiles + chunks - 1) / chunks : 0;
         const int lanes = !entry.pair && longest_chunk > 1 ? 2 : 1;
@@ -548,9 +577,8 @@ __device__ __forceinline__ const T* attn_value_row(const AttnParams& p, const At
     return static_cast<const T*>(seg.v) + page * seg.v_page_stride + row * seg.v_row_stride + head * seg.v_head_stride;
 }
 
-// Ring position of the key and value tile of step t of an item.  Pair: K0 V0 K1 V1 ...  Split (the lanes take turns and
-// each is one key tile ahead of its values): K0 K1 V0 K2 V1 K3 ... V(n-1).
-__device__ __forceinline__ int ring_key(bool pair, int t) { return pair ? 2 * t : (t < 2 ? t : 2 * t - 1); }
+// Ring position of the value tile t of an item.  Pair: K0 V0 K1 V1 ...  Split (the lanes take turns and each is one key
+// tile ahead of its values): K0 K1 V0 K2 V1 K3 ... V(n-1).
 __device__ __forceinline__ int ring_value(bool pair, int t, int tiles) {
     return pair ? 2 * t + 1 : min(2 * t + 2, 2 * tiles - 1);
 }
@@ -570,12 +598,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
         if (threadIdx.x == 0) atomicOr(p.status, ITK_SERVING_BAD_SHARED_BASE);
         return;
     }
-    if (static_cast<int>(blockIdx.x) >= p.w.counters->items * p.a.kv_heads) return;   // more CTAs than work
-
+    grid_launch_dependents();
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh.q_full[i], 1);
-            mbar_init(&sh.q_empty[i], 2);       // both issuers, or the only one that reads it twice
+            mbar_init(&sh.q_empty[i], 2);       // both issuers
             for (int h = 0; h < 2; ++h) {
                 mbar_init(&sh.s_full[i][h], 1);
                 mbar_init(&sh.p_full[i][h], kAttnSoftmaxWarps);
@@ -603,6 +630,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
     tcgen05_fence_before_sync();
     __syncthreads();
     tcgen05_fence_after_sync();
+    grid_wait();                         // the plan's list from here on
     const uint32_t tmem = static_cast<uint32_t>(uniform(static_cast<int>(sh.tmem_base)));
     volatile int* abort_flag = &sh.abort;
     // a wait of the whole warp: its lanes leave together
@@ -667,94 +695,110 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
         }
     } else if (warp == kAttnMmaWarp || warp == kAttnMmaWarp + 1) {
         // ============================================================ UMMA issuer of lane x
-        // One warp per lane: while one waits for its weights the other keeps the tensor pipe fed.
+        // One warp per lane: while one waits for its weights the other keeps the tensor pipe fed.  A parity wait says
+        // nothing about a barrier that is more than one phase behind, so BOTH issuers see every use of q_full and
+        // kv_full, in the order of the loads, and each gives one of the two arrivals that free the buffer: a commit
+        // behind its last read, or a plain arrival for what only the other lane reads.
         constexpr uint32_t kIdescS = umma_idesc_16bit(Element<T>::kBf16, kAttnHalf, false);
         constexpr uint32_t kIdescO = umma_idesc_16bit(Element<T>::kBf16, DIM, true);
         const int x = warp - kAttnMmaWarp;
         const uint32_t tmem_s = tmem + kAttnColumnS + x * 128, tmem_o = tmem + kAttnColumnO + x * 128;
         const uint32_t q_base = smem_u32(smem_q), kv_base = smem_u32(smem_kv);
-        int ring = 0, items = 0, q_uses[2] = {0, 0};
+        int ring = 0, items = 0, q_uses[2] = {0, 0};      // tiles seen so far; items of this lane; uses of the row tiles
         uint32_t p_phase = 0;               // parity of the next weights; both buffers' turn over with a tile
+        auto release = [&](uint64_t* bar) {
+            if (lane == 0) mbar_arrive(bar);
+        };
         while (ok && walk.next(p, item, head)) {
             const AttnLanes l = attn_lanes(item, p.tile_tokens);
             const bool pair = uniform(l.pair) != 0;
             const int tiles = uniform(item.tiles), mine = uniform(l.tiles[x]);
+            if (tiles == 0) continue;
             const int q_tile = pair ? x : 0;
-            const uint32_t q_phase = q_uses[q_tile] & 1;
-            if (tiles > 0) {
-                ++q_uses[0];
-                if (pair) ++q_uses[1];
+            for (int tile = 0; ok && tile < (pair ? 2 : 1); ++tile) {
+                ok = hot_wait(&sh.q_full[tile], q_uses[tile] & 1);
+                ++q_uses[tile];
+                if (ok && (tile != q_tile || mine == 0)) release(&sh.q_empty[tile]);
             }
-            if (mine > 0) {
-                ok = hot_wait(&sh.q_full[q_tile], q_phase);
-                // tiles of a split item alternate between the lanes; each lane's reader count is made up to two
-                const bool twice = !pair;
-                auto key_tile = [&](int j) { return pair ? j : 2 * j + x; };
-                uint32_t k_tile = 0;
-                int k_stage = 0;
-                const uint64_t q_desc = umma_desc_sw128_kmajor(q_base + q_tile * Shape::kTileBytes);
-                // S for half h of the lane's tile j; the key tile is released when its last half has been issued
-                auto scores = [&](int j, int h) {
-                    if (h == 0) {
-                        const int at = ring + ring_key(pair, key_tile(j));
-                        k_stage = at % kStages;
-                        k_tile = kv_base + k_stage * Shape::kTileBytes;
-                        ok = ok && hot_wait(&sh.kv_full[k_stage], (at / kStages) & 1);
-                        if (!ok) return;
+            const uint64_t q_desc = umma_desc_sw128_kmajor(q_base + q_tile * Shape::kTileBytes);
+            uint32_t k_tile = 0;
+            int k_stage = 0;
+            // the next tile of the ring, in shared memory
+            auto arrive_tile = [&](int& stage) {
+                stage = ring % kStages;
+                ok = ok && hot_wait(&sh.kv_full[stage], (ring / kStages) & 1);
+                ++ring;
+                return ok;
+            };
+            // tiles that only the other lane reads (split items)
+            auto pass_tile = [&]() {
+                int stage;
+                if (arrive_tile(stage)) release(&sh.kv_empty[stage]);
+            };
+            // S for half h of the lane's tile j; the key tile is released when its last half has been issued
+            auto scores = [&](int j, int h) {
+                if (h == 0) {
+                    if (!arrive_tile(k_stage)) return;
+                    k_tile = kv_base + k_stage * Shape::kTileBytes;
+                }
+                if (!ok) return;
+                const uint64_t b = umma_desc_sw128_kmajor(k_tile + h * (kAttnHalf * 128));
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < DIM / 16; ++k) {
+                        constexpr int kChunkStep = (kAttnTile * 128) >> 4;
+                        const int offset = (k / 4) * kChunkStep + (k % 4) * 2;      // 16-byte units: 32 bytes per K step
+                        umma_16bit_ss(tmem_s + h * kAttnHalf, q_desc + offset, b + offset, kIdescS, k > 0);
                     }
-                    const uint64_t b = umma_desc_sw128_kmajor(k_tile + h * (kAttnHalf * 128));
+                    umma_commit(&sh.s_full[x][h]);
+                    if (h == 1) {
+                        umma_commit(&sh.kv_empty[k_stage]);
+                        // the last scores of the row tile: its rows may be replaced
+                        if (j + 1 == mine) umma_commit(&sh.q_empty[q_tile]);
+                    }
+                }
+                __syncwarp();
+            };
+            // Loads come as K0 V0 K1 V1 ... (pair) or K0 K1 V0 K2 V1 K3 ... (split, tile t being lane t % 2's)
+            if (!pair && x == 1) pass_tile();
+            if (mine > 0) {
+                scores(0, 0);
+                scores(0, 1);
+            }
+            if (!pair && x == 0 && tiles > 1) pass_tile();
+            for (int t = 0; ok && t < tiles; ++t) {
+                if (!pair && (t & 1) != x) {
+                    pass_tile();
+                    if (t + 2 < tiles) pass_tile();
+                    continue;
+                }
+                const int j = pair ? t : t >> 1;
+                int v_stage;
+                if (!arrive_tile(v_stage)) break;
+                const uint64_t v_desc = umma_desc_sw128_mnmajor(kv_base + v_stage * Shape::kTileBytes, kAttnTile * 128);
+                if (j == 0) ok = hot_wait(&sh.o_empty[x], (items & 1) ^ 1);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (ok) ok = hot_wait(&sh.p_full[x][h], p_phase);
+                    if (!ok) continue;
+                    tcgen05_fence_after_sync();
                     if (elect_one()) {
 #pragma unroll
-                        for (int k = 0; k < DIM / 16; ++k) {
-                            constexpr int kChunkStep = (kAttnTile * 128) >> 4;
-                            const int offset = (k / 4) * kChunkStep + (k % 4) * 2;      // 16-byte units: 32 bytes per K step
-                            umma_16bit_ss(tmem_s + h * kAttnHalf, q_desc + offset, b + offset, kIdescS, k > 0);
-                        }
-                        umma_commit(&sh.s_full[x][h]);
+                        for (int k = 0; k < kAttnHalf / 16; ++k)
+                            umma_16bit_ts(tmem_o, tmem_s + h * kAttnHalf + k * 8, v_desc + (h * (kAttnHalf * 128) + k * 2048) / 16,
+                                          kIdescO, j > 0 || h > 0 || k > 0);
+                        umma_commit(&sh.pv_done[x]);
                         if (h == 1) {
-                            umma_commit(&sh.kv_empty[k_stage]);
-                            if (twice) umma_commit(&sh.kv_empty[k_stage]);
-                            if (j + 1 == mine) {       // the last scores of the row tile: its rows may be replaced
-                                umma_commit(&sh.q_empty[q_tile]);
-                                if (pair || tiles == 1) umma_commit(&sh.q_empty[q_tile]);
-                            }
+                            if (j + 1 == mine) umma_commit(&sh.o_full[x]);
+                            umma_commit(&sh.kv_empty[v_stage]);
                         }
                     }
                     __syncwarp();
-                };
-                scores(0, 0);
-                scores(0, 1);
-                for (int j = 0; ok && j < mine; ++j) {
-                    const int at = ring + ring_value(pair, key_tile(j), tiles);
-                    const int v_stage = at % kStages;
-                    const uint64_t v_desc = umma_desc_sw128_mnmajor(kv_base + v_stage * Shape::kTileBytes, kAttnTile * 128);
-                    ok = hot_wait(&sh.kv_full[v_stage], (at / kStages) & 1);
-                    if (ok && j == 0) ok = hot_wait(&sh.o_empty[x], (items & 1) ^ 1);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (ok) ok = hot_wait(&sh.p_full[x][h], p_phase);
-                        if (!ok) continue;
-                        tcgen05_fence_after_sync();
-                        if (elect_one()) {
-#pragma unroll
-                            for (int k = 0; k < kAttnHalf / 16; ++k)
-                                umma_16bit_ts(tmem_o, tmem_s + h * kAttnHalf + k * 8, v_desc + (h * (kAttnHalf * 128) + k * 2048) / 16,
-                                              kIdescO, j > 0 || h > 0 || k > 0);
-                            umma_commit(&sh.pv_done[x]);
-                            if (h == 1) {
-                                if (j + 1 == mine) umma_commit(&sh.o_full[x]);
-                                umma_commit(&sh.kv_empty[v_stage]);
-                                if (twice) umma_commit(&sh.kv_empty[v_stage]);
-                            }
-                        }
-                        __syncwarp();
-                        if (j + 1 < mine) scores(j + 1, h);
-                    }
-                    p_phase ^= 1u;
+                    if (j + 1 < mine) scores(j + 1, h);
                 }
-                ++items;
+                p_phase ^= 1u;
             }
-            ring += 2 * tiles;
+            if (mine > 0) ++items;
         }
     } else if (warp == kAttnGuardWarp) {
         // ============================================================ guard
@@ -1030,6 +1074,8 @@ constexpr int kJoinThreads = 256;
 template <typename T, int DIM>
 __global__ void __launch_bounds__(kJoinThreads) itk_attention_join_kernel(const __grid_constant__ AttnParams p) {
     constexpr int kOwn = DIM / 32;
+    constexpr int kFlight = 8;           // partial rows on their way at a time: the loop is bound by their latency
+    grid_wait();
     const AttnCounters counters = *p.w.counters;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int span = 2 * p.tile_tokens;
@@ -1071,20 +1117,30 @@ __global__ void __launch_bounds__(kJoinThreads) itk_attention_join_kernel(const 
                         if (base + lane < count[run])
                             weight = exp2_fast(p.w.partial_lse[first[run] + static_cast<long long>(base + lane) * step[run]] - top);
                         const int here = min(32, count[run] - base);
-#pragma unroll 4
-                        for (int c = 0; c < here; ++c) {
-                            const float w = __shfl_sync(0xffffffffu, weight, c);
-                            if (w == 0.0f) continue;       // an empty slot holds no values
-                            const float* source = p.w.partial_out + (first[run] + static_cast<long long>(base + c) * step[run]) * DIM + lane * kOwn;
-                            float held[kOwn];
-                            if constexpr (kOwn == 4) {
-                                *reinterpret_cast<float4*>(held) = *reinterpret_cast<const float4*>(source);
-                            } else {
-                                *reinterpret_cast<float2*>(held) = *reinterpret_cast<const float2*>(source);
-                            }
-                            total += w;
+                        for (int c = 0; c < here; c += kFlight) {
+                            float held[kFlight][kOwn], w[kFlight];
 #pragma unroll
-                            for (int i = 0; i < kOwn; ++i) sums[i] = fmaf(w, held[i], sums[i]);
+                            for (int k = 0; k < kFlight; ++k) {
+                                w[k] = __shfl_sync(0xffffffffu, weight, (c + k) & 31);
+                                if (c + k >= here) w[k] = 0.0f;
+#pragma unroll
+                                for (int i = 0; i < kOwn; ++i) held[k][i] = 0.0f;
+                                if (w[k] != 0.0f) {        // an empty slot holds no values
+                                    const float* source =
+                                        p.w.partial_out + (first[run] + static_cast<long long>(base + c + k) * step[run]) * DIM + lane * kOwn;
+                                    if constexpr (kOwn == 4) {
+                                        *reinterpret_cast<float4*>(held[k]) = *reinterpret_cast<const float4*>(source);
+                                    } else {
+                                        *reinterpret_cast<float2*>(held[k]) = *reinterpret_cast<const float2*>(source);
+                                    }
+                                }
+                            }
+#pragma unroll
+                            for (int k = 0; k < kFlight; ++k) {
+                                total += w[k];
+#pragma unroll
+                                for (int i = 0; i < kOwn; ++i) sums[i] = fmaf(w[k], held[k][i], sums[i]);
+                            }
                         }
                     }
             }

@@ -156,11 +156,27 @@ int segment_map(CUtensorMap* map, const itk_attention_args& a, const itk_kv_segm
     return encode_map(map, a.element, 4, base, dims, strides, box);
 }
 
+// A launch whose prologue may overlap the kernel before it on the stream.
+template <typename Kernel, typename Params>
+cudaError_t launch_after(Kernel kernel, int grid, int threads, size_t smem, cudaStream_t stream, const Params& params) {
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(grid);
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, params);
+}
+
 template <typename T, int DIM>
 int launch_attention(const AttnParams& params, cudaStream_t stream) {
     itk_attention_plan_kernel<<<1, kAttnPlanThreads, 0, stream>>>(params);
-    itk_attention_kernel<T, DIM><<<params.sm_count, kAttnThreads, AttnShape<DIM>::kSmemBytes, stream>>>(params);
-    itk_attention_join_kernel<T, DIM><<<4 * params.sm_count, kJoinThreads, 0, stream>>>(params);
+    ITK_CUDA(launch_after(itk_attention_kernel<T, DIM>, params.sm_count, kAttnThreads, AttnShape<DIM>::kSmemBytes, stream, params));
+    ITK_CUDA(launch_after(itk_attention_join_kernel<T, DIM>, 4 * params.sm_count, kJoinThreads, 0, stream, params));
     return launched("itk_attention_kernel");
 }
 

@@ -13,6 +13,7 @@ from pathlib import Path
 from typing import Any
 
 import os
+import struct
 
 # ITK_B200_LIBRARY points the loader at another build of the same library (timing studies).
 LIBRARY_PATH = Path(os.environ.get("ITK_B200_LIBRARY") or Path(__file__).resolve().parent / "libitk_b200.so")
@@ -169,9 +170,10 @@ def load_library() -> ctypes.CDLL:
     library.itk_repair_produce_paged.argtypes = [c_void_p] * 8 + [c_int] * 7 + [c_void_p, c_int, c_void_p, c_void_p]
     library.itk_quantize_rows_e4m3.argtypes = [c_void_p, c_int] + [c_void_p] * 4 + [c_longlong, c_void_p]
     library.itk_serving_status.argtypes = [POINTER(c_int), c_int]
-    library.itk_plan_pages.argtypes = [POINTER(PagePlanArgs), c_void_p]
-    library.itk_append_tokens.argtypes = [POINTER(AppendArgs), c_void_p]
-    library.itk_attention.argtypes = [POINTER(AttentionArgs), c_void_p]
+    # (the argument blocks of these three are passed as raw memory: see CallTemplate)
+    library.itk_plan_pages.argtypes = [c_void_p, c_void_p]
+    library.itk_append_tokens.argtypes = [c_void_p, c_void_p]
+    library.itk_attention.argtypes = [c_void_p, c_void_p]
     library.itk_attention_workspace_bytes.argtypes = [POINTER(AttentionArgs), POINTER(c_size_t)]
     for name in EXPORTED_SYMBOLS:
         function = getattr(library, name)
@@ -218,6 +220,51 @@ def workspace_sizes(rows: int, keys: int, shards: int = 1) -> WorkspaceSizes:
     sizes = WorkspaceSizes()
     check(load_library().itk_workspace_bytes(rows, keys, shards, ctypes.byref(sizes)))
     return sizes
+
+
+class CallTemplate:
+    """What a call with these shapes, strides and types always passes: a checked argument block without its pointers.
+
+    The serving calls are short, and reading and checking the metadata of half a dozen tensors takes longer than the
+    launch.  A call whose tensors have the metadata of an earlier one takes that one's block and fills in the addresses.
+    Nothing about addresses or contents is kept.
+    """
+
+    LIMIT = 1024
+
+    def __init__(self, args: ctypes.Structure, **extra: Any) -> None:
+        self.block = ctypes.c_char * ctypes.sizeof(args)
+        self.bytes = bytes(args)
+        self.__dict__.update(extra)
+
+    def fill(self, *pointers: tuple[int, Any]) -> Any:
+        """A copy of the block with ``(offset, values)`` runs of 64-bit words put in."""
+
+        block = self.block.from_buffer_copy(self.bytes)
+        for offset, values in pointers:
+            struct.pack_into("<%dQ" % len(values), block, offset, *values)
+        return block
+
+    @classmethod
+    def keep(cls, templates: dict, key: Any, template: "CallTemplate") -> "CallTemplate":
+        if len(templates) >= cls.LIMIT:
+            templates.clear()
+        templates[key] = template
+        return template
+
+
+def metadata(tensors: tuple) -> tuple:
+    return tuple([(t.shape, t.stride(), t.dtype, t.device) for t in tensors])
+
+
+def launch(torch: Any, function: Any, block: Any, device: Any) -> None:
+    """Calls a C entry on the current stream of ``device``."""
+
+    if torch.cuda.current_device() == device.index:
+        check(function(block, torch._C._cuda_getCurrentRawStream(device.index)))
+    else:
+        with torch.cuda.device(device):
+            check(function(block, torch._C._cuda_getCurrentRawStream(device.index)))
 
 
 def check_serving_status(device: Any = None) -> None:

@@ -35,41 +35,27 @@ check_status = _lib.check_serving_status
 
 
 def _rows_ok(tensor: Any) -> bool:
-    """Contiguous heads that start on 16-byte boundaries."""
+    """Contiguous heads whose strides keep them on 16-byte boundaries."""
 
     *outer, inner = tensor.stride()
-    return inner == 1 and all(s % 8 == 0 for s in outer) and tensor.data_ptr() % 16 == 0
+    return inner == 1 and all(s % 8 == 0 for s in outer)
 
 
-def _check_kv(torch: Any, q: Any, k: Any, v: Any, what: str, rank: int) -> None:
+def _check_kv(q: Any, k: Any, v: Any, what: str, rank: int) -> None:
     _require(k.dim() == rank and k.shape == v.shape,
              f"{what} keys and values must both have shape {'[N, H, D]' if rank == 3 else '[P, page_size, H, D]'}")
     _require(k.dtype == q.dtype and v.dtype == q.dtype, f"{what} keys and values must have the type of q")
     _require(k.device == q.device and v.device == q.device, f"{what} keys and values must live on the same device as q")
     _require(k.shape[-1] == q.shape[-1], f"{what} keys must have the head dimension of q")
     heads = k.shape[-2]
-    _require(heads > 0 and q.shape[1] % heads == 0 and q.shape[1] // heads <= 128,
+    _require(heads > 0 and q.shape[1] > 0 and q.shape[1] % heads == 0 and q.shape[1] // heads <= 128,
              f"the query heads must be a multiple of the {what} key heads, at most 128 times as many")
     _require(k.numel() == 0 or (_rows_ok(k) and _rows_ok(v)),
              f"{what} keys and values must be contiguous in their last dimension and 16-byte aligned in every row")
-
-
-def _packed_segment(k: Any, v: Any) -> Any:
-    rows = k.shape[0]
-    if rows == 0:
-        return _lib.KvSegment(None, None, None, 0, 0, 0, 0, 0, 0, 0, 1, 0, 0)
-    return _lib.KvSegment(k.data_ptr(), v.data_ptr(), None, 0, 0, k.stride(0), k.stride(1), 0, v.stride(0), v.stride(1), 1, rows, 0)
-
-
-def _paged_segment(k_pool: Any, v_pool: Any, table: Any, table_stride: int) -> Any:
-    return _lib.KvSegment(k_pool.data_ptr(), v_pool.data_ptr(), table.data_ptr(), table_stride, *k_pool.stride()[:3],
-                          *v_pool.stride()[:3], k_pool.shape[0], k_pool.shape[1], table.shape[-1])
-
-
-def _check_pool(k_pool: Any) -> None:
-    pages, page_size = k_pool.shape[:2]
-    _require(pages > 0 and page_size > 0 and page_size % TILE_KEYS == 0, "page_size must be a positive multiple of 128")
-    _require(pages * page_size < 1 << 31, "pages * page_size must stay below 2^31")
+    if rank == 4:
+        pages, page_size = k.shape[:2]
+        _require(pages > 0 and page_size > 0 and page_size % TILE_KEYS == 0, "page_size must be a positive multiple of 128")
+        _require(pages * page_size < 1 << 31, "pages * page_size must stay below 2^31")
 
 
 def _check_ints(torch: Any, tensor: Any, name: str, device: Any, count: int | None) -> None:
@@ -78,52 +64,109 @@ def _check_ints(torch: Any, tensor: Any, name: str, device: Any, count: int | No
     _require(tensor.device == device, f"{name} must live on the same device as q")
 
 
-def _attend(torch: Any, q: Any, kv_heads: int, own: Any, prefix: Any, prefix_keys: int, cu_seqlens_q: Any, cu_seqlens_k: Any,
-            lengths: Any, causal: bool, scale: float | None, out: Any, return_lse: bool) -> Any:
-    tokens, heads, dim = q.shape
-    device = q.device
-    _check_ints(torch, cu_seqlens_q, "cu_seqlens_q", device, None)
-    requests = cu_seqlens_q.shape[0] - 1
-    _require(requests >= 1, "cu_seqlens_q must be [B+1] with B >= 1")
-    if cu_seqlens_k is not None:
-        _check_ints(torch, cu_seqlens_k, "cu_seqlens_k", device, requests + 1)
-    else:
-        _check_ints(torch, lengths, "seqlens_k", device, requests)
-    _require(tokens * heads < 1 << 31, "rows * heads must stay below 2^31")
-    clear_tail = out is None
-    if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=device)
-    else:
-        _require(out.shape == q.shape and out.dtype == q.dtype and out.device == device and (out.numel() == 0 or _rows_ok(out)),
-                 "out must have the shape, type and device of q and 16-byte aligned rows")
-        _require(tokens < 2 or out.stride(0) >= dim and out.stride(1) >= dim or heads == 1 and out.stride(0) >= dim,
-                 "out must not overlap itself")
-    lse = torch.empty((tokens, heads), dtype=torch.float32, device=device) if return_lse else None
-    if tokens:
-        scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
-        _require(0.0 < scale < 1e38, "scale must be positive and finite")
-        args = _lib.AttentionArgs(
-            q.data_ptr(), out.data_ptr(), _lib.ptr(lse), cu_seqlens_q.data_ptr(), _lib.ptr(cu_seqlens_k), _lib.ptr(lengths),
-            None, 0, q.stride(0), q.stride(1), out.stride(0), out.stride(1), 0, own, prefix, scale,
-            _lib.ELEMENT_BF16 if q.dtype == torch.bfloat16 else _lib.ELEMENT_FP16, tokens, heads, kv_heads, dim, requests,
-            prefix_keys, int(causal), int(clear_tail), 0)
-        library = _lib.load_library()
-        needed = ctypes.c_size_t(0)
-        _lib.check(library.itk_attention_workspace_bytes(ctypes.byref(args), ctypes.byref(needed)))
-        with torch.cuda.device(device):
-            # of the caching allocator, on the call's stream: two calls, streams or captured graphs never share it
-            workspace = torch.empty(needed.value, dtype=torch.uint8, device=device)
-            args.workspace, args.workspace_bytes = workspace.data_ptr(), needed.value
-            _lib.check(library.itk_attention(ctypes.byref(args), _lib.current_stream(torch, device)))
-    return (out, lse) if return_lse else out
+def _segment(k: Any, v: Any, table: Any = None) -> Any:
+    """Strides and sizes of packed (``table`` is None) or paged keys, without their addresses."""
+
+    if table is None:
+        return _lib.KvSegment(None, None, None, 0, 0, k.stride(0), k.stride(1), 0, v.stride(0), v.stride(1), 1, k.shape[0], 0)
+    return _lib.KvSegment(None, None, None, table.stride(0) if table.dim() == 2 else 0, *k.stride()[:3], *v.stride()[:3],
+                          k.shape[0], k.shape[1], table.shape[-1])
 
 
-def _check_q(torch: Any, q: Any) -> None:
+def _check_call(torch: Any, q: Any, own: tuple, prefix: tuple | None, prefix_keys: int, cu_seqlens_q: Any, lengths: Any, out: Any,
+                causal: bool, scale: float | None) -> _lib.CallTemplate:
+    """``own`` and ``prefix`` are ``(k, v)`` packed or ``(k_pool, v_pool, table)``; ``lengths`` are cumulative for packed keys."""
+
     _require(q.is_cuda, "q must be a CUDA tensor (there is no CPU path)")
     _require(q.dim() == 3, "q must have shape [T, Hq, D]")
     _require(q.dtype in (torch.bfloat16, torch.float16), "q must be bfloat16 or float16")
-    _require(q.shape[2] in (64, 128), "the head dimension must be 64 or 128")
+    tokens, heads, dim = q.shape
+    device = q.device
+    _require(dim in (64, 128), "the head dimension must be 64 or 128")
     _require(q.numel() == 0 or _rows_ok(q), "q must be contiguous in its last dimension and 16-byte aligned in every row")
+    _require(tokens * heads < 1 << 31, "rows * heads must stay below 2^31")
+    paged = len(own) == 3
+    _check_kv(q, own[0], own[1], "own", 4 if paged else 3)
+    _check_ints(torch, cu_seqlens_q, "cu_seqlens_q", device, None)
+    requests = cu_seqlens_q.shape[0] - 1
+    _require(requests >= 1, "cu_seqlens_q must be [B+1] with B >= 1")
+    if paged:
+        table = own[2]
+        _require(table.dtype == torch.int32 and table.dim() == 2, "block_table must be int32 [B, table_pages]")
+        _require(table.shape[0] == requests, "block_table must have one row per request")
+        _require(table.shape[1] > 0, "block_table must have at least one column")
+        _require(table.device == device, "block_table must live on the same device as q")
+        _require((table.stride(1) == 1 or table.shape[1] == 1) and table.stride(0) >= 0, "block_table rows must be contiguous")
+        _check_ints(torch, lengths, "seqlens_k", device, requests)
+    else:
+        _check_ints(torch, lengths, "cu_seqlens_k", device, requests + 1)
+    if prefix is not None:
+        _check_kv(q, prefix[0], prefix[1], "prefix", 4 if paged else 3)
+        _require(prefix[0].shape[-2] == own[0].shape[-2], "prefix and own keys must have the same heads")
+        if paged:
+            _check_ints(torch, prefix[2], "prefix_table", device, None)
+            _require(0 <= prefix_keys <= prefix[2].shape[0] * own[0].shape[1], "prefix_table does not cover the prefix keys")
+    if out is not None:
+        _require(out.shape == q.shape and out.dtype == q.dtype and out.device == device and (out.numel() == 0 or _rows_ok(out)),
+                 "out must have the shape, type and device of q and 16-byte aligned rows")
+        strides = sorted((s, n) for s, n in zip(out.stride()[:2], out.shape[:2]) if n > 1)
+        _require(all(s >= dim for s, _ in strides) and (len(strides) < 2 or strides[1][0] >= strides[0][0] * strides[0][1]),
+                 "out must not overlap itself")
+    scale = 1.0 / math.sqrt(dim) if scale is None else scale
+    _require(0.0 < scale < 1e38, "scale must be positive and finite")
+    strides = out.stride() if out is not None else (heads * dim, dim)
+    args = _lib.AttentionArgs(
+        None, None, None, None, None, None, None, 0, q.stride(0), q.stride(1), strides[0], strides[1], 0, _segment(*own),
+        _segment(*prefix) if prefix_keys else _lib.KvSegment(), scale,
+        _lib.ELEMENT_BF16 if q.dtype == torch.bfloat16 else _lib.ELEMENT_FP16, tokens, heads, own[0].shape[-2], dim, requests,
+        prefix_keys, int(causal), int(out is None), 0)
+    needed = ctypes.c_size_t(0)
+    if tokens:
+        _lib.check(_lib.load_library().itk_attention_workspace_bytes(ctypes.byref(args), ctypes.byref(needed)))
+    return _lib.CallTemplate(args, workspace_bytes=needed.value, device=device, tokens=tokens)
+
+
+_TEMPLATES: dict = {}
+_OWN_OFFSET = _lib.AttentionArgs.own.offset
+_PREFIX_OFFSET = _lib.AttentionArgs.prefix.offset
+
+
+def _attend(q: Any, own: tuple, prefix: tuple | None, prefix_keys: int, cu_seqlens_q: Any, lengths: Any, causal: bool,
+            scale: float | None, out: Any, return_lse: bool) -> Any:
+    import torch
+
+    tensors = (q, cu_seqlens_q, lengths, *own)
+    if prefix is not None:
+        tensors += prefix
+    if out is not None:
+        tensors += (out,)
+    if scale is not None:
+        scale = float(scale)
+    key = (_lib.metadata(tensors), len(own), prefix is not None, prefix_keys, bool(causal), scale)
+    template = _TEMPLATES.get(key)
+    if template is None:
+        template = _lib.CallTemplate.keep(_TEMPLATES, key, _check_call(
+            torch, q, own, prefix, prefix_keys, cu_seqlens_q, lengths, out, causal, scale))
+    device, tokens = template.device, template.tokens
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=device) if return_lse else None
+    if tokens:
+        # of the caching allocator, on the call's stream: two calls, streams or captured graphs never share it
+        workspace = torch.empty(template.workspace_bytes, dtype=torch.uint8, device=device)
+        row_addresses = (q.data_ptr(), out.data_ptr())
+        own_addresses = [t.data_ptr() for t in own]
+        prefix_addresses = [t.data_ptr() for t in prefix] if prefix_keys else []
+        for address in (*row_addresses, *own_addresses[:2], *prefix_addresses[:2]):
+            _require(address % 16 == 0, "q, out, keys and values must be 16-byte aligned")
+        paged = len(own) == 3
+        block = template.fill(
+            (0, (*row_addresses, 0 if lse is None else lse.data_ptr(), cu_seqlens_q.data_ptr(),
+                 0 if paged else lengths.data_ptr(), lengths.data_ptr() if paged else 0, workspace.data_ptr(),
+                 template.workspace_bytes)),
+            (_OWN_OFFSET, own_addresses), (_PREFIX_OFFSET, prefix_addresses))
+        _lib.launch(torch, _lib.load_library().itk_attention, block, device)
+    return (out, lse) if return_lse else out
 
 
 def attention_varlen(q: Any, kv: tuple[Any, Any], cu_seqlens_q: Any, cu_seqlens_k: Any, *, causal: bool = True,
@@ -136,26 +179,7 @@ def attention_varlen(q: Any, kv: tuple[Any, Any], cu_seqlens_q: Any, cu_seqlens_
     defaults to ``D ** -0.5``.  Rows behind the last request are zero (log-sum-exp ``-inf``), or left as they were in a given ``out``.
     """
 
-    import torch
-
-    k, v = kv
-    _check_q(torch, q)
-    _check_kv(torch, q, k, v, "own", 3)
-    return _attend(torch, q, k.shape[1], _packed_segment(k, v), _lib.KvSegment(), 0, cu_seqlens_q, cu_seqlens_k, None, causal, scale,
-                   out, return_lse)
-
-
-def _own_pages(torch: Any, q: Any, pools: tuple[Any, Any], block_table: Any, cu_seqlens_q: Any) -> Any:
-    k_pool, v_pool = pools
-    _check_q(torch, q)
-    _check_kv(torch, q, k_pool, v_pool, "own", 4)
-    _check_pool(k_pool)
-    _require(block_table.dtype == torch.int32 and block_table.dim() == 2, "block_table must be int32 [B, table_pages]")
-    _require(block_table.shape[0] == cu_seqlens_q.shape[0] - 1, "block_table must have one row per request")
-    _require(block_table.shape[1] > 0, "block_table must have at least one column")
-    _require(block_table.device == q.device, "block_table must live on the same device as q")
-    _require(block_table.stride(1) == 1 or block_table.shape[1] == 1, "block_table rows must be contiguous")
-    return _paged_segment(k_pool, v_pool, block_table, block_table.stride(0))
+    return _attend(q, tuple(kv), None, 0, cu_seqlens_q, cu_seqlens_k, causal, scale, out, return_lse)
 
 
 def attention_paged(q: Any, pools: tuple[Any, Any], block_table: Any, cu_seqlens_q: Any, seqlens_k: Any, *, causal: bool = True,
@@ -167,10 +191,7 @@ def attention_paged(q: Any, pools: tuple[Any, Any], block_table: Any, cu_seqlens
     ``check_status``.
     """
 
-    import torch
-
-    own = _own_pages(torch, q, pools, block_table, cu_seqlens_q)
-    return _attend(torch, q, pools[0].shape[2], own, _lib.KvSegment(), 0, cu_seqlens_q, None, seqlens_k, causal, scale, out, return_lse)
+    return _attend(q, (*pools, block_table), None, 0, cu_seqlens_q, seqlens_k, causal, scale, out, return_lse)
 
 
 def shared_prefix_attention(q: Any, prefix_kv: tuple[Any, Any], kv: tuple[Any, Any], cu_seqlens_q: Any, cu_seqlens_k: Any, *,
@@ -181,16 +202,7 @@ def shared_prefix_attention(q: Any, prefix_kv: tuple[Any, Any], kv: tuple[Any, A
     prefix is attended by the rows of all requests together, so its keys and values are read once for the batch.
     """
 
-    import torch
-
-    k, v = kv
-    k_prefix, v_prefix = prefix_kv
-    _check_q(torch, q)
-    _check_kv(torch, q, k, v, "own", 3)
-    _check_kv(torch, q, k_prefix, v_prefix, "prefix", 3)
-    _require(k_prefix.shape[1] == k.shape[1], "prefix and own keys must have the same heads")
-    return _attend(torch, q, k.shape[1], _packed_segment(k, v), _packed_segment(k_prefix, v_prefix), k_prefix.shape[0],
-                   cu_seqlens_q, cu_seqlens_k, None, True, scale, out, return_lse)
+    return _attend(q, tuple(kv), tuple(prefix_kv), prefix_kv[0].shape[0], cu_seqlens_q, cu_seqlens_k, True, scale, out, return_lse)
 
 
 def shared_prefix_attention_paged(q: Any, pools: tuple[Any, Any], prefix_table: Any, prefix_keys: int, block_table: Any,
@@ -202,14 +214,8 @@ def shared_prefix_attention_paged(q: Any, pools: tuple[Any, Any], prefix_table: 
     request's own keys, which start on a page of their own.
     """
 
-    import torch
-
-    own = _own_pages(torch, q, pools, block_table, cu_seqlens_q)
-    prefix_keys = int(prefix_keys)
-    _check_ints(torch, prefix_table, "prefix_table", q.device, None)
-    _require(0 <= prefix_keys <= prefix_table.shape[0] * pools[0].shape[1], "prefix_table does not cover the prefix keys")
-    prefix = _paged_segment(pools[0], pools[1], prefix_table, 0) if prefix_keys else _lib.KvSegment()
-    return _attend(torch, q, pools[0].shape[2], own, prefix, prefix_keys, cu_seqlens_q, None, seqlens_k, True, scale, out, return_lse)
+    return _attend(q, (*pools, block_table), (*pools, prefix_table), int(prefix_keys), cu_seqlens_q, seqlens_k, True, scale, out,
+                   return_lse)
 
 
 __all__ = ["attention_paged", "attention_varlen", "check_status", "shared_prefix_attention", "shared_prefix_attention_paged"]

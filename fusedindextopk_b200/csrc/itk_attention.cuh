@@ -73,9 +73,12 @@ struct AttnItem {
     int partial, slot, slots; // row of the partial results of the whole entry (-1: write the output), first slot, slots
 };
 
+// Up to kAttnCombineRows rows (of every key head) that have partial results to join.
+constexpr int kAttnCombineRows = 16;
 struct AttnCombine {
-    int q_first, tokens;
-    int partial, slots;       // own partial results
+    int q_first, tokens;      // of the entry they belong to
+    int partial, slots;       // own partial results of the entry
+    int row_first, pad[3];
 };
 
 struct AttnCounters {
@@ -90,7 +93,7 @@ struct AttnWorkspace {
     AttnCombine* combines;
     float* partial_lse;       // log2 of the sum of exponentials of a partial row
     float* partial_out;       // [partial_rows, DIM], normalised
-    int max_items, max_combines, max_partial_rows;
+    int max_items, max_entries, max_combines, max_partial_rows;     // max_entries: own ones
 };
 
 struct AttnParams {
@@ -261,7 +264,6 @@ __device__ __forceinline__ AttnRequest attn_request(const itk_attention_args& p,
     return r;
 }
 
-constexpr int kAttnPlanThreads = 1024;
 constexpr int kAttnBins = 256;
 constexpr int kAttnTries = 8;
 constexpr int kAttnMinChunk = 2;    // key tiles of a chunk at least: below that a chunk's fixed cost outweighs its keys
@@ -332,13 +334,17 @@ __device__ __forceinline__ AttnEntry attn_entry(const AttnParams& p, const AttnR
     return r;
 }
 
-__device__ __forceinline__ int attn_chunks(const AttnEntry& e, long long cost) {
-    const long long per = max(static_cast<long long>(kAttnMinChunk), (cost + e.unit - 1) / e.unit);
-    return static_cast<int>((e.tiles + per - 1) / per);
+// Key chunks of an entry when a chunk may cost `cost`.
+__device__ __forceinline__ int attn_chunks(const AttnEntry& e, int cost) {
+    const int per = max(kAttnMinChunk, cost / e.unit + (cost % e.unit != 0));
+    return (e.tiles + per - 1) / per;
 }
 
-__global__ void __launch_bounds__(kAttnPlanThreads) itk_attention_plan_kernel(const __grid_constant__ AttnParams p) {
-    __shared__ int warp_sums[kAttnPlanThreads / 32];
+// Most of a small call's time before its first key is read goes by in here: one pass over the lengths, entries kept in
+// registers, five block barriers when the items fit one wave (their order does not matter then).
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) itk_attention_plan_kernel(const __grid_constant__ AttnParams p) {
+    __shared__ int warp_sums[THREADS / 32];
     __shared__ int carry, rows_end;
     __shared__ unsigned long long total_cost;
     __shared__ int counts[kAttnTries], longest, item_count, combine_count, partial_rows;
@@ -358,12 +364,12 @@ __global__ void __launch_bounds__(kAttnPlanThreads) itk_attention_plan_kernel(co
     }
     if (tx == 32) rows_end = min(max(p.a.cu_q[p.a.requests], 0), p.a.tokens);
     if (tx < kAttnTries) counts[tx] = 0;
-    if (tx < kAttnBins) bins[tx] = 0;
+    for (int i = tx; i < kAttnBins; i += THREADS) bins[i] = 0;
     // (the barriers of the first pass below stand between these and their first readers: there is at least one request)
 
     // own entries before every request
     bool bad = false;
-    for (int base = 0; base < p.a.requests; base += kAttnPlanThreads) {
+    for (int base = 0; base < p.a.requests; base += THREADS) {
         const int b = base + tx;
         int mine = 0;
         if (b < p.a.requests) {
@@ -383,111 +389,126 @@ __global__ void __launch_bounds__(kAttnPlanThreads) itk_attention_plan_kernel(co
         for (int w = 0; w < warp; ++w) before += warp_sums[w];
         if (b < p.a.requests) entry_first[b] = before + upto - mine;
         __syncthreads();
-        if (tx == kAttnPlanThreads - 1) carry = before + upto;
-        __syncthreads();
+        if (tx == THREADS - 1) carry = before + upto;
     }
     if (bad) atomicOr(p.status, ITK_SERVING_BAD_LENGTHS);
-    const int prefix_entries = p.a.prefix_keys > 0 ? (rows_end + span - 1) / span : 0;
-    const int own_entries = min(carry, p.w.max_combines);
-    const int entries = prefix_entries + own_entries;
-    if (tx == 0) entry_first[p.a.requests] = own_entries;
     __syncthreads();
+    const int prefix_entries = p.a.prefix_keys > 0 ? (rows_end + span - 1) / span : 0;
+    const int entries = prefix_entries + min(carry, p.w.max_entries);
 
-    // every thread keeps its first entry; batches of more than 1024 entries work the others out again in every pass
-    AttnEntry kept;
+    // every thread keeps its first entry; larger batches work the others out again in every pass
+    AttnEntry kept{};
     if (tx < entries) kept = attn_entry(p, requests, tx, prefix_entries, rows_end);
     auto entry_at = [&](int e) { return e == tx ? kept : attn_entry(p, requests, e, prefix_entries, rows_end); };
 
     // the chunk length that spreads the work over the SMs in one wave, if there is one
     unsigned long long cost = 0;
-    for (int e = tx; e < entries; e += kAttnPlanThreads) {
+    for (int e = tx; e < entries; e += THREADS) {
         const AttnEntry entry = entry_at(e);
         cost += static_cast<unsigned long long>(entry.tiles) * entry.unit;
     }
-    if (cost != 0) atomicAdd(&total_cost, cost);
+#pragma unroll
+    for (int step = 16; step > 0; step >>= 1) cost += __shfl_xor_sync(0xffffffffu, cost, step);
+    if (lane == 0 && cost != 0) atomicAdd(&total_cost, cost);
     __syncthreads();
-    const long long share = max(1ll, (static_cast<long long>(total_cost) * kv_heads + p.sm_count - 1) / p.sm_count);
+    // (a chunk is at most 2^30 long: longer than any entry, 2^24 tiles of cost 4, can be)
+    const unsigned long long fair = (total_cost * kv_heads + p.sm_count - 1) / p.sm_count;
+    const int share = static_cast<int>(min(max(fair, 1ull), 1ull << 29));
     int mine[kAttnTries] = {};
-    for (int e = tx; e < entries; e += kAttnPlanThreads) {
+    for (int e = tx; e < entries; e += THREADS) {
         const AttnEntry entry = entry_at(e);
 #pragma unroll
-        for (int k = 0; k < kAttnTries; ++k) mine[k] += attn_chunks(entry, share + share * k / kAttnTries);
+        for (int k = 0; k < kAttnTries; ++k) mine[k] += max(1, attn_chunks(entry, share + share / kAttnTries * k));
     }
 #pragma unroll
-    for (int k = 0; k < kAttnTries; ++k)
-        if (mine[k] != 0) atomicAdd(&counts[k], mine[k]);
+    for (int k = 0; k < kAttnTries; ++k) {
+        const int sum = __reduce_add_sync(0xffffffffu, mine[k]);
+        if (lane == 0 && sum != 0) atomicAdd(&counts[k], sum);
+    }
     __syncthreads();
-    long long chunk = share;
+    int chunk = share;
+    bool one_wave = false;
     for (int k = kAttnTries - 1; k >= 0; --k)
-        if (static_cast<long long>(counts[k]) * kv_heads <= p.sm_count) chunk = share + share * k / kAttnTries;
+        if (static_cast<long long>(counts[k]) * kv_heads <= p.sm_count) {
+            chunk = share + share / kAttnTries * k;
+            one_wave = true;
+        }
 
-    // items by cost, the costliest first: a counting sort over 256 cost classes
-    for (int e = tx; e < entries; e += kAttnPlanThreads) {
-        const AttnEntry entry = entry_at(e);
-        const int chunks = max(1, attn_chunks(entry, chunk));
-        atomicMax(&longest, (entry.tiles + chunks - 1) / chunks * entry.unit);
-    }
-    __syncthreads();
-    const int top = max(longest, 1);
-    for (int e = tx; e < entries; e += kAttnPlanThreads) {
-        const AttnEntry entry = entry_at(e);
-        const int chunks = max(1, attn_chunks(entry, chunk));
+    // more than a wave: the costliest items first, by a counting sort over 256 cost classes
+    int top = 1;
+    auto bin_of = [&](const AttnEntry& entry, int chunks) {
         const int item_cost = (entry.tiles + chunks - 1) / chunks * entry.unit;
-        const int bin = kAttnBins - 1 - static_cast<int>(static_cast<long long>(item_cost) * (kAttnBins - 1) / top);
-        atomicAdd(&bins[bin], chunks);
+        return kAttnBins - 1 - static_cast<int>(static_cast<long long>(item_cost) * (kAttnBins - 1) / top);
+    };
+    if (!one_wave) {
+        int most = 0;
+        for (int e = tx; e < entries; e += THREADS) {
+            const AttnEntry entry = entry_at(e);
+            const int chunks = max(1, attn_chunks(entry, chunk));
+            most = max(most, (entry.tiles + chunks - 1) / chunks * entry.unit);
+        }
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 0) atomicMax(&longest, most);
+        __syncthreads();
+        top = max(longest, 1);
+        for (int e = tx; e < entries; e += THREADS) {
+            const AttnEntry entry = entry_at(e);
+            const int chunks = max(1, attn_chunks(entry, chunk));
+            atomicAdd(&bins[bin_of(entry, chunks)], chunks);
+        }
+        __syncthreads();
+        if (warp == 0) {
+            int sum = 0, held[kAttnBins / 32];
+#pragma unroll
+            for (int i = 0; i < kAttnBins / 32; ++i) {
+                held[i] = bins[lane * (kAttnBins / 32) + i];
+                sum += held[i];
+            }
+            int upto = sum;
+#pragma unroll
+            for (int step = 1; step < 32; step <<= 1) {
+                const int other = __shfl_up_sync(0xffffffffu, upto, step);
+                if (lane >= step) upto += other;
+            }
+            int before = upto - sum;
+#pragma unroll
+            for (int i = 0; i < kAttnBins / 32; ++i) {
+                bins[lane * (kAttnBins / 32) + i] = before;
+                before += held[i];
+            }
+            if (lane == 31) item_count = before;
+        }
+        __syncthreads();
     }
-    __syncthreads();
-    if (warp == 0) {
-        int sum = 0, held[kAttnBins / 32];
-#pragma unroll
-        for (int i = 0; i < kAttnBins / 32; ++i) {
-            held[i] = bins[lane * (kAttnBins / 32) + i];
-            sum += held[i];
-        }
-        int upto = sum;
-#pragma unroll
-        for (int step = 1; step < 32; step <<= 1) {
-            const int other = __shfl_up_sync(0xffffffffu, upto, step);
-            if (lane >= step) upto += other;
-        }
-        int before = upto - sum;
-#pragma unroll
-        for (int i = 0; i < kAttnBins / 32; ++i) {
-            bins[lane * (kAttnBins / 32) + i] = before;
-            before += held[i];
-        }
-        if (lane == 31) item_count = before;
-    }
-    __syncthreads();
-    for (int e = tx; e < entries; e += kAttnPlanThreads) {
+    for (int e = tx; e < entries; e += THREADS) {
         AttnEntry entry = entry_at(e);
         const int chunks = attn_chunks(entry, chunk);               // 0: no key at all
         const int longest_chunk = chunks > 0 ? (entry.tiles + chunks - 1) / chunks : 0;
         const int lanes = !entry.pair && longest_chunk > 1 ? 2 : 1;
+        const int rows = entry.item.tokens * p.group;
         entry.item.slots = chunks * lanes;
         entry.item.partial = -1;
         const bool joined = p.a.prefix_keys > 0 || entry.item.slots > 1;
         if (joined && entry.item.slots > 0) {
-            const int rows = entry.item.slots * entry.item.tokens * p.group * kv_heads;
-            const int first = atomicAdd(&partial_rows, rows);
+            const int needed = entry.item.slots * rows * kv_heads;
+            const int first = atomicAdd(&partial_rows, needed);
             // (the host sizes the buffer so that this always fits; nothing is written behind it if it did not)
-            entry.item.partial = first + rows <= p.w.max_partial_rows ? first : -2;
+            entry.item.partial = first + needed <= p.w.max_partial_rows ? first : -2;
             if (entry.item.partial == -2) atomicOr(p.status, ITK_SERVING_BAD_LENGTHS);
         }
+        const int usable = entry.item.partial < 0 ? 0 : entry.item.slots;
         if (entry.prefix) {
-            p.w.prefix_slots[e] = make_int2(entry.item.partial, entry.item.partial < 0 ? 0 : entry.item.slots);
+            p.w.prefix_slots[e] = make_int2(entry.item.partial, usable);
         } else if (joined) {
-            const int at = atomicAdd(&combine_count, 1);
-            p.w.combines[at] = AttnCombine{entry.item.q_first, entry.item.tokens, entry.item.partial,
-                                           entry.item.partial < 0 ? 0 : entry.item.slots};
+            const int records = (rows + kAttnCombineRows - 1) / kAttnCombineRows;
+            const int at = atomicAdd(&combine_count, records);
+            for (int r = 0; r < records; ++r)
+                if (at + r < p.w.max_combines)
+                    p.w.combines[at + r] = AttnCombine{entry.item.q_first, entry.item.tokens, entry.item.partial, usable, r * kAttnCombineRows, {}};
         }
-        if (chunks == 0 && joined) {        // the prefix alone: a place in the list, but nothing to do
-            entry.item.tokens = 0;
-        }
+        if (chunks == 0 && joined) entry.item.tokens = 0;           // the prefix alone: a place in the list, but nothing to do
         const int count = max(1, chunks);
-        const int item_cost = (entry.tiles + count - 1) / count * entry.unit;
-        const int bin = kAttnBins - 1 - static_cast<int>(static_cast<long long>(item_cost) * (kAttnBins - 1) / top);
-        const int place = atomicAdd(&bins[bin], count);
+        const int place = atomicAdd(one_wave ? &item_count : &bins[bin_of(entry, count)], count);
         for (int c = 0; c < count; ++c) {
             const long long lo = static_cast<long long>(entry.tiles) * c / count, hi = static_cast<long long>(entry.tiles) * (c + 1) / count;
             entry.item.tile_begin = static_cast<int>(lo);
@@ -497,7 +518,7 @@ __global__ void __launch_bounds__(kAttnPlanThreads) itk_attention_plan_kernel(co
         }
     }
     __syncthreads();
-    if (tx == 0) *p.w.counters = AttnCounters{min(item_count, p.w.max_items), combine_count, partial_rows, rows_end};
+    if (tx == 0) *p.w.counters = AttnCounters{min(item_count, p.w.max_items), min(combine_count, p.w.max_combines), partial_rows, rows_end};
 }
 
 // ------------------------------------------------------------------ attention
@@ -538,13 +559,14 @@ struct AttnWalk {
         for (;;) {
             const int grid = static_cast<int>(gridDim.x), me = static_cast<int>(blockIdx.x);
             const long long at = static_cast<long long>(wave) * grid + ((wave & 1) ? grid - 1 - me : me);
+            const int index = static_cast<int>(at / heads);
+            // read before it is known whether there is such an item: the two loads overlap
+            const int4* source = reinterpret_cast<const int4*>(p.w.items + min(index, p.w.max_items - 1));
+            const int4 a = source[0], b = source[1], c = source[2];
             if (static_cast<long long>(wave) * grid >= total) return false;
             ++wave;
             if (at >= total) continue;
-            const int index = static_cast<int>(at) / heads;
-            head = static_cast<int>(at) - index * heads;
-            const int4* source = reinterpret_cast<const int4*>(p.w.items + index);
-            const int4 a = source[0], b = source[1], c = source[2];
+            head = static_cast<int>(at - static_cast<long long>(index) * heads);
             item = AttnItem{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, c.x, c.y, c.z, c.w};
             if (item.tokens > 0) return true;
         }
@@ -1083,8 +1105,8 @@ __global__ void __launch_bounds__(kJoinThreads) itk_attention_join_kernel(const 
     for (int work = blockIdx.x; work < counters.combines * heads; work += gridDim.x) {
         const AttnCombine entry = p.w.combines[work / heads];
         const int head = work % heads;
-        const int rows = entry.tokens * p.group;
-        for (int r = warp; r < rows; r += kJoinThreads / 32) {
+        const int rows = entry.tokens * p.group, row_end = min(rows, entry.row_first + kAttnCombineRows);
+        for (int r = entry.row_first + warp; r < row_end; r += kJoinThreads / 32) {
             const int token = entry.q_first + r / p.group;
             const int head_index = head * p.group + r % p.group;
             // two runs of partial rows: first row, distance, count

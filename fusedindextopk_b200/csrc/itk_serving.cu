@@ -116,14 +116,17 @@ int attention_workspace(const itk_attention_args& a, AttnWorkspace* w, size_t* b
         at += (size + 255) / 256 * 256;
         return static_cast<char*>(a.workspace) + offset;
     };
-    w->max_combines = static_cast<int>(own);
+    const long long combines = (rows / a.kv_heads + kAttnCombineRows - 1) / kAttnCombineRows + own;
+    ITK_REQUIRE(combines * a.kv_heads < (1ll << 31), "the batch is too large for one call");
+    w->max_entries = static_cast<int>(own);
+    w->max_combines = static_cast<int>(combines);
     w->max_items = static_cast<int>(own + prefix + kAttnMaxSms);
     w->max_partial_rows = static_cast<int>(partial);
     w->counters = reinterpret_cast<AttnCounters*>(take(sizeof(AttnCounters)));
     w->entry_first = reinterpret_cast<int*>(take((static_cast<size_t>(a.requests) + 1) * sizeof(int)));
     w->prefix_slots = reinterpret_cast<int2*>(take(static_cast<size_t>(prefix) * sizeof(int2)));
     w->items = reinterpret_cast<AttnItem*>(take(static_cast<size_t>(w->max_items) * sizeof(AttnItem)));
-    w->combines = reinterpret_cast<AttnCombine*>(take(static_cast<size_t>(own) * sizeof(AttnCombine)));
+    w->combines = reinterpret_cast<AttnCombine*>(take(static_cast<size_t>(combines) * sizeof(AttnCombine)));
     w->partial_lse = reinterpret_cast<float*>(take(static_cast<size_t>(partial) * sizeof(float)));
     w->partial_out = reinterpret_cast<float*>(take(static_cast<size_t>(partial) * a.dim * sizeof(float)));
     *bytes = at;
@@ -174,7 +177,11 @@ cudaError_t launch_after(Kernel kernel, int grid, int threads, size_t smem, cuda
 
 template <typename T, int DIM>
 int launch_attention(const AttnParams& params, cudaStream_t stream) {
-    itk_attention_plan_kernel<<<1, kAttnPlanThreads, 0, stream>>>(params);
+    // barriers of a small block cost a third of a large one's; the large one is for batches with more entries than threads
+    if (params.w.max_entries <= 256)
+        itk_attention_plan_kernel<256><<<1, 256, 0, stream>>>(params);
+    else
+        itk_attention_plan_kernel<1024><<<1, 1024, 0, stream>>>(params);
     ITK_CUDA(launch_after(itk_attention_kernel<T, DIM>, params.sm_count, kAttnThreads, AttnShape<DIM>::kSmemBytes, stream, params));
     ITK_CUDA(launch_after(itk_attention_join_kernel<T, DIM>, 4 * params.sm_count, kJoinThreads, 0, stream, params));
     return launched("itk_attention_kernel");

@@ -23,8 +23,7 @@ to those slots; ``attention.attention_paged`` reads them.
 
 from __future__ import annotations
 
-import ctypes
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Any
 
 from . import _lib
@@ -195,6 +194,7 @@ class PagePlan:
     k_end: Any
     pages_needed: Any
     block_table: Any = None
+    templates: dict = field(default_factory=dict, repr=False)     # checked argument blocks, with this plan's own buffers
 
 
 def make_page_plan(requests: int, table_pages: int, rows: int, *, page_size: int, device: Any) -> PagePlan:
@@ -233,6 +233,18 @@ def plan_pages(plan: PagePlan, block_table: Any, lengths: Any, new_tokens: Any, 
 
     import torch
 
+    tensors = (block_table, lengths, new_tokens, free_pages)
+    key = _lib.metadata(tensors)
+    template = plan.templates.get(key)
+    if template is None:
+        template = _lib.CallTemplate.keep(plan.templates, key, _check_plan(torch, plan, *tensors))
+    block = template.fill((0, [t.data_ptr() for t in tensors]))
+    _lib.launch(torch, _lib.load_library().itk_plan_pages, block, plan.slots.device)
+    plan.block_table = block_table
+    return plan
+
+
+def _check_plan(torch: Any, plan: PagePlan, block_table: Any, lengths: Any, new_tokens: Any, free_pages: Any) -> _lib.CallTemplate:
     rows, requests = plan.rows, plan.requests
     device = plan.slots.device
     for name, tensor, count in (("lengths", lengths, requests), ("new_tokens", new_tokens, requests),
@@ -245,15 +257,10 @@ def plan_pages(plan: PagePlan, block_table: Any, lengths: Any, new_tokens: Any, 
     _require(block_table.device == device, "block_table must live on the plan's device")
     _require((block_table.stride(1) == 1 or plan.table_pages == 1) and (block_table.stride(0) >= plan.table_pages or requests == 1),
              "block_table rows must be contiguous and must not overlap")
-    args = _lib.PagePlanArgs(
-        block_table.data_ptr(), lengths.data_ptr(), new_tokens.data_ptr(), free_pages.data_ptr(), plan.slots.data_ptr(),
-        plan.cu_seqlens_q.data_ptr(), plan.lengths.data_ptr(), plan.flat_table.data_ptr(), plan.k_start.data_ptr(),
-        plan.k_end.data_ptr(), plan.pages_needed.data_ptr(), max(block_table.stride(0), plan.table_pages), requests,
-        plan.table_pages, plan.page_size, free_pages.shape[0], rows)
-    with torch.cuda.device(device):
-        _lib.check(_lib.load_library().itk_plan_pages(ctypes.byref(args), _lib.current_stream(torch, device)))
-    plan.block_table = block_table
-    return plan
+    return _lib.CallTemplate(_lib.PagePlanArgs(
+        None, None, None, None, plan.slots.data_ptr(), plan.cu_seqlens_q.data_ptr(), plan.lengths.data_ptr(),
+        plan.flat_table.data_ptr(), plan.k_start.data_ptr(), plan.k_end.data_ptr(), plan.pages_needed.data_ptr(),
+        max(block_table.stride(0), plan.table_pages), requests, plan.table_pages, plan.page_size, free_pages.shape[0], rows))
 
 
 def append_tokens(slots: Any, kv: tuple[Any, Any], pools: tuple[Any, Any], *, index_keys: Any = None,
@@ -274,11 +281,31 @@ def append_tokens(slots: Any, kv: tuple[Any, Any], pools: tuple[Any, Any], *, in
 
     k, v = kv
     k_pool, v_pool = pools
+    tensors = (slots, k, v, k_pool, v_pool)
+    if index_keys is not None or index_pools is not None:
+        _require(index_keys is not None and index_pools is not None, "index_keys and index_pools go together")
+        tensors += (index_keys, *index_pools)
+    key = _lib.metadata(tensors)
+    template = _APPEND_TEMPLATES.get(key)
+    if template is None:
+        template = _lib.CallTemplate.keep(_APPEND_TEMPLATES, key, _check_append(torch, *tensors))
+    addresses = [t.data_ptr() for t in tensors]
+    for name, address in zip(("k", "v", "k_pool", "v_pool", "index_keys", "index_pool"), addresses[1:7]):
+        _require(address % 16 == 0, f"{name} must be 16-byte aligned")
+    _lib.launch(torch, _lib.load_library().itk_append_tokens, template.fill((0, addresses)), template.device)
+
+
+_APPEND_TEMPLATES: dict = {}
+
+
+def _check_append(torch: Any, slots: Any, k: Any, v: Any, k_pool: Any, v_pool: Any, index_keys: Any = None, index_pool: Any = None,
+                  index_scales: Any = None) -> _lib.CallTemplate:
     _require(k.is_cuda, "k must be a CUDA tensor (there is no CPU path)")
     device = k.device
     _require(k.dim() == 3 and k.shape == v.shape, "k and v must both have shape [T, H, D]")
     tokens, heads, dim = k.shape
     _require(dim in (64, 128), "the head dimension must be 64 or 128")
+    _require(heads > 0, "need at least one head")
     _require(k.dtype in (torch.bfloat16, torch.float16), "k and v must be bfloat16 or float16")
     _require(k_pool.dim() == 4 and k_pool.shape == v_pool.shape and tuple(k_pool.shape[2:]) == (heads, dim),
              "the pools must both have shape [P, page_size, H, D]")
@@ -288,18 +315,16 @@ def append_tokens(slots: Any, kv: tuple[Any, Any], pools: tuple[Any, Any], *, in
     for name, tensor in (("k", k), ("v", v), ("k_pool", k_pool), ("v_pool", v_pool)):
         _require(tensor.dtype == k.dtype, f"{name} must have the type of k")
         _require(tensor.device == device, f"{name} must live on the same device as k")
-        _require(tensor.stride(-1) == 1 and all(s % 8 == 0 for s in tensor.stride()[:-1]) and tensor.data_ptr() % 16 == 0,
+        _require(tensor.stride(-1) == 1 and all(s % 8 == 0 for s in tensor.stride()[:-1]),
                  f"{name} must be contiguous in its last dimension and 16-byte aligned in every row")
+    for name, pool in (("k_pool", k_pool), ("v_pool", v_pool)):
+        _require(all(s > 0 for s, n in zip(pool.stride(), pool.shape) if n > 1), f"{name} must not overlap itself")
     _require(slots.device == device, "slots must live on the same device as k")
-    index_source = index_pool = index_scales = None
     index_stride = index_dtype = 0
     if index_keys is not None:
-        _require(index_pools is not None, "index_keys need index_pools")
-        index_pool, index_scales = index_pools
-        index_source = index_keys
         _require(index_keys.dtype in (torch.float32, torch.bfloat16) and tuple(index_keys.shape) == (tokens, _lib.HEAD_DIM),
                  "index_keys must be float32 or bfloat16 [T, 128]")
-        _require((index_keys.stride(1) == 1) and index_keys.stride(0) % 8 == 0 and index_keys.data_ptr() % 16 == 0,
+        _require((index_keys.stride(1) == 1) and index_keys.stride(0) % 8 == 0,
                  "index_keys must be contiguous in the last dimension and 16-byte aligned in every row")
         _require(index_pool.dtype == torch.float8_e4m3fn and tuple(index_pool.shape) == (pages, page_size, _lib.HEAD_DIM)
                  and index_pool.is_contiguous(), "the index pool must be contiguous float8_e4m3fn [P, page_size, 128]")
@@ -308,14 +333,9 @@ def append_tokens(slots: Any, kv: tuple[Any, Any], pools: tuple[Any, Any], *, in
         _require(index_keys.device == device and index_pool.device == device and index_scales.device == device,
                  "index keys and pools must live on the same device as k")
         index_stride, index_dtype = index_keys.stride(0), 1 if index_keys.dtype == torch.bfloat16 else 0
-    else:
-        _require(index_pools is None, "index_pools without index_keys")
-    args = _lib.AppendArgs(
-        slots.data_ptr(), k.data_ptr(), v.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), _lib.ptr(index_source),
-        _lib.ptr(index_pool), _lib.ptr(index_scales), *k.stride()[:2], *v.stride()[:2], *k_pool.stride()[:3],
-        *v_pool.stride()[:3], index_stride, index_dtype, tokens, heads, dim, pages, page_size)
-    with torch.cuda.device(device):
-        _lib.check(_lib.load_library().itk_append_tokens(ctypes.byref(args), _lib.current_stream(torch, device)))
+    return _lib.CallTemplate(_lib.AppendArgs(
+        None, None, None, None, None, None, None, None, *k.stride()[:2], *v.stride()[:2], *k_pool.stride()[:3],
+        *v_pool.stride()[:3], index_stride, index_dtype, tokens, heads, dim, pages, page_size), device=device)
 
 
 check_serving_status = _lib.check_serving_status

@@ -172,19 +172,33 @@ __device__ __forceinline__ void umma_16bit_ts(uint32_t tmem_d, uint32_t tmem_a, 
         : "memory");
 }
 
-__device__ __forceinline__ void tmem_store_32(uint32_t tmem_address, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_load_16(uint32_t tmem_address, uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(tmem_address)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_store_16(uint32_t tmem_address, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
         ::"r"(tmem_address), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
-          "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]),
-          "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
 
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// A read of shared memory that the compiler does not replace by the registers the values were written from.
+__device__ __forceinline__ int4 load_shared_again(const int4* address) {
+    int4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(smem_u32(address)) : "memory");
+    return v;
+}
 
 // Maximum of three; a NaN among them is passed over.
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -201,6 +215,24 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     float2 d;
     asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(rd));
     return d;
+}
+
+__device__ __forceinline__ void mask_scores(uint32_t (&s)[32], int limit) {
+#pragma unroll
+    for (int k = 0; k < 32; ++k)
+        if (k >= limit) s[k] = 0xff800000u;
+}
+
+// A NaN is no maximum; its weight is NaN all the same.
+__device__ __forceinline__ float top_of(const uint32_t (&s)[32]) {
+    float most[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        most[c] = fmaxf(__uint_as_float(s[16 * c]), __uint_as_float(s[16 * c + 1]));
+#pragma unroll
+        for (int k = 2; k < 16; k += 2) most[c] = max3(most[c], __uint_as_float(s[16 * c + k]), __uint_as_float(s[16 * c + k + 1]));
+    }
+    return max3(most[0], most[1], -INFINITY);
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -529,6 +561,7 @@ struct AttnShared {
     uint64_t s_full[2][2], p_full[2][2];      // lane, step parity
     uint64_t pv_done[2], o_full[2], o_empty[2];
     int poison[kAttnPoison];
+    int4 kept[2 * kAttnSoftmaxWarps][4];      // a softmax warp's item, between its first and its last step
     uint32_t tmem_base;
     int abort;
 };
@@ -880,103 +913,150 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
     } else {
         // ============================================================ softmax
         const int x = warp >> 2;                      // lane A or B
-        const int row = (warp & 3) * 32 + lane;
-        const int token_of_row = row / p.group, head_of_row = row - token_of_row * p.group;
         const uint32_t tmem_row = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const uint32_t tmem_s = tmem_row + kAttnColumnS + x * 128;
         const uint32_t tmem_o = tmem_row + kAttnColumnO + x * 128;
         const float scale = p.scale_log2;
         const float lazy = kAttnLazy / scale;
+        // What a row of the tile means in an item, worked out where it is needed: the loop over the keys has 64 scores in
+        // registers, and what it had to spill would go to L2 (shared memory takes all of L1).
+        struct Row {
+            int token, head;       // of the item, of the key head's group
+            bool valid;
+            int visible;           // keys it sees
+        };
+        auto row_of = [&](const AttnItem& it, bool pair) {
+            Row r;
+            const int row = (warp & 3) * 32 + lane, token_of_row = row / p.group;
+            r.head = row - token_of_row * p.group;
+            r.token = token_of_row + (pair ? x * p.tile_tokens : 0);
+            r.valid = token_of_row < p.tile_tokens && r.token < it.tokens;
+            r.visible = max(0, min(it.keys, it.visible + it.slope * r.token));
+            return r;
+        };
         int steps = 0, items = 0, sequence = 0;       // steps and items with keys of this lane, items of the walk
         while (ok && walk.next(p, item, head)) {
-            const AttnLanes l = attn_lanes(item, p.tile_tokens);
             ++sequence;
-            const int token = token_of_row + (l.pair ? x * p.tile_tokens : 0);      // of the item
-            const bool valid = token_of_row < p.tile_tokens && token < item.tokens;
-            const bool active = __any_sync(0xffffffffu, valid) != 0;
-            const int visible = max(0, min(item.keys, item.visible + item.slope * token));
-            const int tiles = l.tiles[x];
+            __syncwarp();
+            if (lane == 0) {
+                int4* kept = sh.kept[warp];
+                kept[0] = make_int4(item.q_first, item.tokens, item.tile_begin, item.tiles);
+                kept[1] = make_int4(item.keys, item.visible, item.slope, item.request);
+                kept[2] = make_int4(item.k_first, item.partial, item.slot, item.slots);
+                kept[3].x = head;
+            }
+            __syncwarp();
+            const bool pair = item.tokens > p.tile_tokens;
+            const int tiles = pair ? item.tiles : (item.tiles + 1 - x) / 2, tile_begin = item.tile_begin;
+            const Row mine = row_of(item, pair);
+            const bool active = __any_sync(0xffffffffu, mine.valid) != 0;
+            const int visible = mine.visible;
             float top = -INFINITY, base = 0.0f;           // raw maximum in use, the same scaled
             float2 total = make_float2(0.0f, 0.0f);       // sum of weights
-            for (int i = 0; i < 2 * tiles; ++i, ++steps) {
-                const int h = i & 1;
-                ok = hot_wait(&sh.s_full[x][h], (steps >> 1) & 1);
-                if (!ok) break;
-                tcgen05_fence_after_sync();
-                if (active) {
-                    const int t = item.tile_begin + (l.pair ? i >> 1 : 2 * (i >> 1) + x);
-                    const int limit = visible - t * kAttnTile - h * kAttnHalf;
-                    const uint32_t tmem_step = tmem_s + h * kAttnHalf;
-                    uint32_t s[2][32];
-                    tmem_load_32(tmem_step, s[0]);
-                    tmem_load_32(tmem_step + 32, s[1]);
-                    tmem_load_wait(s[0]);
-                    tmem_load_wait(s[1]);
-                    if (__any_sync(0xffffffffu, limit < kAttnHalf)) {
-#pragma unroll
-                        for (int c = 0; c < 2; ++c)
-#pragma unroll
-                            for (int k = 0; k < 32; ++k)
-                                if (c * 32 + k >= limit) s[c][k] = 0xff800000u;
-                    }
-                    float most[4];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const uint32_t* part = &s[c >> 1][(c & 1) * 16];
-                        most[c] = fmaxf(__uint_as_float(part[0]), __uint_as_float(part[1]));
-#pragma unroll
-                        for (int k = 2; k < 16; k += 2) most[c] = max3(most[c], __uint_as_float(part[k]), __uint_as_float(part[k + 1]));
-                    }
-                    const float step_top = max3(fmaxf(most[0], most[1]), most[2], most[3]);
-                    if (i == 0) {
-                        top = fmaxf(step_top, -INFINITY);       // a NaN is no maximum; its weight is NaN all the same
-                        base = top == -INFINITY ? 0.0f : top * scale;
-                    } else {
-                        const bool moves = step_top > top + lazy;
-                        if (__any_sync(0xffffffffu, moves)) {
-                            float shrink = 1.0f;
-                            if (moves) {
-                                const float new_base = step_top * scale;
-                                shrink = top == -INFINITY ? 0.0f : exp2_fast(base - new_base);
-                                top = step_top;
-                                base = new_base;
-                                total.x *= shrink;
-                                total.y *= shrink;
-                            }
-                            // O has to hold the steps up to the one before (S of this step implies all but that one);
-                            // the next P V waits for this step's weights
-                            ok = hot_wait(&sh.pv_done[x], (steps + 1) & 1);
-                            if (!ok) break;
-                            tcgen05_fence_after_sync();
-#pragma unroll 1
-                            for (int c = 0; c < DIM; c += 32) {
-                                uint32_t o[32];
-                                tmem_load_32(tmem_o + c, o);
-                                tmem_load_wait(o);
-#pragma unroll
-                                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * shrink);
-                                tmem_store_32(tmem_o + c, o);
-                            }
-                        }
-                    }
-                    const float2 scale2 = make_float2(scale, scale), base2 = make_float2(-base, -base);
-                    float2 sums[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-                    uint32_t packed[32];
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) {
-                        const uint32_t* pair = &s[k >> 4][(k & 15) * 2];
-                        const float2 z = fma2(make_float2(__uint_as_float(pair[0]), __uint_as_float(pair[1])), scale2, base2);
-                        const float2 w = make_float2(exp2_fast(z.x), exp2_fast(z.y));
-                        sums[k & 1] = add2(sums[k & 1], w);
-                        packed[k] = Element<T>::pack(w.x, w.y);
-                    }
-                    tmem_store_32(tmem_step, packed);
-                    total = add2(total, add2(sums[0], sums[1]));
-                    tmem_store_wait();
-                }
+            const int count = 2 * tiles, first_step = steps;
+            steps += count;
+            // the first step in which a row of this warp does not see all 64 keys
+            const int whole = __reduce_min_sync(0xffffffffu, visible);
+            auto keys_before = [&](int i) { return (tile_begin + (pair ? i >> 1 : 2 * (i >> 1) + x)) * kAttnTile + (i & 1) * kAttnHalf; };
+            auto hand_over = [&](int i) {
                 tcgen05_fence_before_sync();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.p_full[x][h]);
+                if (lane == 0) mbar_arrive(&sh.p_full[x][i & 1]);
+            };
+            uint32_t s[2][32];
+            float step_top = -INFINITY;
+            // the scores of step i, which are on their way to s: masked, and their maximum
+            auto take_scores = [&](int i) {
+                tmem_load_wait(s[0]);
+                tmem_load_wait(s[1]);
+                const int before = keys_before(i);
+                if (before + kAttnHalf > whole) {
+                    mask_scores(s[0], visible - before);
+                    mask_scores(s[1], visible - before - 32);
+                }
+                step_top = fmaxf(top_of(s[0]), top_of(s[1]));
+            };
+            // the weights of 32 scores, rounded to the element type for the product; the sum takes them unrounded
+            const float2 scale2 = make_float2(scale, scale);
+            auto weigh = [&](const uint32_t (&part)[32], uint32_t address) {
+                const float2 base2 = make_float2(-base, -base);
+                float2 sums[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                uint32_t packed[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    const float2 z = fma2(make_float2(__uint_as_float(part[2 * k]), __uint_as_float(part[2 * k + 1])), scale2, base2);
+                    const float2 w = make_float2(exp2_fast(z.x), exp2_fast(z.y));
+                    sums[k & 1] = add2(sums[k & 1], w);
+                    packed[k] = Element<T>::pack(w.x, w.y);
+                }
+                tmem_store_16(address, packed);
+                total = add2(total, add2(sums[0], sums[1]));
+            };
+            if (!active) {
+                for (int i = 0; ok && i < count; ++i) {
+                    ok = wait(&sh.s_full[x][i & 1], ((first_step + i) >> 1) & 1);
+                    if (ok) hand_over(i);
+                }
+            } else if (count > 0) {
+                ok = hot_wait(&sh.s_full[x][0], (first_step >> 1) & 1);
+                if (!ok) break;
+                tcgen05_fence_after_sync();
+                tmem_load_32(tmem_s, s[0]);
+                tmem_load_32(tmem_s + 32, s[1]);
+                take_scores(0);
+                top = step_top;
+                base = top == -INFINITY ? 0.0f : top * scale;
+                for (int i = 0;; ++i) {
+                    const uint32_t here = tmem_s + (i & 1) * kAttnHalf, there = tmem_s + ((i + 1) & 1) * kAttnHalf;
+                    const bool more = i + 1 < count;
+                    uint64_t* next_full = &sh.s_full[x][(i + 1) & 1];
+                    const uint32_t next_phase = ((first_step + i + 1) >> 1) & 1;
+                    // The next step's scores, when they are there by now, are loaded into the registers that this
+                    // step's exponentials free: the loads and the hand-over run behind the second half of those.
+                    const bool early = more && __all_sync(0xffffffffu, mbar_test_wait(next_full, next_phase));
+                    if (early) tcgen05_fence_after_sync();
+                    weigh(s[0], here);
+                    if (early) tmem_load_32(there, s[0]);
+                    weigh(s[1], here + 16);
+                    if (early) tmem_load_32(there + 32, s[1]);
+                    tmem_store_wait();
+                    hand_over(i);
+                    if (!more) break;
+                    if (!early) {
+                        ok = hot_wait(next_full, next_phase);
+                        if (!ok) break;
+                        tcgen05_fence_after_sync();
+                        tmem_load_32(there, s[0]);
+                        tmem_load_32(there + 32, s[1]);
+                    }
+                    take_scores(i + 1);
+                    const bool moves = step_top > top + lazy;
+                    if (__any_sync(0xffffffffu, moves)) {
+                        float shrink = 1.0f;
+                        if (moves) {
+                            const float new_base = step_top * scale;
+                            shrink = top == -INFINITY ? 0.0f : exp2_fast(base - new_base);
+                            top = step_top;
+                            base = new_base;
+                            total.x *= shrink;
+                            total.y *= shrink;
+                        }
+                        // O has to hold the steps up to this one (the next step's scores imply all but that); the
+                        // next P V waits for the next step's weights
+                        ok = hot_wait(&sh.pv_done[x], (first_step + i) & 1);
+                        if (!ok) break;
+                        tcgen05_fence_after_sync();
+#pragma unroll 1
+                        for (int c = 0; c < DIM; c += 16) {      // in small pieces: the scores sit in 64 registers
+                            uint32_t o[16];
+                            tmem_load_16(tmem_o + c, o);
+                            tmem_load_wait16(o);
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * shrink);
+                            tmem_store_16(tmem_o + c, o);
+                        }
+                    }
+                }
             }
             if (!ok) break;
 
@@ -988,11 +1068,19 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
                 tcgen05_fence_after_sync();
             }
             const float sum = total.x + total.y;
-            const bool direct = item.partial < 0;
+            {
+                const int4* kept = sh.kept[warp];
+                const int4 a = load_shared_again(kept), b = load_shared_again(kept + 1), c = load_shared_again(kept + 2);
+                item = AttnItem{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, c.x, c.y, c.z, c.w};
+                head = load_shared_again(kept + 3).x;
+            }
+            const AttnLanes l = attn_lanes(item, p.tile_tokens);
+            const Row r = row_of(item, l.pair);
+            const bool valid = r.valid, direct = item.partial < 0;
             // lane B of a split item has rows of its own only among partial results
-            const bool writes = active && item.partial != -2 && (l.pair || x == 0 || (!direct && item.slots > 1));
-            const int head_index = head * p.group + head_of_row;
-            const long long out_token = item.q_first + token;
+            const bool writes = __any_sync(0xffffffffu, valid) != 0 && item.partial != -2 && (l.pair || x == 0 || (!direct && item.slots > 1));
+            const int head_index = head * p.group + r.head;
+            const long long out_token = item.q_first + r.token;
             const bool empty = sum == 0.0f;
             const float inverse = empty ? 0.0f : 1.0f / sum;
             long long partial_row = 0;
@@ -1000,9 +1088,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
             if (!direct) {
                 const int rows = item.tokens * p.group;
                 const int slot = item.slot + (l.pair ? 0 : x);
-                // a split entry of single-tile chunks has one slot per chunk: lane A's
+                // a split entry of a single tile has one slot: lane A's
                 if (!l.pair && x == 1 && slot >= item.slots) stores = false;
-                partial_row = item.partial + (static_cast<long long>(head) * item.slots + slot) * rows + token * p.group + head_of_row;
+                partial_row = item.partial + (static_cast<long long>(head) * item.slots + slot) * rows + r.token * p.group + r.head;
             }
             const bool poisoned = tiles > 0 && *reinterpret_cast<volatile int*>(&sh.poison[sequence % kAttnPoison]) == sequence;
             if (writes) {
@@ -1017,7 +1105,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
                     for (int i = 0; i < 32; ++i) o[i] = empty ? 0u : __float_as_uint(__uint_as_float(o[i]) * inverse);
                     if (poisoned && valid) {
                         const int from = max(l.first_visible, item.tile_begin * kAttnTile);
-                        const int to = min(visible, (item.tile_begin + item.tiles) * kAttnTile);
+                        const int to = min(r.visible, (item.tile_begin + item.tiles) * kAttnTile);
 #pragma unroll 1
                         for (int key = from; key < to; ++key) {
                             if (!l.pair && (((key / kAttnTile - item.tile_begin) & 1) != x)) continue;

@@ -48,6 +48,8 @@ constexpr int kAttnTmemColumns = 512;
 constexpr int kAttnHalf = 64;                  // keys of a step: half a tile
 constexpr int kAttnColumnS = 0, kAttnColumnO = 256;   // lane B: + 128; step i of a lane uses S columns 64 * (i % 2)
 constexpr int kAttnMaxStages = 10;
+constexpr int kAttnQueue = 4;                  // units of work the producer may be ahead of the last reader
+constexpr int kAttnReaders = 2 * kAttnSoftmaxWarps + 3;    // warps that read them: softmax, issuers, guard
 constexpr int kAttnPoison = 16;                // items the guard may be ahead of an epilogue, with room to spare
 constexpr float kAttnLazy = 8.0f;              // log2 of how far weights may exceed 1 before the maximum moves
 constexpr float kLn2 = 0.69314718055994530942f;
@@ -83,6 +85,7 @@ struct AttnCombine {
 
 struct AttnCounters {
     int items, combines, partial_rows, rows_end;
+    int next;                 // the first unit of work (item, key head) that no CTA has taken yet
 };
 
 struct AttnWorkspace {
@@ -102,8 +105,8 @@ struct AttnParams {
     AttnWorkspace w;
     int* status;
     int group, tile_tokens, sm_count, withhold_loads;
-    float scale_log2;
-    unsigned long long wait_limit_ns;
+    float scale_log2, lazy;                        // lazy: kAttnLazy in units of the scores
+    uint32_t wait_polls;
 };
 
 // ------------------------------------------------------------------ PTX
@@ -112,6 +115,17 @@ struct AttnParams {
 // reads behind grid_wait, which returns when this one has completed.
 __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Waits for the phase with the given parity, `polls` probes at most; each may be parked until the phase completes or the
+// hint runs out.  (The bound is a count, not a time: a deadline costs registers that the softmax loop does not have.)
+__device__ __forceinline__ bool attn_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint32_t polls) {
+    for (uint32_t n = 0; n < polls; ++n) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*abort_flag != 0) return false;
+    }
+    *abort_flag = 1;
+    return false;
+}
 
 // True in one thread of the warp, always the same one.  The tcgen05 instructions take their operands from uniform
 // registers: under this predicate, with operands that come out of a broadcast, they are moved there once; under a
@@ -299,6 +313,11 @@ __device__ __forceinline__ AttnRequest attn_request(const itk_attention_args& p,
 constexpr int kAttnBins = 256;
 constexpr int kAttnTries = 8;
 constexpr int kAttnMinChunk = 2;    // key tiles of a chunk at least: below that a chunk's fixed cost outweighs its keys
+// When the items do not fit one wave, the CTAs take them from the list as they get free, the longest first.  Entries of up
+// to half a CTA's fair share are not cut then (cutting 592 equal ones, four waves, into halves cost 532 -> 778 us); longer
+// ones are cut into kAttnWaves-ths of the share, which is what the last one taken may run beyond the others, but not
+// below the length at which writing and joining their partial results shows.
+constexpr int kAttnWaves = 6, kAttnWaveChunk = 16;
 static_assert(kAttnMinChunk >= 2, "a split item of one tile is its entry's only item: it has one slot and no lane B");
 // Relative cost of a key tile: a pair tile is bound by tensor and exponential work for 256 rows, a split tile by
 // the time its keys take to arrive.
@@ -366,8 +385,9 @@ __device__ __forceinline__ AttnEntry attn_entry(const AttnParams& p, const AttnR
     return r;
 }
 
-// Key chunks of an entry when a chunk may cost `cost`.
-__device__ __forceinline__ int attn_chunks(const AttnEntry& e, int cost) {
+// Key chunks of an entry when a chunk may cost `cost` and entries up to `whole` are not cut.
+__device__ __forceinline__ int attn_chunks(const AttnEntry& e, int cost, int whole) {
+    if (e.tiles <= whole / e.unit) return e.tiles > 0 ? 1 : 0;
     const int per = max(kAttnMinChunk, cost / e.unit + (cost % e.unit != 0));
     return (e.tiles + per - 1) / per;
 }
@@ -450,7 +470,7 @@ __global__ void __launch_bounds__(THREADS) itk_attention_plan_kernel(const __gri
     for (int e = tx; e < entries; e += THREADS) {
         const AttnEntry entry = entry_at(e);
 #pragma unroll
-        for (int k = 0; k < kAttnTries; ++k) mine[k] += max(1, attn_chunks(entry, share + share / kAttnTries * k));
+        for (int k = 0; k < kAttnTries; ++k) mine[k] += max(1, attn_chunks(entry, share + share / kAttnTries * k, 0));
     }
 #pragma unroll
     for (int k = 0; k < kAttnTries; ++k) {
@@ -458,11 +478,12 @@ __global__ void __launch_bounds__(THREADS) itk_attention_plan_kernel(const __gri
         if (lane == 0 && sum != 0) atomicAdd(&counts[k], sum);
     }
     __syncthreads();
-    int chunk = share;
+    int chunk = min(share, max(share / kAttnWaves, kAttnWaveChunk * kAttnPairCost)), whole = share / 2;
     bool one_wave = false;
     for (int k = kAttnTries - 1; k >= 0; --k)
         if (static_cast<long long>(counts[k]) * kv_heads <= p.sm_count) {
             chunk = share + share / kAttnTries * k;
+            whole = 0;
             one_wave = true;
         }
 
@@ -476,7 +497,7 @@ __global__ void __launch_bounds__(THREADS) itk_attention_plan_kernel(const __gri
         int most = 0;
         for (int e = tx; e < entries; e += THREADS) {
             const AttnEntry entry = entry_at(e);
-            const int chunks = max(1, attn_chunks(entry, chunk));
+            const int chunks = max(1, attn_chunks(entry, chunk, whole));
             most = max(most, (entry.tiles + chunks - 1) / chunks * entry.unit);
         }
         most = __reduce_max_sync(0xffffffffu, most);
@@ -485,7 +506,7 @@ __global__ void __launch_bounds__(THREADS) itk_attention_plan_kernel(const __gri
         top = max(longest, 1);
         for (int e = tx; e < entries; e += THREADS) {
             const AttnEntry entry = entry_at(e);
-            const int chunks = max(1, attn_chunks(entry, chunk));
+            const int chunks = max(1, attn_chunks(entry, chunk, whole));
             atomicAdd(&bins[bin_of(entry, chunks)], chunks);
         }
         __syncthreads();
@@ -514,7 +535,7 @@ __global__ void __launch_bounds__(THREADS) itk_attention_plan_kernel(const __gri
     }
     for (int e = tx; e < entries; e += THREADS) {
         AttnEntry entry = entry_at(e);
-        const int chunks = attn_chunks(entry, chunk);               // 0: no key at all
+        const int chunks = attn_chunks(entry, chunk, whole);               // 0: no key at all
         const int longest_chunk = chunks > 0 ? (entry.tiles + chunks - 1) / chunks : 0;
         const int lanes = !entry.pair && longest_chunk > 1 ? 2 : 1;
         const int rows = entry.item.tokens * p.group;
@@ -550,7 +571,7 @@ __global__ void __launch_bounds__(THREADS) itk_attention_plan_kernel(const __gri
         }
     }
     __syncthreads();
-    if (tx == 0) *p.w.counters = AttnCounters{min(item_count, p.w.max_items), min(combine_count, p.w.max_combines), partial_rows, rows_end};
+    if (tx == 0) *p.w.counters = AttnCounters{min(item_count, p.w.max_items), min(combine_count, p.w.max_combines), partial_rows, rows_end, p.sm_count};
 }
 
 // ------------------------------------------------------------------ attention
@@ -560,8 +581,9 @@ struct AttnShared {
     uint64_t kv_full[kAttnMaxStages], kv_empty[kAttnMaxStages], guard_full[kAttnMaxStages];
     uint64_t s_full[2][2], p_full[2][2];      // lane, step parity
     uint64_t pv_done[2], o_full[2], o_empty[2];
+    uint64_t item_full[kAttnQueue], item_empty[kAttnQueue];
     int poison[kAttnPoison];
-    int4 kept[2 * kAttnSoftmaxWarps][4];      // a softmax warp's item, between its first and its last step
+    int4 items[kAttnQueue][4];                // the CTA's next units of work: the item, then (key head, 1) or (-, 0) at the end
     uint32_t tmem_base;
     int abort;
 };
@@ -583,29 +605,11 @@ __device__ __forceinline__ AttnLanes attn_lanes(const AttnItem& item, int tile_t
     return r;
 }
 
-// Walks this CTA's share of the list: item k of every wave, the waves in alternating direction so that the CTA with
-// the longest item of one wave has the shortest of the next.
-struct AttnWalk {
-    int wave = 0, total, heads;
-    __device__ __forceinline__ AttnWalk(const AttnParams& p) : total(p.w.counters->items * p.a.kv_heads), heads(p.a.kv_heads) {}
-    __device__ __forceinline__ bool next(const AttnParams& p, AttnItem& item, int& head) {
-        for (;;) {
-            const int grid = static_cast<int>(gridDim.x), me = static_cast<int>(blockIdx.x);
-            const long long at = static_cast<long long>(wave) * grid + ((wave & 1) ? grid - 1 - me : me);
-            const int index = static_cast<int>(at / heads);
-            // read before it is known whether there is such an item: the two loads overlap
-            const int4* source = reinterpret_cast<const int4*>(p.w.items + min(index, p.w.max_items - 1));
-            const int4 a = source[0], b = source[1], c = source[2];
-            if (static_cast<long long>(wave) * grid >= total) return false;
-            ++wave;
-            if (at >= total) continue;
-            head = static_cast<int>(at - static_cast<long long>(index) * heads);
-            item = AttnItem{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, c.x, c.y, c.z, c.w};
-            if (item.tokens > 0) return true;
-        }
-    }
-};
 static_assert(sizeof(AttnItem) == 48, "items are read as three 16-byte vectors");
+
+__device__ __forceinline__ AttnItem attn_item(const int4& a, const int4& b, const int4& c) {
+    return AttnItem{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, c.x, c.y, c.z, c.w};
+}
 
 // Where key tile t of a segment lies.
 __device__ __forceinline__ int attn_page(const AttnParams& p, const AttnItem& item, int t) {
@@ -671,6 +675,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
             mbar_init(&sh.kv_empty[i], 2);
             mbar_init(&sh.guard_full[i], 1);
         }
+        for (int i = 0; i < kAttnQueue; ++i) {
+            mbar_init(&sh.item_full[i], 1);
+            mbar_init(&sh.item_empty[i], kAttnReaders);
+        }
         for (int i = 0; i < kAttnPoison; ++i) sh.poison[i] = 0;
         sh.abort = 0;
         fence_mbar_init();
@@ -690,24 +698,63 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
     volatile int* abort_flag = &sh.abort;
     // a wait of the whole warp: its lanes leave together
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-        return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.wait_limit_ns)) != 0;
-    };
-    auto hot_wait = [&](uint64_t* bar, uint32_t parity) {
-        return __all_sync(0xffffffffu, mbar_wait<kHotWait>(bar, parity, abort_flag, p.wait_limit_ns)) != 0;
+        return __all_sync(0xffffffffu, attn_wait(bar, parity, abort_flag, p.wait_polls)) != 0;
     };
     bool ok = true;
     AttnItem item;
     int head;
-    AttnWalk walk(p);
+    // The units of work, for all warps but the producer that hands them out: take() reads the next one, done() gives its
+    // place in the queue back (a softmax warp reads it once more before its epilogue).
+    int units = 0;
+    auto read_unit = [&](int unit) {
+        const int4* source = sh.items[unit % kAttnQueue];
+        item = attn_item(load_shared_again(source), load_shared_again(source + 1), load_shared_again(source + 2));
+        const int4 tail = load_shared_again(source + 3);
+        head = tail.x;
+        return tail.y != 0;
+    };
+    auto done = [&]() {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.item_empty[(units - 1) % kAttnQueue]);
+    };
+    auto take = [&]() {
+        ok = wait(&sh.item_full[units % kAttnQueue], (units / kAttnQueue) & 1);
+        return ok && read_unit(units++);
+    };
 
     if (warp == kAttnLoadWarp) {
         // ============================================================ TMA producer
         int ring = 0;                 // tiles loaded so far
         int q_uses[2] = {0, 0};
         const int q_bytes = Shape::kChunks * p.tile_tokens * p.group * 128;
-        while (ok && p.withhold_loads == 0 && walk.next(p, item, head)) {
+        const int kv_heads = p.a.kv_heads;
+        // The first unit of a CTA is the one with its number, the others are taken when their turn comes.
+        int unit = static_cast<int>(blockIdx.x), next_unit = 0;
+        for (; ok; unit = __shfl_sync(0xffffffffu, next_unit, 0)) {
+            const int index = min(unit / kv_heads, p.w.max_items - 1);
+            // read before it is known whether there is such an item: the loads overlap
+            const int4* source = reinterpret_cast<const int4*>(p.w.items + index);
+            const int4 a = source[0], b = source[1], c = source[2];
+            const bool there = unit < p.w.counters->items * kv_heads;
+            item = attn_item(a, b, c);
+            head = unit - index * kv_heads;
+            if (there && lane == 0) next_unit = atomicAdd(&p.w.counters->next, 1);
+            if (there && item.tokens == 0) continue;              // nothing to do
+            ok = wait(&sh.item_empty[units % kAttnQueue], ((units / kAttnQueue) & 1) ^ 1);
+            if (!ok) break;
+            if (lane == 0) {
+                int4* target = sh.items[units % kAttnQueue];
+                target[0] = a;
+                target[1] = b;
+                target[2] = c;
+                target[3] = make_int4(head, there ? 1 : 0, 0, 0);
+                mbar_arrive(&sh.item_full[units % kAttnQueue]);
+            }
+            __syncwarp();
+            ++units;
+            if (!there) break;
             const AttnLanes l = attn_lanes(item, p.tile_tokens);
-            if (item.tiles == 0) continue;
+            if (item.tiles == 0 || p.withhold_loads != 0) continue;
             for (int tile = 0; ok && tile < (l.pair ? 2 : 1); ++tile) {
                 ok = wait(&sh.q_empty[tile], (q_uses[tile] & 1) ^ 1);
                 ++q_uses[tile];
@@ -764,14 +811,15 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
         auto release = [&](uint64_t* bar) {
             if (lane == 0) mbar_arrive(bar);
         };
-        while (ok && walk.next(p, item, head)) {
+        while (ok && take()) {
+            done();
             const AttnLanes l = attn_lanes(item, p.tile_tokens);
             const bool pair = uniform(l.pair) != 0;
             const int tiles = uniform(item.tiles), mine = uniform(l.tiles[x]);
             if (tiles == 0) continue;
             const int q_tile = pair ? x : 0;
             for (int tile = 0; ok && tile < (pair ? 2 : 1); ++tile) {
-                ok = hot_wait(&sh.q_full[tile], q_uses[tile] & 1);
+                ok = wait(&sh.q_full[tile], q_uses[tile] & 1);
                 ++q_uses[tile];
                 if (ok && (tile != q_tile || mine == 0)) release(&sh.q_empty[tile]);
             }
@@ -781,7 +829,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
             // the next tile of the ring, in shared memory
             auto arrive_tile = [&](int& stage) {
                 stage = ring % kStages;
-                ok = ok && hot_wait(&sh.kv_full[stage], (ring / kStages) & 1);
+                ok = ok && wait(&sh.kv_full[stage], (ring / kStages) & 1);
                 ++ring;
                 return ok;
             };
@@ -831,10 +879,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
                 int v_stage;
                 if (!arrive_tile(v_stage)) break;
                 const uint64_t v_desc = umma_desc_sw128_mnmajor(kv_base + v_stage * Shape::kTileBytes, kAttnTile * 128);
-                if (j == 0) ok = hot_wait(&sh.o_empty[x], (items & 1) ^ 1);
+                if (j == 0) ok = wait(&sh.o_empty[x], (items & 1) ^ 1);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    if (ok) ok = hot_wait(&sh.p_full[x][h], p_phase);
+                    if (ok) ok = wait(&sh.p_full[x][h], p_phase);
                     if (!ok) continue;
                     tcgen05_fence_after_sync();
                     if (elect_one()) {
@@ -857,11 +905,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
         }
     } else if (warp == kAttnGuardWarp) {
         // ============================================================ guard
-        int ring = 0, sequence = 0;
+        int ring = 0;
         uint32_t phases = 0;          // of guard_full: a stage's flips with every tile the guard takes from it
-        while (ok && p.withhold_loads == 0 && walk.next(p, item, head)) {
+        while (ok && p.withhold_loads == 0 && take()) {
+            done();
             const AttnLanes l = attn_lanes(item, p.tile_tokens);
-            ++sequence;
             if (item.tiles == 0) continue;
             const int first = max(0, l.first_visible / kAttnTile - item.tile_begin);
             for (int t = first; ok && t < item.tiles; ++t) {
@@ -903,7 +951,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 found = __any_sync(0xffffffffu, found) != 0;
                 if (lane == 0) {
-                    if (found) *reinterpret_cast<volatile int*>(&sh.poison[sequence % kAttnPoison]) = sequence;
+                    if (found) *reinterpret_cast<volatile int*>(&sh.poison[units % kAttnPoison]) = units;
                     mbar_arrive(&sh.kv_full[stage]);
                 }
                 __syncwarp();
@@ -915,9 +963,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
         const int x = warp >> 2;                      // lane A or B
         const uint32_t tmem_row = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const uint32_t tmem_s = tmem_row + kAttnColumnS + x * 128;
-        const uint32_t tmem_o = tmem_row + kAttnColumnO + x * 128;
+        constexpr int kToO = kAttnColumnO - kAttnColumnS;
         const float scale = p.scale_log2;
-        const float lazy = kAttnLazy / scale;
         // What a row of the tile means in an item, worked out where it is needed: the loop over the keys has 64 scores in
         // registers, and what it had to spill would go to L2 (shared memory takes all of L1).
         struct Row {
@@ -934,18 +981,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
             r.visible = max(0, min(it.keys, it.visible + it.slope * r.token));
             return r;
         };
-        int steps = 0, items = 0, sequence = 0;       // steps and items with keys of this lane, items of the walk
-        while (ok && walk.next(p, item, head)) {
-            ++sequence;
-            __syncwarp();
-            if (lane == 0) {
-                int4* kept = sh.kept[warp];
-                kept[0] = make_int4(item.q_first, item.tokens, item.tile_begin, item.tiles);
-                kept[1] = make_int4(item.keys, item.visible, item.slope, item.request);
-                kept[2] = make_int4(item.k_first, item.partial, item.slot, item.slots);
-                kept[3].x = head;
-            }
-            __syncwarp();
+        int steps = 0, items = 0;       // steps and items with keys of this lane
+        while (ok && take()) {
             const bool pair = item.tokens > p.tile_tokens;
             const int tiles = pair ? item.tiles : (item.tiles + 1 - x) / 2, tile_begin = item.tile_begin;
             const Row mine = row_of(item, pair);
@@ -953,26 +990,26 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
             const int visible = mine.visible;
             float top = -INFINITY, base = 0.0f;           // raw maximum in use, the same scaled
             float2 total = make_float2(0.0f, 0.0f);       // sum of weights
-            const int count = 2 * tiles, first_step = steps;
-            steps += count;
-            // the first step in which a row of this warp does not see all 64 keys
-            const int whole = __reduce_min_sync(0xffffffffu, visible);
-            auto keys_before = [&](int i) { return (tile_begin + (pair ? i >> 1 : 2 * (i >> 1) + x)) * kAttnTile + (i & 1) * kAttnHalf; };
-            auto hand_over = [&](int i) {
+            // step `at` of the lane's count works in buffer at % 2; an item has an even number of them
+            int at = steps;
+            steps += 2 * tiles;
+            // keys from the step's first one on that the row sees, and that all rows of this warp see
+            int left = visible - (tile_begin + (pair ? 0 : x)) * kAttnTile;
+            int left_all = __reduce_min_sync(0xffffffffu, left);
+            auto hand_over = [&]() {
                 tcgen05_fence_before_sync();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.p_full[x][i & 1]);
+                if (lane == 0) mbar_arrive(&sh.p_full[x][at & 1]);
             };
             uint32_t s[2][32];
             float step_top = -INFINITY;
-            // the scores of step i, which are on their way to s: masked, and their maximum
-            auto take_scores = [&](int i) {
+            // the scores of a step, which are on their way to s: masked, and their maximum
+            auto take_scores = [&]() {
                 tmem_load_wait(s[0]);
                 tmem_load_wait(s[1]);
-                const int before = keys_before(i);
-                if (before + kAttnHalf > whole) {
-                    mask_scores(s[0], visible - before);
-                    mask_scores(s[1], visible - before - 32);
+                if (left_all < kAttnHalf) {
+                    mask_scores(s[0], left);
+                    mask_scores(s[1], left - 32);
                 }
                 step_top = fmaxf(top_of(s[0]), top_of(s[1]));
             };
@@ -980,37 +1017,37 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
             const float2 scale2 = make_float2(scale, scale);
             auto weigh = [&](const uint32_t (&part)[32], uint32_t address) {
                 const float2 base2 = make_float2(-base, -base);
-                float2 sums[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                float2 sum = make_float2(0.0f, 0.0f);
                 uint32_t packed[16];
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
                     const float2 z = fma2(make_float2(__uint_as_float(part[2 * k]), __uint_as_float(part[2 * k + 1])), scale2, base2);
                     const float2 w = make_float2(exp2_fast(z.x), exp2_fast(z.y));
-                    sums[k & 1] = add2(sums[k & 1], w);
+                    sum = add2(sum, w);
                     packed[k] = Element<T>::pack(w.x, w.y);
                 }
                 tmem_store_16(address, packed);
-                total = add2(total, add2(sums[0], sums[1]));
+                total = add2(total, sum);
             };
             if (!active) {
-                for (int i = 0; ok && i < count; ++i) {
-                    ok = wait(&sh.s_full[x][i & 1], ((first_step + i) >> 1) & 1);
-                    if (ok) hand_over(i);
+                for (; ok && at < steps; ++at) {
+                    ok = wait(&sh.s_full[x][at & 1], (at >> 1) & 1);
+                    if (ok) hand_over();
                 }
-            } else if (count > 0) {
-                ok = hot_wait(&sh.s_full[x][0], (first_step >> 1) & 1);
+            } else if (at < steps) {
+                ok = wait(&sh.s_full[x][0], (at >> 1) & 1);
                 if (!ok) break;
                 tcgen05_fence_after_sync();
                 tmem_load_32(tmem_s, s[0]);
                 tmem_load_32(tmem_s + 32, s[1]);
-                take_scores(0);
+                take_scores();
                 top = step_top;
                 base = top == -INFINITY ? 0.0f : top * scale;
-                for (int i = 0;; ++i) {
-                    const uint32_t here = tmem_s + (i & 1) * kAttnHalf, there = tmem_s + ((i + 1) & 1) * kAttnHalf;
-                    const bool more = i + 1 < count;
-                    uint64_t* next_full = &sh.s_full[x][(i + 1) & 1];
-                    const uint32_t next_phase = ((first_step + i + 1) >> 1) & 1;
+                for (;; ++at) {
+                    const uint32_t here = tmem_s + (at & 1) * kAttnHalf, there = tmem_s + ((at + 1) & 1) * kAttnHalf;
+                    const bool more = at + 1 < steps;
+                    uint64_t* next_full = &sh.s_full[x][(at + 1) & 1];
+                    const uint32_t next_phase = ((at + 1) >> 1) & 1;
                     // The next step's scores, when they are there by now, are loaded into the registers that this
                     // step's exponentials free: the loads and the hand-over run behind the second half of those.
                     const bool early = more && __all_sync(0xffffffffu, mbar_test_wait(next_full, next_phase));
@@ -1020,17 +1057,20 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
                     weigh(s[1], here + 16);
                     if (early) tmem_load_32(there + 32, s[1]);
                     tmem_store_wait();
-                    hand_over(i);
+                    hand_over();
                     if (!more) break;
                     if (!early) {
-                        ok = hot_wait(next_full, next_phase);
+                        ok = wait(next_full, next_phase);
                         if (!ok) break;
                         tcgen05_fence_after_sync();
                         tmem_load_32(there, s[0]);
                         tmem_load_32(there + 32, s[1]);
                     }
-                    take_scores(i + 1);
-                    const bool moves = step_top > top + lazy;
+                    const int on = !pair && (at & 1) != 0 ? kAttnHalf + kAttnTile : kAttnHalf;     // the other lane's tile is passed over
+                    left -= on;
+                    left_all -= on;
+                    take_scores();
+                    const bool moves = step_top > top + p.lazy;
                     if (__any_sync(0xffffffffu, moves)) {
                         float shrink = 1.0f;
                         if (moves) {
@@ -1043,17 +1083,17 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
                         }
                         // O has to hold the steps up to this one (the next step's scores imply all but that); the
                         // next P V waits for the next step's weights
-                        ok = hot_wait(&sh.pv_done[x], (first_step + i) & 1);
+                        ok = wait(&sh.pv_done[x], at & 1);
                         if (!ok) break;
                         tcgen05_fence_after_sync();
 #pragma unroll 1
                         for (int c = 0; c < DIM; c += 16) {      // in small pieces: the scores sit in 64 registers
                             uint32_t o[16];
-                            tmem_load_16(tmem_o + c, o);
+                            tmem_load_16(tmem_s + kToO + c, o);
                             tmem_load_wait16(o);
 #pragma unroll
                             for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * shrink);
-                            tmem_store_16(tmem_o + c, o);
+                            tmem_store_16(tmem_s + kToO + c, o);
                         }
                     }
                 }
@@ -1062,18 +1102,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
 
             // ------------------------------------------------------ epilogue
             if (tiles > 0) {
-                ok = hot_wait(&sh.o_full[x], items & 1);
+                ok = wait(&sh.o_full[x], items & 1);
                 ++items;
                 if (!ok) break;
                 tcgen05_fence_after_sync();
             }
             const float sum = total.x + total.y;
-            {
-                const int4* kept = sh.kept[warp];
-                const int4 a = load_shared_again(kept), b = load_shared_again(kept + 1), c = load_shared_again(kept + 2);
-                item = AttnItem{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, c.x, c.y, c.z, c.w};
-                head = load_shared_again(kept + 3).x;
-            }
+            read_unit(units - 1);
+            done();
             const AttnLanes l = attn_lanes(item, p.tile_tokens);
             const Row r = row_of(item, l.pair);
             const bool valid = r.valid, direct = item.partial < 0;
@@ -1092,13 +1128,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
                 if (!l.pair && x == 1 && slot >= item.slots) stores = false;
                 partial_row = item.partial + (static_cast<long long>(head) * item.slots + slot) * rows + r.token * p.group + r.head;
             }
-            const bool poisoned = tiles > 0 && *reinterpret_cast<volatile int*>(&sh.poison[sequence % kAttnPoison]) == sequence;
+            const bool poisoned = tiles > 0 && *reinterpret_cast<volatile int*>(&sh.poison[units % kAttnPoison]) == units;
             if (writes) {
 #pragma unroll 1
                 for (int c = 0; c < DIM / 32; ++c) {
                     uint32_t o[32];
                     if (tiles > 0) {
-                        tmem_load_32(tmem_o + c * 32, o);
+                        tmem_load_32(tmem_s + kToO + c * 32, o);
                         tmem_load_wait(o);
                     }
 #pragma unroll

@@ -96,18 +96,21 @@ int check_attention(const itk_attention_args& a) {
     return ITK_OK;
 }
 
-constexpr int kAttnMaxSms = 256;     // the workspace is sized for any device the library runs on
+constexpr int kAttnMaxSms = 160;     // the workspace is sized for any device the library runs on
 
 // Workspace of a call: what the plan kernel can write at most.  With T tokens, B requests and 2 TT tokens per entry
-// there are at most T / (2 TT) + B own entries; the prefix has T / (2 TT) + 1.  Chunking adds at most one item per SM
-// (a chunk costs at least a fair share of the work).  Partial rows: a split entry (at most one per request, at most
-// 128 rows per key head) has two lanes; chunks add at most two row tiles per SM and as many again for the rounding of
-// entries that are cut; with a prefix every own row and every prefix row has one more, two in split entries.
+// there are at most T / (2 TT) + B own entries; the prefix has T / (2 TT) + 1.  A chunk costs at least a kAttnWaves-th of an
+// SM's share of the work, so that chunking adds at most kAttnWaves items per SM over all key heads.  Partial rows: a split
+// entry (at most one per request, at most 128 rows per key head) has two lanes; an added chunk has at most two row tiles, and
+// no row has more of them than there are chunks for one key head; with a prefix every own row and every prefix row has one
+// more, two in split entries.
 int attention_workspace(const itk_attention_args& a, AttnWorkspace* w, size_t* bytes) {
     const long long tile_tokens = kAttnTile / (a.heads / a.kv_heads), span = 2 * tile_tokens;
     const long long rows = static_cast<long long>(a.tokens) * a.heads;
     const long long own = a.tokens / span + a.requests, prefix = a.prefix_keys > 0 ? a.tokens / span + 1 : 0;
-    long long partial = 2 * std::min(rows, static_cast<long long>(a.requests) * kAttnTile * a.kv_heads) + 2ll * kAttnMaxSms * 2 * kAttnTile;
+    const long long added = static_cast<long long>(kAttnMaxSms) * kAttnWaves;
+    long long partial = 2 * std::min(rows, static_cast<long long>(a.requests) * kAttnTile * a.kv_heads) +
+                        2 * std::min(2 * added * kAttnTile, rows * (added / a.kv_heads + 1));
     if (prefix > 0) partial += 3 * rows;
     ITK_REQUIRE(partial < (1ll << 31) - 1 && own + prefix < (1ll << 28), "the batch is too large for one call");
     size_t at = 0;
@@ -120,7 +123,7 @@ int attention_workspace(const itk_attention_args& a, AttnWorkspace* w, size_t* b
     ITK_REQUIRE(combines * a.kv_heads < (1ll << 31), "the batch is too large for one call");
     w->max_entries = static_cast<int>(own);
     w->max_combines = static_cast<int>(combines);
-    w->max_items = static_cast<int>(own + prefix + kAttnMaxSms);
+    w->max_items = static_cast<int>(own + prefix + added);
     w->max_partial_rows = static_cast<int>(partial);
     w->counters = reinterpret_cast<AttnCounters*>(take(sizeof(AttnCounters)));
     w->entry_first = reinterpret_cast<int*>(take((static_cast<size_t>(a.requests) + 1) * sizeof(int)));
@@ -303,7 +306,8 @@ int itk_attention(const itk_attention_args* args, itk_stream_t stream) {
     params.sm_count = std::min(device.sm_count, kAttnMaxSms);
     params.withhold_loads = a.withhold_loads;
     params.scale_log2 = a.scale * kLog2e;
-    params.wait_limit_ns = a.wait_limit_ns != 0 ? a.wait_limit_ns : kWaitLimitNs;
+    params.lazy = kAttnLazy / params.scale_log2;
+    params.wait_polls = static_cast<uint32_t>(std::min(std::max((a.wait_limit_ns != 0 ? a.wait_limit_ns : kWaitLimitNs) / 1000, 1ull), 1ull << 31));
     {
         const cuuint64_t dims[3] = {static_cast<cuuint64_t>(a.dim), static_cast<cuuint64_t>(a.heads), static_cast<cuuint64_t>(a.tokens)};
         const cuuint64_t strides[2] = {map_stride(a.q_head_stride, a.heads), map_stride(a.q_token_stride, a.tokens)};

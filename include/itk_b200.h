@@ -430,7 +430,7 @@ typedef struct itk_attention_args {
     void* workspace;
     size_t workspace_bytes;
     long long q_token_stride, q_head_stride, out_token_stride, out_head_stride;
-    unsigned long long wait_limit_ns;   /* 0 = default (2 s) */
+    unsigned long long wait_limit_ns;   /* 0 = default (2 s); counted in probes, a thousand nanoseconds each at least nominally */
     itk_kv_segment own;
     itk_kv_segment prefix;     /* k = null: no prefix */
     float scale;

@@ -105,6 +105,8 @@ struct AttnParams {
     AttnWorkspace w;
     int* status;
     int group, tile_tokens, sm_count, withhold_loads;
+    int out_sectors;                               // rows of the output start on 32-byte boundaries
+    float inverse_sms;                             // 1 / sm_count
     float scale_log2, lazy;                        // lazy: kAttnLazy in units of the scores
     uint32_t wait_polls;
 };
@@ -219,6 +221,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
+}
+
+// 32 bytes, a whole sector: rows lie far apart, so half-sector stores would take twice the time.
+__device__ __forceinline__ void store_sector(void* address, const uint32_t* r) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(address), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
 }
 
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
@@ -387,9 +396,9 @@ __device__ __forceinline__ AttnEntry attn_entry(const AttnParams& p, const AttnR
 
 // Key chunks of an entry when a chunk may cost `cost` and entries up to `whole` are not cut.
 __device__ __forceinline__ int attn_chunks(const AttnEntry& e, int cost, int whole) {
-    if (e.tiles <= whole / e.unit) return e.tiles > 0 ? 1 : 0;
-    const int per = max(kAttnMinChunk, cost / e.unit + (cost % e.unit != 0));
-    return (e.tiles + per - 1) / per;
+    if (whole > 0 && static_cast<long long>(e.tiles) * e.unit <= whole) return e.tiles > 0 ? 1 : 0;
+    const unsigned per = max(kAttnMinChunk, e.pair ? (cost + kAttnPairCost - 1) / kAttnPairCost : (cost + kAttnSplitCost - 1) / kAttnSplitCost);
+    return static_cast<int>((static_cast<unsigned>(e.tiles) + per - 1) / per);
 }
 
 // Most of a small call's time before its first key is read goes by in here: one pass over the lengths, entries kept in
@@ -463,9 +472,8 @@ __global__ void __launch_bounds__(THREADS) itk_attention_plan_kernel(const __gri
     for (int step = 16; step > 0; step >>= 1) cost += __shfl_xor_sync(0xffffffffu, cost, step);
     if (lane == 0 && cost != 0) atomicAdd(&total_cost, cost);
     __syncthreads();
-    // (a chunk is at most 2^30 long: longer than any entry, 2^24 tiles of cost 4, can be)
-    const unsigned long long fair = (total_cost * kv_heads + p.sm_count - 1) / p.sm_count;
-    const int share = static_cast<int>(min(max(fair, 1ull), 1ull << 29));
+    // in fp32: it only has to be near.  (A chunk costs at most 2^29, more than any entry, 2^24 tiles of cost 4, does.)
+    const int share = static_cast<int>(fminf(ceilf(static_cast<float>(total_cost) * kv_heads * p.inverse_sms) + 1.0f, 536870912.0f));
     int mine[kAttnTries] = {};
     for (int e = tx; e < entries; e += THREADS) {
         const AttnEntry entry = entry_at(e);
@@ -562,12 +570,13 @@ __global__ void __launch_bounds__(THREADS) itk_attention_plan_kernel(const __gri
         if (chunks == 0 && joined) entry.item.tokens = 0;           // the prefix alone: a place in the list, but nothing to do
         const int count = max(1, chunks);
         const int place = atomicAdd(one_wave ? &item_count : &bins[bin_of(entry, count)], count);
+        const int even = entry.tiles / count, odd = entry.tiles - even * count;        // the first `odd` chunks are one tile longer
+        entry.item.tile_begin = 0;
         for (int c = 0; c < count; ++c) {
-            const long long lo = static_cast<long long>(entry.tiles) * c / count, hi = static_cast<long long>(entry.tiles) * (c + 1) / count;
-            entry.item.tile_begin = static_cast<int>(lo);
-            entry.item.tiles = static_cast<int>(hi - lo);
+            entry.item.tiles = even + (c < odd ? 1 : 0);
             entry.item.slot = c * lanes;
             if (place + c < p.w.max_items) p.w.items[place + c] = entry.item;
+            entry.item.tile_begin += entry.item.tiles;
         }
     }
     __syncthreads();
@@ -1159,17 +1168,19 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
                     if (stores && direct) {
                         T* out = static_cast<T*>(p.a.out) + out_token * p.a.out_token_stride + head_index * p.a.out_head_stride + c * 32;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            uint32_t w[4];
+                        for (int i = 0; i < 16; ++i) o[i] = Element<T>::pack(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
+                        if (p.out_sectors != 0) {
+                            store_sector(out, &o[0]);
+                            store_sector(out + 16, &o[8]);
+                        } else {
 #pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                w[k] = Element<T>::pack(__uint_as_float(o[8 * i + 2 * k]), __uint_as_float(o[8 * i + 2 * k + 1]));
-                            reinterpret_cast<uint4*>(out)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                            for (int i = 0; i < 4; ++i)
+                                reinterpret_cast<uint4*>(out)[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                         }
                     } else if (stores && !empty) {
-                        uint4* out = reinterpret_cast<uint4*>(p.w.partial_out + partial_row * DIM + c * 32);
+                        float* out = p.w.partial_out + partial_row * DIM + c * 32;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) out[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                        for (int i = 0; i < 4; ++i) store_sector(out + 8 * i, &o[8 * i]);
                     }
                 }
                 if (stores) {
@@ -1220,75 +1231,74 @@ constexpr int kJoinThreads = 256;
 template <typename T, int DIM>
 __global__ void __launch_bounds__(kJoinThreads) itk_attention_join_kernel(const __grid_constant__ AttnParams p) {
     constexpr int kOwn = DIM / 32;
-    constexpr int kFlight = 8;           // partial rows on their way at a time: the loop is bound by their latency
-    grid_wait();
-    const AttnCounters counters = *p.w.counters;
+    constexpr int kFlight = 16;          // partial rows on their way at a time
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int span = 2 * p.tile_tokens;
     const int heads = p.a.kv_heads;
-    for (int work = blockIdx.x; work < counters.combines * heads; work += gridDim.x) {
-        const AttnCombine entry = p.w.combines[work / heads];
-        const int head = work % heads;
+    grid_wait();
+    AttnCounters counters;
+    for (int work = blockIdx.x;; work += gridDim.x) {
+        // (the record is read before it is known whether there is one: what this kernel takes is the chain of loads that
+        // depend on one another)
+        const int index = work / heads, head = work - index * heads;
+        const int4* source = reinterpret_cast<const int4*>(p.w.combines + min(index, p.w.max_combines - 1));
+        const int4 record = source[0];
+        const int row_first = source[1].x;
+        if (work == static_cast<int>(blockIdx.x)) counters = *p.w.counters;
+        if (work >= counters.combines * heads) break;
+        const AttnCombine entry{record.x, record.y, record.z, record.w, row_first, {}};
         const int rows = entry.tokens * p.group, row_end = min(rows, entry.row_first + kAttnCombineRows);
         for (int r = entry.row_first + warp; r < row_end; r += kJoinThreads / 32) {
             const int token = entry.q_first + r / p.group;
             const int head_index = head * p.group + r % p.group;
-            // two runs of partial rows: first row, distance, count
-            long long first[2] = {entry.partial + static_cast<long long>(head) * entry.slots * rows + r, 0};
-            int step[2] = {rows, 0}, count[2] = {entry.slots, 0};
+            // the row's own partial results, then the prefix's: two runs of rows
+            int count = entry.slots, prefix_count = 0, prefix_rows = 0;
+            const long long first = entry.partial + static_cast<long long>(head) * entry.slots * rows + r;
+            long long prefix_first = 0;
             if (p.a.prefix_keys > 0) {
                 const int e = token / span;
                 const int2 slots = p.w.prefix_slots[e];
-                const int prefix_rows = min(span, counters.rows_end - e * span) * p.group;
-                first[1] = slots.x + static_cast<long long>(head) * slots.y * prefix_rows + (token - e * span) * p.group + r % p.group;
-                step[1] = prefix_rows;
-                count[1] = slots.y;
+                prefix_rows = min(span, counters.rows_end - e * span) * p.group;
+                prefix_first = slots.x + static_cast<long long>(head) * slots.y * prefix_rows + (token - e * span) * p.group + r % p.group;
+                prefix_count = slots.y;
             }
-            float top = -INFINITY;
+            count += prefix_count;
+            auto row_of = [&](int c) {
+                return c < entry.slots ? first + static_cast<long long>(c) * rows
+                                       : prefix_first + static_cast<long long>(c - entry.slots) * prefix_rows;
+            };
+            float top = -INFINITY, total = 0.0f, sums[kOwn] = {};
             bool broken = false;
-            for (int run = 0; run < 2; ++run)
-                for (int c = lane; c < count[run]; c += 32) {
-                    const float lse = p.w.partial_lse[first[run] + static_cast<long long>(c) * step[run]];
-                    broken |= lse != lse;
-                    top = fmaxf(top, lse);
-                }
+            for (int base = 0; base < count; base += kFlight) {
+                const int here = min(kFlight, count - base);
+                const float lse = lane < here ? p.w.partial_lse[row_of(base + lane)] : -INFINITY;
+                float held[kFlight][kOwn];
 #pragma unroll
-            for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            broken = __any_sync(0xffffffffu, broken) != 0;
-            float total = 0.0f, sums[kOwn] = {};
-            if (top > -INFINITY) {
-                for (int run = 0; run < 2; ++run)
-                    for (int base = 0; base < count[run]; base += 32) {
-                        float weight = 0.0f;
-                        if (base + lane < count[run])
-                            weight = exp2_fast(p.w.partial_lse[first[run] + static_cast<long long>(base + lane) * step[run]] - top);
-                        const int here = min(32, count[run] - base);
-                        for (int c = 0; c < here; c += kFlight) {
-                            float held[kFlight][kOwn], w[kFlight];
-#pragma unroll
-                            for (int k = 0; k < kFlight; ++k) {
-                                w[k] = __shfl_sync(0xffffffffu, weight, (c + k) & 31);
-                                if (c + k >= here) w[k] = 0.0f;
-#pragma unroll
-                                for (int i = 0; i < kOwn; ++i) held[k][i] = 0.0f;
-                                if (w[k] != 0.0f) {        // an empty slot holds no values
-                                    const float* source =
-                                        p.w.partial_out + (first[run] + static_cast<long long>(base + c + k) * step[run]) * DIM + lane * kOwn;
-                                    if constexpr (kOwn == 4) {
-                                        *reinterpret_cast<float4*>(held[k]) = *reinterpret_cast<const float4*>(source);
-                                    } else {
-                                        *reinterpret_cast<float2*>(held[k]) = *reinterpret_cast<const float2*>(source);
-                                    }
-                                }
-                            }
-#pragma unroll
-                            for (int k = 0; k < kFlight; ++k) {
-                                total += w[k];
-#pragma unroll
-                                for (int i = 0; i < kOwn; ++i) sums[i] = fmaf(w[k], held[k][i], sums[i]);
-                            }
-                        }
+                for (int k = 0; k < kFlight; ++k) {
+                    const float* values = p.w.partial_out + row_of(base + min(k, here - 1)) * DIM + lane * kOwn;
+                    if constexpr (kOwn == 4) {
+                        *reinterpret_cast<float4*>(held[k]) = *reinterpret_cast<const float4*>(values);
+                    } else {
+                        *reinterpret_cast<float2*>(held[k]) = *reinterpret_cast<const float2*>(values);
                     }
+                }
+                broken |= __any_sync(0xffffffffu, lse != lse) != 0;
+                float new_top = fmaxf(top, lse);
+#pragma unroll
+                for (int d = 16; d > 0; d >>= 1) new_top = fmaxf(new_top, __shfl_xor_sync(0xffffffffu, new_top, d));
+                if (new_top == -INFINITY) continue;
+                const float shrink = exp2_fast(top - new_top), weight = exp2_fast(lse - new_top);
+                top = new_top;
+                total *= shrink;
+#pragma unroll
+                for (int i = 0; i < kOwn; ++i) sums[i] *= shrink;
+#pragma unroll
+                for (int k = 0; k < kFlight; ++k) {
+                    const float w = __shfl_sync(0xffffffffu, weight, k);
+                    total += w;
+#pragma unroll
+                    for (int i = 0; i < kOwn; ++i) sums[i] = w != 0.0f ? fmaf(w, held[k][i], sums[i]) : sums[i];   // an empty slot holds no values
+                }
             }
             const bool empty = total == 0.0f && !broken;
             const float nan = __int_as_float(0x7fffffff);

@@ -305,6 +305,8 @@ int itk_attention(const itk_attention_args* args, itk_stream_t stream) {
     params.tile_tokens = kAttnTile / params.group;
     params.sm_count = std::min(device.sm_count, kAttnMaxSms);
     params.withhold_loads = a.withhold_loads;
+    params.inverse_sms = 1.0f / static_cast<float>(params.sm_count);
+    params.out_sectors = (reinterpret_cast<uintptr_t>(a.out) & 31u) == 0 && a.out_token_stride % 16 == 0 && a.out_head_stride % 16 == 0;
     params.scale_log2 = a.scale * kLog2e;
     params.lazy = kAttnLazy / params.scale_log2;
     params.wait_polls = static_cast<uint32_t>(std::min(std::max((a.wait_limit_ns != 0 ? a.wait_limit_ns : kWaitLimitNs) / 1000, 1ull), 1ull << 31));

@@ -55,13 +55,15 @@ constexpr float kAttnLazy = 8.0f;              // log2 of how far weights may ex
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
+constexpr int kAttnSharedTail = 2048;
+
 template <int DIM>
 struct AttnShape {
     static constexpr int kChunks = DIM / 64;                    // 128-byte wide column chunks
     static constexpr int kTileBytes = kAttnTile * DIM * 2;
     static constexpr int kStages = DIM == 128 ? 5 : 10;         // 160 KB of key and value tiles in flight
     static constexpr int kSmemTiles = (2 + kStages) * kTileBytes;
-    static constexpr int kSmemBytes = kSmemTiles + 1024;
+    static constexpr int kSmemBytes = kSmemTiles + kAttnSharedTail;
 };
 
 // One unit of work for every key head.
@@ -105,6 +107,7 @@ struct AttnParams {
     AttnWorkspace w;
     int* status;
     int group, tile_tokens, sm_count, withhold_loads;
+    int small_plan;                                // no plan kernel ran: see attn_small_plan
     int out_sectors;                               // rows of the output start on 32-byte boundaries
     float inverse_sms;                             // 1 / sm_count
     float scale_log2, lazy;                        // lazy: kAttnLazy in units of the scores
@@ -401,6 +404,30 @@ __device__ __forceinline__ int attn_chunks(const AttnEntry& e, int cost, int who
     return static_cast<int>((static_cast<unsigned>(e.tiles) + per - 1) / per);
 }
 
+// Slots of an entry cut into `chunks` (0: no key at all), and whether its results are partial ones.
+__device__ __forceinline__ bool attn_slots(const AttnParams& p, AttnEntry& entry, int chunks) {
+    const int longest_chunk = chunks > 0 ? (entry.tiles + chunks - 1) / chunks : 0;
+    entry.item.slots = chunks * (!entry.pair && longest_chunk > 1 ? 2 : 1);
+    entry.item.partial = -1;
+    return p.a.prefix_keys > 0 || entry.item.slots > 1;
+}
+
+// Chunk c of `count` of an entry whose slots are set; the first tiles % count chunks are one tile longer.
+__device__ __forceinline__ AttnItem attn_chunk(const AttnEntry& entry, int c, int count) {
+    AttnItem item = entry.item;
+    const int even = entry.tiles / count, odd = entry.tiles - even * count;
+    item.tile_begin = c * even + min(c, odd);
+    item.tiles = even + (c < odd ? 1 : 0);
+    item.slot = c * (entry.item.slots / count);
+    return item;
+}
+
+// A fair share of the work of all SMs, in fp32: it only has to be near.  (A chunk costs at most 2^29, more than any
+// entry, 2^24 tiles of cost 4, does.)
+__device__ __forceinline__ int attn_share(const AttnParams& p, unsigned long long cost) {
+    return static_cast<int>(fminf(ceilf(static_cast<float>(cost) * p.a.kv_heads * p.inverse_sms) + 1.0f, 536870912.0f));
+}
+
 // Most of a small call's time before its first key is read goes by in here: one pass over the lengths, entries kept in
 // registers, five block barriers when the items fit one wave (their order does not matter then).
 template <int THREADS>
@@ -472,8 +499,7 @@ __global__ void __launch_bounds__(THREADS) itk_attention_plan_kernel(const __gri
     for (int step = 16; step > 0; step >>= 1) cost += __shfl_xor_sync(0xffffffffu, cost, step);
     if (lane == 0 && cost != 0) atomicAdd(&total_cost, cost);
     __syncthreads();
-    // in fp32: it only has to be near.  (A chunk costs at most 2^29, more than any entry, 2^24 tiles of cost 4, does.)
-    const int share = static_cast<int>(fminf(ceilf(static_cast<float>(total_cost) * kv_heads * p.inverse_sms) + 1.0f, 536870912.0f));
+    const int share = attn_share(p, total_cost);
     int mine[kAttnTries] = {};
     for (int e = tx; e < entries; e += THREADS) {
         const AttnEntry entry = entry_at(e);
@@ -544,12 +570,8 @@ __global__ void __launch_bounds__(THREADS) itk_attention_plan_kernel(const __gri
     for (int e = tx; e < entries; e += THREADS) {
         AttnEntry entry = entry_at(e);
         const int chunks = attn_chunks(entry, chunk, whole);               // 0: no key at all
-        const int longest_chunk = chunks > 0 ? (entry.tiles + chunks - 1) / chunks : 0;
-        const int lanes = !entry.pair && longest_chunk > 1 ? 2 : 1;
         const int rows = entry.item.tokens * p.group;
-        entry.item.slots = chunks * lanes;
-        entry.item.partial = -1;
-        const bool joined = p.a.prefix_keys > 0 || entry.item.slots > 1;
+        const bool joined = attn_slots(p, entry, chunks);
         if (joined && entry.item.slots > 0) {
             const int needed = entry.item.slots * rows * kv_heads;
             const int first = atomicAdd(&partial_rows, needed);
@@ -570,17 +592,86 @@ __global__ void __launch_bounds__(THREADS) itk_attention_plan_kernel(const __gri
         if (chunks == 0 && joined) entry.item.tokens = 0;           // the prefix alone: a place in the list, but nothing to do
         const int count = max(1, chunks);
         const int place = atomicAdd(one_wave ? &item_count : &bins[bin_of(entry, count)], count);
-        const int even = entry.tiles / count, odd = entry.tiles - even * count;        // the first `odd` chunks are one tile longer
-        entry.item.tile_begin = 0;
-        for (int c = 0; c < count; ++c) {
-            entry.item.tiles = even + (c < odd ? 1 : 0);
-            entry.item.slot = c * lanes;
-            if (place + c < p.w.max_items) p.w.items[place + c] = entry.item;
-            entry.item.tile_begin += entry.item.tiles;
-        }
+        for (int c = 0; c < count; ++c)
+            if (place + c < p.w.max_items) p.w.items[place + c] = attn_chunk(entry, c, count);
     }
     __syncthreads();
     if (tx == 0) *p.w.counters = AttnCounters{min(item_count, p.w.max_items), min(combine_count, p.w.max_combines), partial_rows, rows_end, p.sm_count};
+}
+
+// The plan of a call with at most 32 requests and 32 entries that fit one wave of CTAs uncut: every CTA's producer warp
+// works out the whole of it for itself, a request and an entry per lane, and takes the one unit that has the CTA's number.
+// That saves the plan's launch and the wait for it.  CTA 0 also writes down what the join needs.  `cache` and `first` are
+// scratch for the requests.  Returns whether there is a unit.
+constexpr int kAttnSmallEntries = 32;
+
+__device__ __forceinline__ int warp_prefix(int value, int lane, int& total) {
+    int upto = value;
+#pragma unroll
+    for (int step = 1; step < 32; step <<= 1) {
+        const int other = __shfl_up_sync(0xffffffffu, upto, step);
+        if (lane >= step) upto += other;
+    }
+    total = __shfl_sync(0xffffffffu, upto, 31);
+    return upto - value;
+}
+
+__device__ __forceinline__ bool attn_small_plan(const AttnParams& p, AttnRequest* cache, int* first, int4* unit, int lane) {
+    const int span = 2 * p.tile_tokens, kv_heads = p.a.kv_heads;
+    const int rows_end = min(max(p.a.cu_q[p.a.requests], 0), p.a.tokens);
+    bool bad = false;
+    int mine = 0, own;
+    if (lane < p.a.requests) {
+        const AttnRequest request = attn_request(p.a, lane, bad);
+        cache[lane] = request;
+        mine = (request.q_count + span - 1) / span;
+    }
+    first[lane] = warp_prefix(mine, lane, own);
+    if (bad && blockIdx.x == 0) atomicOr(p.status, ITK_SERVING_BAD_LENGTHS);
+    __syncwarp();
+    const int prefix_entries = p.a.prefix_keys > 0 ? (rows_end + span - 1) / span : 0;
+    const bool there = lane < prefix_entries + own;             // (the host has counted them: 32 at most)
+    AttnEntry entry{};
+    entry.unit = 1;
+    if (there) entry = attn_entry(p, AttnRequests{cache, first, true}, lane, prefix_entries, rows_end);
+    const int cost = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(entry.tiles) * entry.unit);
+    const int share = attn_share(p, static_cast<unsigned>(cost));
+    int counts[kAttnTries];
+#pragma unroll
+    for (int t = 0; t < kAttnTries; ++t) counts[t] = there ? max(1, attn_chunks(entry, share + share / kAttnTries * t, 0)) : 0;
+    int chunk = 1 << 30;            // nothing is cut: that fits a wave
+#pragma unroll
+    for (int t = kAttnTries - 1; t >= 0; --t)
+        if (static_cast<int>(__reduce_add_sync(0xffffffffu, counts[t])) * kv_heads <= p.sm_count) chunk = share + share / kAttnTries * t;
+
+    const int chunks = there ? attn_chunks(entry, chunk, 0) : 0, count = there ? max(1, chunks) : 0;
+    const bool joined = there && attn_slots(p, entry, chunks);
+    const int rows = there ? entry.item.tokens * p.group : 0;
+    int items, partial, records;
+    const int place = warp_prefix(count, lane, items);
+    const int first_row = warp_prefix(joined ? entry.item.slots * rows * kv_heads : 0, lane, partial);
+    if (joined && entry.item.slots > 0) entry.item.partial = partial <= p.w.max_partial_rows ? first_row : -2;
+    const int index = static_cast<int>(blockIdx.x) / kv_heads, head = static_cast<int>(blockIdx.x) - index * kv_heads;
+    const bool found = index >= place && index < place + count && !(chunks == 0 && joined);
+    if (found) {
+        const AttnItem item = attn_chunk(entry, index - place, count);
+        unit[0] = make_int4(item.q_first, item.tokens, item.tile_begin, item.tiles);
+        unit[1] = make_int4(item.keys, item.visible, item.slope, item.request);
+        unit[2] = make_int4(item.k_first, item.partial, item.slot, item.slots);
+        unit[3] = make_int4(head, 1, 0, 0);
+    }
+    if (blockIdx.x == 0) {
+        const int usable = entry.item.partial < 0 ? 0 : entry.item.slots;
+        if (there && entry.prefix) p.w.prefix_slots[lane] = make_int2(entry.item.partial, usable);
+        const int wanted = joined && !entry.prefix ? (rows + kAttnCombineRows - 1) / kAttnCombineRows : 0;
+        const int at = warp_prefix(wanted, lane, records);
+        for (int r = 0; r < wanted; ++r)
+            if (at + r < p.w.max_combines)
+                p.w.combines[at + r] = AttnCombine{entry.item.q_first, entry.item.tokens, entry.item.partial, usable, r * kAttnCombineRows, {}};
+        if (lane == 0) *p.w.counters = AttnCounters{items, min(records, p.w.max_combines), partial, rows_end, 0};
+    }
+    __syncwarp();
+    return __any_sync(0xffffffffu, found) != 0;
 }
 
 // ------------------------------------------------------------------ attention
@@ -592,11 +683,13 @@ struct AttnShared {
     uint64_t pv_done[2], o_full[2], o_empty[2];
     uint64_t item_full[kAttnQueue], item_empty[kAttnQueue];
     int poison[kAttnPoison];
+    AttnRequest small_requests[kAttnSmallEntries];
+    int small_first[kAttnSmallEntries];
     int4 items[kAttnQueue][4];                // the CTA's next units of work: the item, then (key head, 1) or (-, 0) at the end
     uint32_t tmem_base;
     int abort;
 };
-static_assert(sizeof(AttnShared) <= 1024, "barriers fit the tail of the shared-memory block");
+static_assert(sizeof(AttnShared) <= kAttnSharedTail, "barriers fit the tail of the shared-memory block");
 
 // What an item means for one lane.
 struct AttnLanes {
@@ -740,26 +833,38 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
         // The first unit of a CTA is the one with its number, the others are taken when their turn comes.
         int unit = static_cast<int>(blockIdx.x), next_unit = 0;
         for (; ok; unit = __shfl_sync(0xffffffffu, next_unit, 0)) {
-            const int index = min(unit / kv_heads, p.w.max_items - 1);
-            // read before it is known whether there is such an item: the loads overlap
-            const int4* source = reinterpret_cast<const int4*>(p.w.items + index);
-            const int4 a = source[0], b = source[1], c = source[2];
-            const bool there = unit < p.w.counters->items * kv_heads;
-            item = attn_item(a, b, c);
-            head = unit - index * kv_heads;
-            if (there && lane == 0) next_unit = atomicAdd(&p.w.counters->next, 1);
-            if (there && item.tokens == 0) continue;              // nothing to do
-            ok = wait(&sh.item_empty[units % kAttnQueue], ((units / kAttnQueue) & 1) ^ 1);
-            if (!ok) break;
-            if (lane == 0) {
-                int4* target = sh.items[units % kAttnQueue];
-                target[0] = a;
-                target[1] = b;
-                target[2] = c;
-                target[3] = make_int4(head, there ? 1 : 0, 0, 0);
-                mbar_arrive(&sh.item_full[units % kAttnQueue]);
+            int4* place = sh.items[units % kAttnQueue];
+            bool there;
+            if (p.small_plan != 0) {
+                // (at most one unit: nothing in the queue is waited for)
+                there = units == 0 && attn_small_plan(p, sh.small_requests, sh.small_first, place, lane);
+                if (!there && lane == 0) place[3] = make_int4(0, 0, 0, 0);
+                __syncwarp();
+                if (there) {
+                    item = attn_item(load_shared_again(place), load_shared_again(place + 1), load_shared_again(place + 2));
+                    head = load_shared_again(place + 3).x;
+                }
+            } else {
+                const int index = min(unit / kv_heads, p.w.max_items - 1);
+                // read before it is known whether there is such an item: the loads overlap
+                const int4* source = reinterpret_cast<const int4*>(p.w.items + index);
+                const int4 a = source[0], b = source[1], c = source[2];
+                there = unit < p.w.counters->items * kv_heads;
+                item = attn_item(a, b, c);
+                head = unit - index * kv_heads;
+                if (there && lane == 0) next_unit = atomicAdd(&p.w.counters->next, 1);
+                if (there && item.tokens == 0) continue;              // nothing to do
+                ok = wait(&sh.item_empty[units % kAttnQueue], ((units / kAttnQueue) & 1) ^ 1);
+                if (!ok) break;
+                if (lane == 0) {
+                    place[0] = a;
+                    place[1] = b;
+                    place[2] = c;
+                    place[3] = make_int4(head, there ? 1 : 0, 0, 0);
+                }
             }
             __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.item_full[units % kAttnQueue]);
             ++units;
             if (!there) break;
             const AttnLanes l = attn_lanes(item, p.tile_tokens);

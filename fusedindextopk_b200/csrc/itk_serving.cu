@@ -180,12 +180,16 @@ cudaError_t launch_after(Kernel kernel, int grid, int threads, size_t smem, cuda
 
 template <typename T, int DIM>
 int launch_attention(const AttnParams& params, cudaStream_t stream) {
-    // barriers of a small block cost a third of a large one's; the large one is for batches with more entries than threads
-    if (params.w.max_entries <= 256)
-        itk_attention_plan_kernel<256><<<1, 256, 0, stream>>>(params);
-    else
-        itk_attention_plan_kernel<1024><<<1, 1024, 0, stream>>>(params);
-    ITK_CUDA(launch_after(itk_attention_kernel<T, DIM>, params.sm_count, kAttnThreads, AttnShape<DIM>::kSmemBytes, stream, params));
+    if (params.small_plan) {
+        itk_attention_kernel<T, DIM><<<params.sm_count, kAttnThreads, AttnShape<DIM>::kSmemBytes, stream>>>(params);
+    } else {
+        // barriers of a small block cost a third of a large one's; the large one is for batches with more entries than threads
+        if (params.w.max_entries <= 256)
+            itk_attention_plan_kernel<256><<<1, 256, 0, stream>>>(params);
+        else
+            itk_attention_plan_kernel<1024><<<1, 1024, 0, stream>>>(params);
+        ITK_CUDA(launch_after(itk_attention_kernel<T, DIM>, params.sm_count, kAttnThreads, AttnShape<DIM>::kSmemBytes, stream, params));
+    }
     ITK_CUDA(launch_after(itk_attention_join_kernel<T, DIM>, 4 * params.sm_count, kJoinThreads, 0, stream, params));
     return launched("itk_attention_kernel");
 }
@@ -305,6 +309,8 @@ int itk_attention(const itk_attention_args* args, itk_stream_t stream) {
     params.tile_tokens = kAttnTile / params.group;
     params.sm_count = std::min(device.sm_count, kAttnMaxSms);
     params.withhold_loads = a.withhold_loads;
+    const long long entries = params.w.max_entries + (a.prefix_keys > 0 ? a.tokens / (2 * params.tile_tokens) + 1 : 0);
+    params.small_plan = entries <= kAttnSmallEntries && entries * a.kv_heads <= params.sm_count && a.requests <= kAttnSmallEntries;
     params.inverse_sms = 1.0f / static_cast<float>(params.sm_count);
     params.out_sectors = (reinterpret_cast<uintptr_t>(a.out) & 31u) == 0 && a.out_token_stride % 16 == 0 && a.out_head_stride % 16 == 0;
     params.scale_log2 = a.scale * kLog2e;

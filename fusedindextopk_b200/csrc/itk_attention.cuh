@@ -51,6 +51,7 @@ constexpr int kAttnMaxStages = 10;
 constexpr int kAttnQueue = 4;                  // units of work the producer may be ahead of the last reader
 constexpr int kAttnReaders = 2 * kAttnSoftmaxWarps + 3;    // warps that read them: softmax, issuers, guard
 constexpr int kAttnPoison = 16;                // items the guard may be ahead of an epilogue, with room to spare
+constexpr int kAttnPolynomial = 8;             // one pair of weights in so many takes exp2_polynomial (4: no gain, none: 4 % slower)
 constexpr float kAttnLazy = 8.0f;              // log2 of how far weights may exceed 1 before the maximum moves
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -219,6 +220,8 @@ __device__ __forceinline__ int4 load_shared_again(const int4* address) {
     return v;
 }
 
+__device__ __forceinline__ float2 neg2(float2 a) { return make_float2(-a.x, -a.y); }
+
 // Maximum of three; a NaN among them is passed over.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
@@ -265,6 +268,25 @@ __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// 2^z on the FMA pipe, for some of the weights: the special-function unit gives 16 exponentials a cycle to an SM, which
+// is what the softmax is short of.  z = n + f with n the nearest whole number (adding 1.5 * 2^23 leaves it in the low bits),
+// 2^f by a polynomial of degree 5, fitted for the least relative error on [-1/2, 1/2] by iteratively reweighted least
+// squares (7.5e-8), 2^n by its exponent bits.  Below the normal range the result is 0, as exp2_fast's is; NaN stays NaN.
+// z <= 127 is all that is asked for (weights are at most 2^kAttnLazy).
+__device__ __forceinline__ float2 exp2_polynomial(float2 z) {
+    auto both = [](float x) { return make_float2(x, x); };
+    const float2 shifted = add2(z, both(12582912.0f));
+    const float2 f = add2(z, neg2(add2(shifted, both(-12582912.0f))));
+    float2 q = fma2(both(0.0013276471520115847f), f, both(0.009675541330697653f));
+    q = fma2(q, f, both(0.05550713274959883f));
+    q = fma2(q, f, both(0.24022119723933577f));
+    q = fma2(q, f, both(0.6931469670638649f));
+    q = fma2(q, f, both(1.0000000716546569f));
+    const float low = q.x * __uint_as_float((__float_as_uint(shifted.x) << 23) + 0x3f800000u);
+    const float high = q.y * __uint_as_float((__float_as_uint(shifted.y) << 23) + 0x3f800000u);
+    return make_float2(z.x < -126.0f ? 0.0f : low, z.y < -126.0f ? 0.0f : high);
 }
 
 template <typename T>
@@ -1117,30 +1139,31 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
             };
             uint32_t s[2][32];
             float step_top = -INFINITY;
-            // the scores of a step, which are on their way to s: masked, and their maximum
+            // the scores of a step, which have arrived in s: masked where a row does not see all of them, and their maximum
             auto take_scores = [&]() {
-                tmem_load_wait(s[0]);
-                tmem_load_wait(s[1]);
                 if (left_all < kAttnHalf) {
                     mask_scores(s[0], left);
                     mask_scores(s[1], left - 32);
                 }
                 step_top = fmaxf(top_of(s[0]), top_of(s[1]));
             };
+            auto next_step = [&]() {
+                const int on = !pair && (at & 1) != 0 ? kAttnHalf + kAttnTile : kAttnHalf;     // the other lane's tile is passed over
+                left -= on;
+                left_all -= on;
+            };
             // the weights of 32 scores, rounded to the element type for the product; the sum takes them unrounded
             const float2 scale2 = make_float2(scale, scale);
-            auto weigh = [&](const uint32_t (&part)[32], uint32_t address) {
+            auto weigh = [&](const uint32_t (&part)[32], uint32_t (&packed)[16]) {
                 const float2 base2 = make_float2(-base, -base);
                 float2 sum = make_float2(0.0f, 0.0f);
-                uint32_t packed[16];
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
                     const float2 z = fma2(make_float2(__uint_as_float(part[2 * k]), __uint_as_float(part[2 * k + 1])), scale2, base2);
-                    const float2 w = make_float2(exp2_fast(z.x), exp2_fast(z.y));
+                    const float2 w = k % kAttnPolynomial == kAttnPolynomial - 1 ? exp2_polynomial(z) : make_float2(exp2_fast(z.x), exp2_fast(z.y));
                     sum = add2(sum, w);
                     packed[k] = Element<T>::pack(w.x, w.y);
                 }
-                tmem_store_16(address, packed);
                 total = add2(total, sum);
             };
             if (!active) {
@@ -1154,6 +1177,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
                 tcgen05_fence_after_sync();
                 tmem_load_32(tmem_s, s[0]);
                 tmem_load_32(tmem_s + 32, s[1]);
+                tmem_load_wait(s[0]);
+                tmem_load_wait(s[1]);
                 take_scores();
                 top = step_top;
                 base = top == -INFINITY ? 0.0f : top * scale;
@@ -1163,27 +1188,44 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
                     uint64_t* next_full = &sh.s_full[x][(at + 1) & 1];
                     const uint32_t next_phase = ((at + 1) >> 1) & 1;
                     // The next step's scores, when they are there by now, are loaded into the registers that this
-                    // step's exponentials free: the loads and the hand-over run behind the second half of those.
+                    // step's exponentials free: the loads, half of the maximum and the hand-over run behind the
+                    // second half of those.
                     const bool early = more && __all_sync(0xffffffffu, mbar_test_wait(next_full, next_phase));
-                    if (early) tcgen05_fence_after_sync();
-                    weigh(s[0], here);
-                    if (early) tmem_load_32(there, s[0]);
-                    weigh(s[1], here + 16);
-                    if (early) tmem_load_32(there + 32, s[1]);
-                    tmem_store_wait();
-                    hand_over();
-                    if (!more) break;
-                    if (!early) {
+                    uint32_t packed[16];
+                    weigh(s[0], packed);
+                    tmem_store_16(here, packed);
+                    if (early) {
+                        tcgen05_fence_after_sync();
+                        tmem_load_32(there, s[0]);
+                        next_step();
+                        weigh(s[1], packed);
+                        tmem_load_wait(s[0]);
+                        const float lower_top = top_of(s[0]);
+                        tmem_store_16(here + 16, packed);
+                        tmem_load_32(there + 32, s[1]);
+                        tmem_store_wait();
+                        hand_over();
+                        tmem_load_wait(s[1]);
+                        if (left_all < kAttnHalf)
+                            take_scores();
+                        else
+                            step_top = fmaxf(lower_top, top_of(s[1]));
+                    } else {
+                        weigh(s[1], packed);
+                        tmem_store_16(here + 16, packed);
+                        tmem_store_wait();
+                        hand_over();
+                        if (!more) break;
                         ok = wait(next_full, next_phase);
                         if (!ok) break;
                         tcgen05_fence_after_sync();
                         tmem_load_32(there, s[0]);
                         tmem_load_32(there + 32, s[1]);
+                        next_step();
+                        tmem_load_wait(s[0]);
+                        tmem_load_wait(s[1]);
+                        take_scores();
                     }
-                    const int on = !pair && (at & 1) != 0 ? kAttnHalf + kAttnTile : kAttnHalf;     // the other lane's tile is passed over
-                    left -= on;
-                    left_all -= on;
-                    take_scores();
                     const bool moves = step_top > top + p.lazy;
                     if (__any_sync(0xffffffffu, moves)) {
                         float shrink = 1.0f;

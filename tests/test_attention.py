@@ -247,10 +247,11 @@ def test_rows_behind_the_last_request(device, q_len, k_len):
 @pytest.mark.gpu
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
 @pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 128), (16, 2, 64)])
-def test_what_a_row_does_not_see_does_not_reach_it(device, bad, heads, kv_heads, dim):
+@pytest.mark.parametrize("at", [317, 271, 0, 499])
+def test_what_a_row_does_not_see_does_not_reach_it(device, bad, heads, kv_heads, dim, at):
     """Keys and values behind a row's last visible key may hold anything; the rows that see them get it."""
 
-    n, at = 500, 317
+    n = 500
     q, k, v = make(device, [n], [n], heads, kv_heads, dim, torch.bfloat16, seed=1)
     clean = expected(q, [n], [(k, v, None, None)])
     k_bad, v_bad = k.clone(), v.clone()

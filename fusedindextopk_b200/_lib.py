@@ -103,7 +103,7 @@ class AppendArgs(ctypes.Structure):
 
 class KvSegment(ctypes.Structure):
     _fields_ = [
-        ("k", c_void_p), ("v", c_void_p), ("table", c_void_p), ("table_stride", c_longlong),
+        ("table_stride", c_longlong),
         ("k_page_stride", c_longlong), ("k_row_stride", c_longlong), ("k_head_stride", c_longlong),
         ("v_page_stride", c_longlong), ("v_row_stride", c_longlong), ("v_head_stride", c_longlong),
         ("pages", c_int), ("page_size", c_int), ("table_pages", c_int),
@@ -114,6 +114,8 @@ class AttentionArgs(ctypes.Structure):
     _fields_ = [
         ("q", c_void_p), ("out", c_void_p), ("lse", c_void_p), ("cu_q", c_void_p), ("cu_k", c_void_p),
         ("lens_k", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+        ("k", c_void_p), ("v", c_void_p), ("table", c_void_p),
+        ("k_prefix", c_void_p), ("v_prefix", c_void_p), ("prefix_table", c_void_p),
         ("q_token_stride", c_longlong), ("q_head_stride", c_longlong),
         ("out_token_stride", c_longlong), ("out_head_stride", c_longlong), ("wait_limit_ns", ctypes.c_ulonglong),
         ("own", KvSegment), ("prefix", KvSegment), ("scale", ctypes.c_float), ("element", c_int),
@@ -237,12 +239,11 @@ class CallTemplate:
         self.bytes = bytes(args)
         self.__dict__.update(extra)
 
-    def fill(self, *pointers: tuple[int, Any]) -> Any:
-        """A copy of the block with ``(offset, values)`` runs of 64-bit words put in."""
+    def fill(self, words: Any) -> Any:
+        """A copy of the block with the 64-bit words it begins with put in."""
 
         block = self.block.from_buffer_copy(self.bytes)
-        for offset, values in pointers:
-            struct.pack_into("<%dQ" % len(values), block, offset, *values)
+        _WORDS[len(words)].pack_into(block, 0, *words)
         return block
 
     @classmethod
@@ -253,6 +254,9 @@ class CallTemplate:
         return template
 
 
+_WORDS = [struct.Struct("<%dQ" % n) for n in range(32)]
+
+
 def metadata(tensors: tuple) -> tuple:
     return tuple([(t.shape, t.stride(), t.dtype, t.device) for t in tensors])
 
@@ -260,11 +264,14 @@ def metadata(tensors: tuple) -> tuple:
 def launch(torch: Any, function: Any, block: Any, device: Any) -> None:
     """Calls a C entry on the current stream of ``device``."""
 
-    if torch.cuda.current_device() == device.index:
-        check(function(block, torch._C._cuda_getCurrentRawStream(device.index)))
+    index = device.index
+    if torch.cuda.current_device() == index:
+        status = function(block, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            check(function(block, torch._C._cuda_getCurrentRawStream(device.index)))
+            status = function(block, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        check(status)
 
 
 def check_serving_status(device: Any = None) -> None:

@@ -68,8 +68,8 @@ def _segment(k: Any, v: Any, table: Any = None) -> Any:
     """Strides and sizes of packed (``table`` is None) or paged keys, without their addresses."""
 
     if table is None:
-        return _lib.KvSegment(None, None, None, 0, 0, k.stride(0), k.stride(1), 0, v.stride(0), v.stride(1), 1, k.shape[0], 0)
-    return _lib.KvSegment(None, None, None, table.stride(0) if table.dim() == 2 else 0, *k.stride()[:3], *v.stride()[:3],
+        return _lib.KvSegment(0, 0, k.stride(0), k.stride(1), 0, v.stride(0), v.stride(1), 1, k.shape[0], 0)
+    return _lib.KvSegment(table.stride(0) if table.dim() == 2 else 0, *k.stride()[:3], *v.stride()[:3],
                           k.shape[0], k.shape[1], table.shape[-1])
 
 
@@ -116,19 +116,17 @@ def _check_call(torch: Any, q: Any, own: tuple, prefix: tuple | None, prefix_key
     _require(0.0 < scale < 1e38, "scale must be positive and finite")
     strides = out.stride() if out is not None else (heads * dim, dim)
     args = _lib.AttentionArgs(
-        None, None, None, None, None, None, None, 0, q.stride(0), q.stride(1), strides[0], strides[1], 0, _segment(*own),
+        None, None, None, None, None, None, None, 0, None, None, None, None, None, None, q.stride(0), q.stride(1), strides[0], strides[1], 0, _segment(*own),
         _segment(*prefix) if prefix_keys else _lib.KvSegment(), scale,
         _lib.ELEMENT_BF16 if q.dtype == torch.bfloat16 else _lib.ELEMENT_FP16, tokens, heads, own[0].shape[-2], dim, requests,
         prefix_keys, int(causal), int(out is None), 0)
     needed = ctypes.c_size_t(0)
     if tokens:
         _lib.check(_lib.load_library().itk_attention_workspace_bytes(ctypes.byref(args), ctypes.byref(needed)))
-    return _lib.CallTemplate(args, workspace_bytes=needed.value, device=device, tokens=tokens)
+    return _lib.CallTemplate(args, workspace_bytes=needed.value, device=device, tokens=tokens, paged=paged)
 
 
 _TEMPLATES: dict = {}
-_OWN_OFFSET = _lib.AttentionArgs.own.offset
-_PREFIX_OFFSET = _lib.AttentionArgs.prefix.offset
 
 
 def _attend(q: Any, own: tuple, prefix: tuple | None, prefix_keys: int, cu_seqlens_q: Any, lengths: Any, causal: bool,
@@ -147,25 +145,25 @@ def _attend(q: Any, own: tuple, prefix: tuple | None, prefix_keys: int, cu_seqle
     if template is None:
         template = _lib.CallTemplate.keep(_TEMPLATES, key, _check_call(
             torch, q, own, prefix, prefix_keys, cu_seqlens_q, lengths, out, causal, scale))
-    device, tokens = template.device, template.tokens
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=device) if return_lse else None
-    if tokens:
+        out = q.new_empty(q.shape)
+    lse = q.new_empty(q.shape[:2], dtype=torch.float32) if return_lse else None
+    if template.tokens:
         # of the caching allocator, on the call's stream: two calls, streams or captured graphs never share it
-        workspace = torch.empty(template.workspace_bytes, dtype=torch.uint8, device=device)
-        row_addresses = (q.data_ptr(), out.data_ptr())
-        own_addresses = [t.data_ptr() for t in own]
-        prefix_addresses = [t.data_ptr() for t in prefix] if prefix_keys else []
-        for address in (*row_addresses, *own_addresses[:2], *prefix_addresses[:2]):
-            _require(address % 16 == 0, "q, out, keys and values must be 16-byte aligned")
-        paged = len(own) == 3
-        block = template.fill(
-            (0, (*row_addresses, 0 if lse is None else lse.data_ptr(), cu_seqlens_q.data_ptr(),
-                 0 if paged else lengths.data_ptr(), lengths.data_ptr() if paged else 0, workspace.data_ptr(),
-                 template.workspace_bytes)),
-            (_OWN_OFFSET, own_addresses), (_PREFIX_OFFSET, prefix_addresses))
-        _lib.launch(torch, _lib.load_library().itk_attention, block, device)
+        workspace = q.new_empty(template.workspace_bytes, dtype=torch.uint8)
+        # in the order of the argument block: rows, lengths, workspace, own keys, prefix
+        k, v = own[0].data_ptr(), own[1].data_ptr()
+        rows, result, ends = q.data_ptr(), out.data_ptr(), lengths.data_ptr()
+        words = [rows, result, 0 if lse is None else lse.data_ptr(), cu_seqlens_q.data_ptr(), 0 if template.paged else ends,
+                 ends if template.paged else 0, workspace.data_ptr(), template.workspace_bytes, k, v,
+                 own[2].data_ptr() if template.paged else 0]
+        aligned = rows | result | k | v
+        if prefix_keys:
+            k, v = prefix[0].data_ptr(), prefix[1].data_ptr()
+            words += [k, v, prefix[2].data_ptr() if template.paged else 0]
+            aligned |= k | v
+        _require(aligned & 15 == 0, "q, out, keys and values must be 16-byte aligned")
+        _lib.launch(torch, _lib.load_library().itk_attention, template.fill(words), template.device)
     return (out, lse) if return_lse else out
 
 

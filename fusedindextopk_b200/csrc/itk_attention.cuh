@@ -738,8 +738,9 @@ __device__ __forceinline__ AttnItem attn_item(const int4& a, const int4& b, cons
 // Where key tile t of a segment lies.
 __device__ __forceinline__ int attn_page(const AttnParams& p, const AttnItem& item, int t) {
     const itk_kv_segment& seg = item.request < 0 ? p.a.prefix : p.a.own;
-    if (seg.table == nullptr) return 0;
-    const int32_t* table = seg.table + (item.request < 0 ? 0 : item.request * seg.table_stride);
+    const int32_t* table = item.request < 0 ? p.a.prefix_table : p.a.table;
+    if (table == nullptr) return 0;
+    if (item.request >= 0) table += item.request * seg.table_stride;
     const int page = table[t / (seg.page_size / kAttnTile)];
     if (page < 0 || page >= seg.pages) {
         atomicOr(p.status, ITK_SERVING_BAD_PAGE);
@@ -753,11 +754,11 @@ __device__ __forceinline__ const T* attn_value_row(const AttnParams& p, const At
     const itk_kv_segment& seg = item.request < 0 ? p.a.prefix : p.a.own;
     long long row = item.k_first + key;
     long long page = 0;
-    if (seg.table != nullptr) {
+    if ((item.request < 0 ? p.a.prefix_table : p.a.table) != nullptr) {
         page = attn_page(p, item, key / kAttnTile);
         row = key % seg.page_size;
     }
-    return static_cast<const T*>(seg.v) + page * seg.v_page_stride + row * seg.v_row_stride + head * seg.v_head_stride;
+    return static_cast<const T*>(item.request < 0 ? p.a.v_prefix : p.a.v) + page * seg.v_page_stride + row * seg.v_row_stride + head * seg.v_head_stride;
 }
 
 // Ring position of the value tile t of an item.  Pair: K0 V0 K1 V1 ...  Split (the lanes take turns and each is one key
@@ -904,7 +905,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
             const itk_kv_segment& seg = item.request < 0 ? p.a.prefix : p.a.own;
             const CUtensorMap* map_k = item.request < 0 ? &p.map_k_prefix : &p.map_k;
             const CUtensorMap* map_v = item.request < 0 ? &p.map_v_prefix : &p.map_v;
-            const bool table = seg.table != nullptr;
+            const bool table = (item.request < 0 ? p.a.prefix_table : p.a.table) != nullptr;
             const int steps = 2 * item.tiles;
             int k_next = 0, v_next = 0;
             int k_pages = 0, v_pages = 0;       // pages of 32 key (value) tiles, one per lane

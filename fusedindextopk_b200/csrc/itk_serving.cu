@@ -71,13 +71,13 @@ bool strides_ok(std::initializer_list<long long> strides) {
 // Rows of a pool are counted in 31 bits; addresses are formed in 64.
 bool pool_rows_ok(long long pages, long long page_size) { return pages > 0 && page_size > 0 && pages * page_size < (1ll << 31); }
 
-int check_segment(const itk_kv_segment& s, const char* what) {
-    ITK_REQUIRE(s.k && s.v, "%s: keys and values must not be null", what);
-    ITK_REQUIRE(aligned16(s.k) && aligned16(s.v), "%s: keys and values must be 16-byte aligned", what);
+int check_segment(const itk_kv_segment& s, const void* k, const void* v, const int32_t* table, const char* what) {
+    ITK_REQUIRE(k && v, "%s: keys and values must not be null", what);
+    ITK_REQUIRE(aligned16(k) && aligned16(v), "%s: keys and values must be 16-byte aligned", what);
     ITK_REQUIRE(strides_ok({s.k_page_stride, s.k_row_stride, s.k_head_stride, s.v_page_stride, s.v_row_stride, s.v_head_stride}),
                 "%s: strides must be multiples of 8 elements", what);
     ITK_REQUIRE(pool_rows_ok(s.pages, s.page_size), "%s: need 0 < pages * page_size < 2^31", what);
-    if (s.table != nullptr) {
+    if (table != nullptr) {
         ITK_REQUIRE(s.page_size % 128 == 0, "%s: page_size must be a multiple of 128", what);
         ITK_REQUIRE(s.table_pages >= 0 && s.table_stride >= 0, "%s: table sizes must not be negative", what);
     } else {
@@ -279,18 +279,18 @@ int itk_attention(const itk_attention_args* args, itk_stream_t stream) {
     ITK_REQUIRE(a.requests > 0, "need at least one request");
     ITK_REQUIRE(a.q && a.out && a.cu_q, "q, out and cu_q must not be null");
     ITK_REQUIRE((a.cu_k != nullptr) != (a.lens_k != nullptr), "own keys need either cu_k (packed) or lens_k (paged)");
-    ITK_REQUIRE((a.lens_k != nullptr) == (a.own.table != nullptr), "paged own keys need a block table, packed ones have none");
+    ITK_REQUIRE((a.lens_k != nullptr) == (a.table != nullptr), "paged own keys need a block table, packed ones have none");
     ITK_REQUIRE(aligned16(a.q) && aligned16(a.out), "q and out must be 16-byte aligned");
     ITK_REQUIRE(strides_ok({a.q_token_stride, a.q_head_stride, a.out_token_stride, a.out_head_stride}),
                 "strides must be multiples of 8 elements");
     // packed batches may have no own key at all (every key is in the prefix): then there is nothing to point at
-    if (a.own.k == nullptr)
+    if (a.k == nullptr)
         ITK_REQUIRE(a.cu_k != nullptr && a.own.page_size == 0, "own keys: keys and values must not be null");
-    else if ((rc = check_segment(a.own, "own keys")) != ITK_OK)
+    else if ((rc = check_segment(a.own, a.k, a.v, a.table, "own keys")) != ITK_OK)
         return rc;
-    if (a.prefix.k != nullptr) {
-        if ((rc = check_segment(a.prefix, "prefix keys")) != ITK_OK) return rc;
-        const long long room = a.prefix.table != nullptr ? static_cast<long long>(a.prefix.table_pages) * a.prefix.page_size : a.prefix.page_size;
+    if (a.k_prefix != nullptr) {
+        if ((rc = check_segment(a.prefix, a.k_prefix, a.v_prefix, a.prefix_table, "prefix keys")) != ITK_OK) return rc;
+        const long long room = a.prefix_table != nullptr ? static_cast<long long>(a.prefix.table_pages) * a.prefix.page_size : a.prefix.page_size;
         ITK_REQUIRE(a.prefix_keys <= room, "prefix_keys exceeds the prefix");
     } else {
         ITK_REQUIRE(a.prefix_keys == 0, "prefix keys: keys and values must not be null");
@@ -322,17 +322,17 @@ int itk_attention(const itk_attention_args* args, itk_stream_t stream) {
         const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(params.group), static_cast<cuuint32_t>(params.tile_tokens)};
         if ((rc = encode_map(&params.map_q, a.element, 3, a.q, dims, strides, box)) != ITK_OK) return rc;
     }
-    if (a.own.k != nullptr) {
+    if (a.k != nullptr) {
         const itk_kv_segment& s = a.own;
-        if ((rc = segment_map(&params.map_k, a, s, s.k, s.k_page_stride, s.k_row_stride, s.k_head_stride)) != ITK_OK) return rc;
-        if ((rc = segment_map(&params.map_v, a, s, s.v, s.v_page_stride, s.v_row_stride, s.v_head_stride)) != ITK_OK) return rc;
+        if ((rc = segment_map(&params.map_k, a, s, a.k, s.k_page_stride, s.k_row_stride, s.k_head_stride)) != ITK_OK) return rc;
+        if ((rc = segment_map(&params.map_v, a, s, a.v, s.v_page_stride, s.v_row_stride, s.v_head_stride)) != ITK_OK) return rc;
     } else {        // no own key: no item loads through these
         params.map_k = params.map_v = params.map_q;
     }
     if (a.prefix_keys > 0) {
         const itk_kv_segment& s = a.prefix;
-        if ((rc = segment_map(&params.map_k_prefix, a, s, s.k, s.k_page_stride, s.k_row_stride, s.k_head_stride)) != ITK_OK) return rc;
-        if ((rc = segment_map(&params.map_v_prefix, a, s, s.v, s.v_page_stride, s.v_row_stride, s.v_head_stride)) != ITK_OK) return rc;
+        if ((rc = segment_map(&params.map_k_prefix, a, s, a.k_prefix, s.k_page_stride, s.k_row_stride, s.k_head_stride)) != ITK_OK) return rc;
+        if ((rc = segment_map(&params.map_v_prefix, a, s, a.v_prefix, s.v_page_stride, s.v_row_stride, s.v_head_stride)) != ITK_OK) return rc;
     } else {
         params.map_k_prefix = params.map_k;
         params.map_v_prefix = params.map_v;

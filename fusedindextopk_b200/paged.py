@@ -238,7 +238,7 @@ def plan_pages(plan: PagePlan, block_table: Any, lengths: Any, new_tokens: Any, 
     template = plan.templates.get(key)
     if template is None:
         template = _lib.CallTemplate.keep(plan.templates, key, _check_plan(torch, plan, *tensors))
-    block = template.fill((0, [t.data_ptr() for t in tensors]))
+    block = template.fill([t.data_ptr() for t in tensors])
     _lib.launch(torch, _lib.load_library().itk_plan_pages, block, plan.slots.device)
     plan.block_table = block_table
     return plan
@@ -290,9 +290,11 @@ def append_tokens(slots: Any, kv: tuple[Any, Any], pools: tuple[Any, Any], *, in
     if template is None:
         template = _lib.CallTemplate.keep(_APPEND_TEMPLATES, key, _check_append(torch, *tensors))
     addresses = [t.data_ptr() for t in tensors]
-    for name, address in zip(("k", "v", "k_pool", "v_pool", "index_keys", "index_pool"), addresses[1:7]):
-        _require(address % 16 == 0, f"{name} must be 16-byte aligned")
-    _lib.launch(torch, _lib.load_library().itk_append_tokens, template.fill((0, addresses)), template.device)
+    aligned = 0
+    for address in addresses[1:7]:
+        aligned |= address
+    _require(aligned & 15 == 0, "keys, values, index keys and their pools must be 16-byte aligned")
+    _lib.launch(torch, _lib.load_library().itk_append_tokens, template.fill(addresses), template.device)
 
 
 _APPEND_TEMPLATES: dict = {}

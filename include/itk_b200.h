@@ -404,12 +404,9 @@ typedef struct itk_append_args {
 } itk_append_args;
 int itk_append_tokens(const itk_append_args* args, itk_stream_t stream);
 
-/* Keys and values of one segment: packed rows (table = null, one page of `page_size` rows) or a pool of pages
- * read through a table.  Strides in elements. */
+/* Layout of keys and values: packed rows (no table, one page of `page_size` rows) or a pool of pages read through a
+ * table.  Strides in elements. */
 typedef struct itk_kv_segment {
-    const void* k;
-    const void* v;
-    const int32_t* table;      /* int32 [requests, table_pages] (own keys) or [table_pages] (prefix), or null */
     long long table_stride;
     long long k_page_stride, k_row_stride, k_head_stride;
     long long v_page_stride, v_row_stride, v_head_stride;
@@ -429,10 +426,16 @@ typedef struct itk_attention_args {
     const int32_t* lens_k;     /* int32 [requests]: paged own keys */
     void* workspace;
     size_t workspace_bytes;
+    const void* k;             /* own keys and values; null: no request has any */
+    const void* v;
+    const int32_t* table;      /* int32 [requests, table_pages], or null: packed */
+    const void* k_prefix;      /* null: no prefix */
+    const void* v_prefix;
+    const int32_t* prefix_table; /* int32 [table_pages], or null: packed */
     long long q_token_stride, q_head_stride, out_token_stride, out_head_stride;
     unsigned long long wait_limit_ns;   /* 0 = default (2 s); counted in probes, a thousand nanoseconds each at least nominally */
     itk_kv_segment own;
-    itk_kv_segment prefix;     /* k = null: no prefix */
+    itk_kv_segment prefix;
     float scale;
     int element;               /* ITK_ELEMENT_* */
     int tokens, heads, kv_heads, dim, requests, prefix_keys, causal, clear_tail;

@@ -403,7 +403,7 @@ def test_c_entry_refuses_before_any_launch():
     assert library.itk_attention(ctypes.byref(args), None) == -1
     assert b"must not be null" in library.itk_last_error()
     args.q = args.out = args.cu_q = args.lens_k = 1 << 20
-    args.own.k = args.own.v = args.own.table = 1 << 20
+    args.k = args.v = args.table = 1 << 20
     args.own.pages, args.own.page_size = 4, 96
     assert library.itk_attention(ctypes.byref(args), None) == -1
     assert b"multiple of 128" in library.itk_last_error()

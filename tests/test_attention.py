@@ -331,6 +331,91 @@ def test_calls_repeat_to_the_bit(device):
 
 
 @pytest.mark.gpu
+def test_more_requests_than_a_plan_block_has_threads(device):
+    g = torch.Generator().manual_seed(8)
+    k_lens = torch.randint(0, 200, (1500,), generator=g).tolist()
+    q_lens = [min(k, int(n)) for k, n in zip(k_lens, torch.randint(0, 4, (1500,), generator=g))]
+    q, k, v = make(device, q_lens, k_lens, 2, 1, 64, torch.bfloat16, seed=8)
+    got, lse = attention.attention_varlen(q, (k, v), sums(q_lens, device), sums(k_lens, device), return_lse=True)
+    attention.check_status(device)
+    assert_close(got, lse, expected(q, q_lens, split(k, v, k_lens)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("prefix,q_lens,k_lens,heads,kv_heads,dim", [
+    (30000, [3] * 70, [5 + 11 * i for i in range(70)], 32, 4, 128),        # the prefix in many chunks, several waves of items
+    (0, [1] * 30 + [700], [200 * i + 1 for i in range(30)] + [9000], 16, 2, 128),
+    (0, [3000], [3000], 16, 4, 64)])
+def test_batches_of_many_waves(device, prefix, q_lens, k_lens, heads, kv_heads, dim):
+    q, k, v = make(device, q_lens, [prefix] + k_lens, heads, kv_heads, dim, torch.float16, seed=prefix + 1)
+    kp, vp, k, v = k[:prefix], v[:prefix], k[prefix:], v[prefix:]
+    got, lse = attention.shared_prefix_attention(q, (kp, vp), (k, v), sums(q_lens, device), sums(k_lens, device), return_lse=True)
+    attention.check_status(device)
+    assert_close(got, lse, expected(q, q_lens, split(k, v, k_lens, kp if prefix else None, vp if prefix else None)))
+
+
+@pytest.mark.gpu
+def test_rows_of_a_cache_whose_offsets_pass_32_bits(device):
+    """Pools of 2.2 billion elements: the last pages lie beyond 2^32 bytes and 2^31 elements."""
+
+    pages, page, heads, dim = 8400, 256, 8, 128
+    pool = torch.empty((pages, page, heads, dim), dtype=torch.bfloat16, device=device)
+    assert pool.numel() > 1 << 31
+    k_len = 700
+    q, k, v = make(device, [5], [k_len], 16, heads, dim, torch.bfloat16, seed=9)
+    table = torch.tensor([[pages - 1, 0, pages - 2]], dtype=torch.int32, device=device)
+    from fusedindextopk_b200 import paged as pages_module
+
+    position = torch.arange(k_len, device=device)
+    slots = table[0].long()[position // page] * page + position % page
+    values = pool.clone()
+    pages_module.append_tokens(slots, (k, v), (pool, values))
+    lens = torch.tensor([k_len], dtype=torch.int32, device=device)
+    got, lse = attention.attention_paged(q, (pool, values), table, sums([5], device), lens, return_lse=True)
+    attention.check_status(device)
+    assert_close(got, lse, expected(q, [5], [(k, v, None, None)]))
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_at_once(device):
+    shapes = [([1] * 20, [300 * i + 7 for i in range(20)]), ([900, 30], [900, 4000])]
+    made = [make(device, ql, kl, 16, 2, 128, torch.bfloat16, seed=i) for i, (ql, kl) in enumerate(shapes)]
+    ends = [(sums(ql, device), sums(kl, device)) for ql, kl in shapes]
+    streams = [torch.cuda.Stream(device) for _ in shapes]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(attention.attention_varlen(made[i][0], made[i][1:], *ends[i]))
+    torch.cuda.synchronize()
+    attention.check_status(device)
+    for i, (ql, kl) in enumerate(shapes):
+        q, k, v = made[i]
+        assert_close(got[i][0], None, expected(q, ql, split(k, v, kl)))
+        assert all(torch.equal(got[i][0], other) for other in got[i])
+
+
+@pytest.mark.gpu
+def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(device):
+    q, k, v = make(device, [40], [500], 8, 2, 128, torch.bfloat16)
+    cu_q, cu_k = sums([40], device), sums([500], device)
+    out = torch.empty_like(q)
+    template = attention._check_call(torch, q, (k, v), None, 0, cu_q, cu_k, out, True, None)
+    args = _lib.AttentionArgs.from_buffer_copy(template.bytes)
+    args.withhold_loads, args.wait_limit_ns = 1, 1_000_000
+    workspace = torch.empty(template.workspace_bytes, dtype=torch.uint8, device=device)
+    args.q, args.out, args.cu_q, args.cu_k = q.data_ptr(), out.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr()
+    args.k, args.v, args.workspace, args.workspace_bytes = k.data_ptr(), v.data_ptr(), workspace.data_ptr(), workspace.numel()
+    _lib.check(_lib.load_library().itk_attention(ctypes.byref(args), _lib.current_stream(torch, device)))
+    with pytest.raises(_lib.ItkError, match="wait"):
+        attention.check_status(device)
+    got, lse = attention.attention_varlen(q, (k, v), cu_q, cu_k, return_lse=True)
+    attention.check_status(device)
+    assert_close(got, lse, expected(q, [40], [(k, v, None, None)]))
+
+
+@pytest.mark.gpu
 def test_bad_lengths_and_pages_are_clamped_and_reported(device):
     q, k, v = make(device, [4], [300], 4, 2, 128, torch.bfloat16)
     cu = torch.tensor([0, 9], dtype=torch.int32, device=device)             # more rows than q has

@@ -1191,10 +1191,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
                     // The next step's scores, when they are there by now, are loaded into the registers that this
                     // step's exponentials free: the loads, half of the maximum and the hand-over run behind the
                     // second half of those.
-                    const bool early = more && __all_sync(0xffffffffu, mbar_test_wait(next_full, next_phase));
                     uint32_t packed[16];
                     weigh(s[0], packed);
                     tmem_store_16(here, packed);
+                    const bool early = more && __all_sync(0xffffffffu, mbar_test_wait(next_full, next_phase));
                     if (early) {
                         tcgen05_fence_after_sync();
                         tmem_load_32(there, s[0]);

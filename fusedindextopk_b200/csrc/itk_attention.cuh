@@ -351,7 +351,7 @@ constexpr int kAttnMinChunk = 2;    // key tiles of a chunk at least: below that
 // to half a CTA's fair share are not cut then (cutting 592 equal ones, four waves, into halves cost 532 -> 778 us); longer
 // ones are cut into kAttnWaves-ths of the share, which is what the last one taken may run beyond the others, but not
 // below the length at which writing and joining their partial results shows.
-constexpr int kAttnWaves = 6, kAttnWaveChunk = 16;
+constexpr int kAttnWaves = 6, kAttnWaveChunk = 24;
 static_assert(kAttnMinChunk >= 2, "a split item of one tile is its entry's only item: it has one slot and no lane B");
 // Relative cost of a key tile: a pair tile is bound by tensor and exponential work for 256 rows, a split tile by
 // the time its keys take to arrive.

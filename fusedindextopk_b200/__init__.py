@@ -7,7 +7,9 @@ Public surface:
 * ``create_variant(options)`` -> the operator as a plugin with
   ``descriptor / supports / fingerprint_metadata / prepare``;
 * ``make_workspace`` and the ``run_*`` stage functions for callers that manage
-  their own buffers.
+  their own buffers;
+* ``attention`` and ``paged``: the serving step around the operator (attention of
+  packed, paged and shared-prefix batches, page plans, token appends).
 
 Importing the package initialises neither torch nor CUDA; the CUDA library
 (``libitk_b200.so``, built by ``python -m fusedindextopk_b200.build``) is loaded

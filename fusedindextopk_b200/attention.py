@@ -174,7 +174,7 @@ def attention_varlen(q: Any, kv: tuple[Any, Any], cu_seqlens_q: Any, cu_seqlens_
     ``q`` is ``[T, Hq, D]``, ``kv = (k, v)`` both ``[N, H, D]``; request ``b`` owns rows
     ``cu_seqlens_q[b]:cu_seqlens_q[b+1]`` and keys ``cu_seqlens_k[b]:cu_seqlens_k[b+1]`` (int32 ``[B+1]`` each, lengths of
     zero allowed).  With ``causal`` row i of its Q sees its first ``N - Q + i + 1`` keys, else all N.  ``scale`` (positive)
-    defaults to ``D ** -0.5``.  Rows behind the last request are zero (log-sum-exp ``-inf``), or left as they were in a given ``out``.
+    defaults to ``D ** -0.5``.  Rows of no request are zero (log-sum-exp ``-inf``), or left as they were in a given ``out``.
     """
 
     return _attend(q, tuple(kv), None, 0, cu_seqlens_q, cu_seqlens_k, causal, scale, out, return_lse)

@@ -3,7 +3,8 @@
 //     s_j = scale * q . k_j,   m = max_j s_j,   l = sum_j exp(s_j - m),   out = sum_j exp(s_j - m) v_j / l
 //
 // over the prefix keys (all of them) and the request's own keys (the first min(N, N - Q + i + 1) of them for row i
-// of Q when causal).  Scores, statistics and sums are fp32.
+// of Q when causal).  Scores, statistics and sums are fp32; the weights are rounded to the element type once, for the
+// product with the values (half a step of 16 bits each, against the output's own half step), and summed unrounded.
 //
 // Rows.  The G = heads / kv_heads query heads of a key head share its keys, so one 128-row tile holds TT = 128 / G
 // consecutive tokens x G heads (row r = token r / G, head r % G): a single token of a decode step fills G rows of a
@@ -16,15 +17,27 @@
 //              independent softmax states over the same rows, joined like any two partial results.  The tensor work
 //              and the softmax of one lane overlap the other's although there is one row tile only.
 // A plan kernel (one CTA) turns the lengths on the device into a list of items, longest first, cuts long ones into
-// chunks of keys when there are too few to fill the SMs, and lays out the partial results; the attention kernel
-// walks the list; a third kernel joins the partial results.  No length is read by the host.
+// chunks of keys where that spreads the work better, and lays out the partial results; the CTAs of the attention
+// kernel take the items from the list as they get free; a third kernel joins the partial results.  Small calls plan
+// themselves in the attention kernel (attn_small_plan).  No length is read by the host.
 //
-// Attention kernel, one CTA per SM, 12 warps: 0-3 softmax of lane A, 4-7 softmax of lane B (one row per thread),
-// 8 and 9 UMMA issuers of lane A and B, 10 TMA producer, 11 guard.  TMEM: S_A, S_B (128 columns each; the weights P overwrite
-// the first half of S as 16-bit pairs and are the A operand of P V from there), O_A, O_B.  The row maximum is only
-// moved when it grows by more than 2^8 (kLazy): until then weights are at most 2^8 and O needs no rescaling; when it
-// does, the row's own softmax warp rescales O in TMEM, which is safe because S of a tile is complete only after P V
-// of the tile before it.
+// Attention kernel, one CTA per SM, 12 warps: 0-3 softmax of lane A, 4-7 softmax of lane B (one row per thread), 8 and 9
+// UMMA issuers of lane A and B, 10 TMA producer (it also takes the items), 11 guard.  A key tile is worked on in two
+// steps of 64 keys.  TMEM: two buffers of 64 score columns per lane, so that the scores of step i + 1 are computed while
+// the softmax works on step i (the weights P overwrite the first half of their scores as 16-bit pairs and are the A
+// operand of P V from there), and O_A, O_B.  The row maximum is only moved when it grows by more than 2^8 (kAttnLazy):
+// until then weights are at most 2^8 and O needs no rescaling; when it does, the row's own softmax warp rescales O in TMEM
+// after the last P V issued so far.
+//
+// What bounds it (B200, 4736 x 8192 rows, 32 / 8 heads, bf16, no mask).  D = 128: 0.52 ms, 1220 TFLOP/s; the tensor unit is
+// busy 77 % of the time (61 % of it with products: the N = 64 score products read 1.5 times the shared memory that
+// their arithmetic takes time for); without the exponentials it takes 0.50 ms, with an eighth of the products
+// 0.43 ms.  D = 64: 0.43 ms, 735 TFLOP/s, bound by the softmax warps: 16 exponentials a cycle and SM alone take 0.26 ms.
+// Single tokens (split mode): 5.9 TB/s of keys and values, 0.9 of the measured copy rate.
+// Measured and left out (D = 128 / 64, ms): 128-key steps with single score buffers 0.76 / 0.64; UMMAs issued under
+// a lane comparison 1.16 / 0.99 (see elect_one); four softmax warps a scheduler with 96 registers 0.64 / 0.55; the lanes'
+// exponentials in turns 0.70 / 0.61; setmaxnreg (ptxas spills); every register spilled in the softmax loop costs, as
+// shared memory takes all of L1 (76 bytes: 0.55 / 0.50 against 0.53 / 0.46 then).
 //
 // Masked places.  Scores behind a row's last key are replaced, not added to, so keys may hold anything there.  A value
 // row that some row of the item does not see could still reach it as 0 * inf: the guard warp zeroes value rows
@@ -89,6 +102,7 @@ struct AttnCombine {
 struct AttnCounters {
     int items, combines, partial_rows, rows_end;
     int next;                 // the first unit of work (item, key head) that no CTA has taken yet
+    int rows_begin;           // rows of the first request; rows_end: behind the last one
 };
 
 struct AttnWorkspace {
@@ -450,8 +464,21 @@ __device__ __forceinline__ int attn_share(const AttnParams& p, unsigned long lon
     return static_cast<int>(fminf(ceilf(static_cast<float>(cost) * p.a.kv_heads * p.inverse_sms) + 1.0f, 536870912.0f));
 }
 
+// Sum of the values of the lanes before this one; `total`: of all lanes.
+__device__ __forceinline__ int warp_prefix(int value, int lane, int& total) {
+    int upto = value;
+#pragma unroll
+    for (int step = 1; step < 32; step <<= 1) {
+        const int other = __shfl_up_sync(0xffffffffu, upto, step);
+        if (lane >= step) upto += other;
+    }
+    total = __shfl_sync(0xffffffffu, upto, 31);
+    return upto - value;
+}
+
 // Most of a small call's time before its first key is read goes by in here: one pass over the lengths, entries kept in
-// registers, five block barriers when the items fit one wave (their order does not matter then).
+// registers, six block barriers when the items fit one wave (their order does not matter then), no 64-bit division
+// (those took half of 7.8 us for one request).
 template <int THREADS>
 __global__ void __launch_bounds__(THREADS) itk_attention_plan_kernel(const __grid_constant__ AttnParams p) {
     __shared__ int warp_sums[THREADS / 32];
@@ -487,19 +514,15 @@ __global__ void __launch_bounds__(THREADS) itk_attention_plan_kernel(const __gri
             if (is_cached) cache[b] = request;
             mine = (request.q_count + span - 1) / span;
         }
-        int upto = mine;
-#pragma unroll
-        for (int step = 1; step < 32; step <<= 1) {
-            const int other = __shfl_up_sync(0xffffffffu, upto, step);
-            if (lane >= step) upto += other;
-        }
-        if (lane == 31) warp_sums[warp] = upto;
+        int total;
+        const int in_warp = warp_prefix(mine, lane, total);
+        if (lane == 31) warp_sums[warp] = total;
         __syncthreads();
         int before = carry;
         for (int w = 0; w < warp; ++w) before += warp_sums[w];
-        if (b < p.a.requests) entry_first[b] = before + upto - mine;
+        if (b < p.a.requests) entry_first[b] = before + in_warp;
         __syncthreads();
-        if (tx == THREADS - 1) carry = before + upto;
+        if (tx == THREADS - 1) carry = before + total;
     }
     if (bad) atomicOr(p.status, ITK_SERVING_BAD_LENGTHS);
     __syncthreads();
@@ -573,13 +596,8 @@ __global__ void __launch_bounds__(THREADS) itk_attention_plan_kernel(const __gri
                 held[i] = bins[lane * (kAttnBins / 32) + i];
                 sum += held[i];
             }
-            int upto = sum;
-#pragma unroll
-            for (int step = 1; step < 32; step <<= 1) {
-                const int other = __shfl_up_sync(0xffffffffu, upto, step);
-                if (lane >= step) upto += other;
-            }
-            int before = upto - sum;
+            int total;
+            int before = warp_prefix(sum, lane, total);
 #pragma unroll
             for (int i = 0; i < kAttnBins / 32; ++i) {
                 bins[lane * (kAttnBins / 32) + i] = before;
@@ -618,7 +636,8 @@ __global__ void __launch_bounds__(THREADS) itk_attention_plan_kernel(const __gri
             if (place + c < p.w.max_items) p.w.items[place + c] = attn_chunk(entry, c, count);
     }
     __syncthreads();
-    if (tx == 0) *p.w.counters = AttnCounters{min(item_count, p.w.max_items), min(combine_count, p.w.max_combines), partial_rows, rows_end, p.sm_count};
+    if (tx == 0) *p.w.counters = AttnCounters{min(item_count, p.w.max_items), min(combine_count, p.w.max_combines), partial_rows, rows_end, p.sm_count,
+                                               min(max(p.a.cu_q[0], 0), p.a.tokens)};
 }
 
 // The plan of a call with at most 32 requests and 32 entries that fit one wave of CTAs uncut: every CTA's producer warp
@@ -626,17 +645,6 @@ __global__ void __launch_bounds__(THREADS) itk_attention_plan_kernel(const __gri
 // That saves the plan's launch and the wait for it.  CTA 0 also writes down what the join needs.  `cache` and `first` are
 // scratch for the requests.  Returns whether there is a unit.
 constexpr int kAttnSmallEntries = 32;
-
-__device__ __forceinline__ int warp_prefix(int value, int lane, int& total) {
-    int upto = value;
-#pragma unroll
-    for (int step = 1; step < 32; step <<= 1) {
-        const int other = __shfl_up_sync(0xffffffffu, upto, step);
-        if (lane >= step) upto += other;
-    }
-    total = __shfl_sync(0xffffffffu, upto, 31);
-    return upto - value;
-}
 
 __device__ __forceinline__ bool attn_small_plan(const AttnParams& p, AttnRequest* cache, int* first, int4* unit, int lane) {
     const int span = 2 * p.tile_tokens, kv_heads = p.a.kv_heads;
@@ -690,7 +698,7 @@ __device__ __forceinline__ bool attn_small_plan(const AttnParams& p, AttnRequest
         for (int r = 0; r < wanted; ++r)
             if (at + r < p.w.max_combines)
                 p.w.combines[at + r] = AttnCombine{entry.item.q_first, entry.item.tokens, entry.item.partial, usable, r * kAttnCombineRows, {}};
-        if (lane == 0) *p.w.counters = AttnCounters{items, min(records, p.w.max_combines), partial, rows_end, 0};
+        if (lane == 0) *p.w.counters = AttnCounters{items, min(records, p.w.max_combines), partial, rows_end, 0, min(max(p.a.cu_q[0], 0), p.a.tokens)};
     }
     __syncwarp();
     return __any_sync(0xffffffffu, found) != 0;
@@ -1465,9 +1473,13 @@ __global__ void __launch_bounds__(kJoinThreads) itk_attention_join_kernel(const 
         }
     }
     if (p.a.clear_tail) {
-        const long long begin = static_cast<long long>(counters.rows_end) * p.a.heads, end = static_cast<long long>(p.a.tokens) * p.a.heads;
-        for (long long r = begin + static_cast<long long>(blockIdx.x) * (kJoinThreads / 32) + warp; r < end;
-             r += static_cast<long long>(gridDim.x) * (kJoinThreads / 32)) {
+        // rows in front of the first request and behind the last one
+        const long long head_rows = static_cast<long long>(counters.rows_begin) * p.a.heads;
+        const long long tail = static_cast<long long>(max(counters.rows_end, counters.rows_begin)) * p.a.heads;
+        const long long all = head_rows + static_cast<long long>(p.a.tokens) * p.a.heads - tail;
+        for (long long i = static_cast<long long>(blockIdx.x) * (kJoinThreads / 32) + warp; i < all;
+             i += static_cast<long long>(gridDim.x) * (kJoinThreads / 32)) {
+            const long long r = i < head_rows ? i : tail + i - head_rows;
             const long long token = r / p.a.heads, head = r - token * p.a.heads;
             T* out = static_cast<T*>(p.a.out) + token * p.a.out_token_stride + head * p.a.out_head_stride + lane * kOwn;
             if constexpr (kOwn == 4) {

@@ -241,6 +241,13 @@ def test_rows_behind_the_last_request(device, q_len, k_len):
     attention.attention_varlen(q, (k, v), cu_q, cu_k, out=out)
     assert_close(out, None, want)
     assert bool((out[q_len:] == 5.0).all()), "rows behind the last request were written"
+    # and rows in front of the first one
+    for given in (None, torch.full_like(q, 5.0)):
+        shifted = attention.attention_varlen(torch.cat([q[q_len:q_len + 30], q[:q_len], q[q_len:q_len + 7]]), (k, v), cu_q + 30, cu_k,
+                                             out=None if given is None else given[:q_len + 37])
+        assert_close(shifted[30:], None, want)
+        rest = torch.cat([shifted[:30], shifted[30 + q_len:]])
+        assert bool((rest == (0.0 if given is None else 5.0)).all())
     attention.check_status(device)
 
 

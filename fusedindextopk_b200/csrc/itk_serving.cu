@@ -96,6 +96,15 @@ int check_attention(const itk_attention_args& a) {
     return ITK_OK;
 }
 
+// Tokens of a row tile.  As many as fit; a batch of single tokens takes one, so that the other requests' queries are not
+// loaded, and multiplied, beside it: the power cap is what holds such a batch back when steps follow each other (64 tokens over 65 to
+// 32768 keys: 370 -> 347 us in a long run, 321 -> 313 cool; whole boxes are no quicker anywhere, but longer requests need them).  No more
+// tokens than requests is the sign of one; a batch that only looks like it gets shorter entries and the same results.  (The
+// prefix pass shares its entries between requests and takes all that fit.)
+int attention_tile_tokens(const itk_attention_args& a) {
+    return a.tokens <= a.requests && a.prefix_keys == 0 ? 1 : kAttnTile / (a.heads / a.kv_heads);
+}
+
 constexpr int kAttnMaxSms = 160;     // the workspace is sized for any device the library runs on
 
 // Workspace of a call: what the plan kernel can write at most.  With T tokens, B requests and 2 TT tokens per entry
@@ -105,7 +114,7 @@ constexpr int kAttnMaxSms = 160;     // the workspace is sized for any device th
 // no row has more of them than there are chunks for one key head; with a prefix every own row and every prefix row has one
 // more, two in split entries.
 int attention_workspace(const itk_attention_args& a, AttnWorkspace* w, size_t* bytes) {
-    const long long tile_tokens = kAttnTile / (a.heads / a.kv_heads), span = 2 * tile_tokens;
+    const long long span = 2 * attention_tile_tokens(a);
     const long long rows = static_cast<long long>(a.tokens) * a.heads;
     const long long own = a.tokens / span + a.requests, prefix = a.prefix_keys > 0 ? a.tokens / span + 1 : 0;
     const long long added = static_cast<long long>(kAttnMaxSms) * kAttnWaves;
@@ -306,7 +315,7 @@ int itk_attention(const itk_attention_args* args, itk_stream_t stream) {
     params.a = a;
     params.status = device.status;
     params.group = a.heads / a.kv_heads;
-    params.tile_tokens = kAttnTile / params.group;
+    params.tile_tokens = attention_tile_tokens(a);
     params.sm_count = std::min(device.sm_count, kAttnMaxSms);
     params.withhold_loads = a.withhold_loads;
     const long long entries = params.w.max_entries + (a.prefix_keys > 0 ? a.tokens / (2 * params.tile_tokens) + 1 : 0);

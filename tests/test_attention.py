@@ -349,6 +349,18 @@ def test_more_requests_than_a_plan_block_has_threads(device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("q_lens,k_lens,heads,kv_heads,dim", [
+    ([1] * 40, [257 + 31 * i for i in range(40)], 16, 2, 128), ([0] * 90 + [60, 1, 29] + [0] * 7, [300] * 90 + [700, 5, 29] + [9] * 7, 14, 2, 64),
+    ([2, 0, 1, 0, 3, 0] * 7, [900, 0, 1, 4, 130, 128] * 7, 7, 1, 128), ([100] + [0] * 100, [6000] + [70] * 100, 32, 4, 128)])
+def test_batches_with_no_more_tokens_than_requests(device, q_lens, k_lens, heads, kv_heads, dim):
+    q, k, v = make(device, q_lens, k_lens, heads, kv_heads, dim, torch.bfloat16)
+    for causal in (True, False):
+        got, lse = attention.attention_varlen(q, (k, v), sums(q_lens, device), sums(k_lens, device), causal=causal, return_lse=True)
+        assert_close(got, lse, expected(q, q_lens, split(k, v, k_lens), causal))
+    attention.check_status(device)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("prefix,q_lens,k_lens,heads,kv_heads,dim", [
     (30000, [3] * 70, [5 + 11 * i for i in range(70)], 32, 4, 128),        # the prefix in many chunks, several waves of items
     (0, [1] * 30 + [700], [200 * i + 1 for i in range(30)] + [9000], 16, 2, 128),

@@ -52,6 +52,7 @@ def _check_kv(q: Any, k: Any, v: Any, what: str, rank: int) -> None:
              f"the query heads must be a multiple of the {what} key heads, at most 128 times as many")
     _require(k.numel() == 0 or (_rows_ok(k) and _rows_ok(v)),
              f"{what} keys and values must be contiguous in their last dimension and 16-byte aligned in every row")
+    _require(rank == 4 or k.shape[0] < 1 << 31, f"need less than 2^31 {what} keys")
     if rank == 4:
         pages, page_size = k.shape[:2]
         _require(pages > 0 and page_size > 0 and page_size % TILE_KEYS == 0, "page_size must be a positive multiple of 128")
@@ -140,6 +141,11 @@ def _attend(q: Any, own: tuple, prefix: tuple | None, prefix_keys: int, cu_seqle
         tensors += (out,)
     if scale is not None:
         scale = float(scale)
+    if torch.is_grad_enabled():
+        learns = q.requires_grad or own[0].requires_grad or own[1].requires_grad
+        if prefix is not None:
+            learns = learns or prefix[0].requires_grad or prefix[1].requires_grad
+        _require(not learns, "there is no backward pass: call it under torch.no_grad() or detach")
     key = (_lib.metadata(tensors), len(own), prefix is not None, prefix_keys, bool(causal), scale)
     template = _TEMPLATES.get(key)
     if template is None:
@@ -175,6 +181,7 @@ def attention_varlen(q: Any, kv: tuple[Any, Any], cu_seqlens_q: Any, cu_seqlens_
     ``cu_seqlens_q[b]:cu_seqlens_q[b+1]`` and keys ``cu_seqlens_k[b]:cu_seqlens_k[b+1]`` (int32 ``[B+1]`` each, lengths of
     zero allowed).  With ``causal`` row i of its Q sees its first ``N - Q + i + 1`` keys, else all N.  ``scale`` (positive)
     defaults to ``D ** -0.5``.  Rows of no request are zero (log-sum-exp ``-inf``), or left as they were in a given ``out``.
+    ``out`` may be ``q`` itself and shares no other memory with the inputs.
     """
 
     return _attend(q, tuple(kv), None, 0, cu_seqlens_q, cu_seqlens_k, causal, scale, out, return_lse)

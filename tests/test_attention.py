@@ -227,6 +227,19 @@ def test_slices_of_one_projection_and_a_strided_output(device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("prefix,q_lens,k_lens,heads,kv_heads,dim", [
+    (0, [1] * 20, [300 * i + 1 for i in range(20)], 16, 2, 128), (0, [5, 300, 2, 90], [5, 900, 3000, 90], 8, 4, 64),
+    (700, [3] * 12, [9 * i + 3 for i in range(12)], 14, 2, 128)])
+def test_an_output_in_the_place_of_the_queries(device, prefix, q_lens, k_lens, heads, kv_heads, dim):
+    q, k, v = make(device, q_lens, [prefix] + k_lens, heads, kv_heads, dim, torch.bfloat16)
+    kp, vp, k, v = k[:prefix], v[:prefix], k[prefix:], v[prefix:]
+    want = expected(q, q_lens, split(k, v, k_lens, kp if prefix else None, vp if prefix else None))
+    attention.shared_prefix_attention(q, (kp, vp), (k, v), sums(q_lens, device), sums(k_lens, device), out=q)
+    attention.check_status(device)
+    assert_close(q, None, want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("q_len,k_len", [(1, 70), (40, 200), (300, 300)])
 def test_rows_behind_the_last_request(device, q_len, k_len):
     q, k, v = make(device, [q_len + 37], [k_len + 50], 8, 2, 128, torch.bfloat16)
@@ -477,6 +490,12 @@ def test_refusals(device):
     refused("out must", q, (k, v), cu_q, cu_k, out=torch.empty(4, 4, 64, dtype=q.dtype, device=device))
     refused("overlap", q, (k, v), cu_q, cu_k, out=torch.empty(4, 4, 128, dtype=q.dtype, device=device)[:1].expand(4, 4, 128))
     refused("finite", q, (k, v), cu_q, cu_k, scale=float("inf"))
+    refused("less than 2\\^31 own keys", q, (k[:1].expand(1 << 32, 2, 128), v[:1].expand(1 << 32, 2, 128)), cu_q, cu_k)
+    refused("no backward", q.clone().requires_grad_(), (k, v), cu_q, cu_k)
+    refused("no backward", q, (k, v.clone().requires_grad_()), cu_q, cu_k)
+    refused("no backward", q, (k.clone().requires_grad_(), v), (k, v), cu_q, cu_k, call=attention.shared_prefix_attention)
+    with torch.no_grad():
+        attention.attention_varlen(q.clone().requires_grad_(), (k, v), cu_q, cu_k)
     pools, table = paged(k, v, [30], 128, seed=1)
     lens = torch.tensor([30], dtype=torch.int32, device=device)
     refused("multiple of 128", q, tuple(p[:, :64] for p in pools), table, cu_q, lens, call=attention.attention_paged)

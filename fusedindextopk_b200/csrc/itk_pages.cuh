@@ -116,11 +116,13 @@ __global__ void __launch_bounds__(kPlanThreads) itk_plan_pages_kernel(const itk_
         atomicOr(status, (clamped ? ITK_SERVING_BAD_LENGTHS : 0) | (no_room ? ITK_SERVING_OUT_OF_PAGES : 0));
     __syncthreads();
 
-    const int stride = gridDim.x * kPlanThreads;
-    const int start = blockIdx.x * kPlanThreads + threadIdx.x;
-    const int cells = p.requests * p.table_pages;
-    for (int cell = start; cell < cells; cell += stride) {
-        const int b = cell / p.table_pages, column = cell - b * p.table_pages;
+    // counted unsigned: up to 2^31 - 1 cells or rows, and a step behind the last
+    const unsigned stride = gridDim.x * kPlanThreads;
+    const unsigned start = blockIdx.x * kPlanThreads + threadIdx.x;
+    const unsigned cells = static_cast<unsigned>(p.requests) * static_cast<unsigned>(p.table_pages);
+    for (unsigned cell = start; cell < cells; cell += stride) {
+        const int b = static_cast<int>(cell / static_cast<unsigned>(p.table_pages));
+        const int column = static_cast<int>(cell) - b * p.table_pages;
         const PlanRequest r = plan_request(p, b);
         int32_t* entry = p.table + b * p.table_stride + column;
         int page = -1;
@@ -133,10 +135,11 @@ __global__ void __launch_bounds__(kPlanThreads) itk_plan_pages_kernel(const itk_
         }
         if (column < r.after) p.flat[first[b] + column] = page;
     }
-    for (int entry = total_pages + start; entry < cells; entry += stride) p.flat[entry] = 0;
+    for (unsigned entry = total_pages + start; entry < cells; entry += stride) p.flat[entry] = 0;
 
     const int last = cu[p.requests];
-    for (int row = start; row < p.rows; row += stride) {
+    for (unsigned at = start; at < static_cast<unsigned>(p.rows); at += stride) {
+        const int row = static_cast<int>(at);
         long long slot = -1;
         int k_start = 0, k_end = 0;
         if (row < last) {
@@ -200,9 +203,9 @@ __device__ __forceinline__ void load_index_quad<__nv_bfloat16>(const __nv_bfloat
 // flight per lane, and the index key (128 elements, four per lane) is quantised from registers.  Bound by HBM.
 template <typename Source>
 __global__ void __launch_bounds__(kAppendThreads) itk_append_tokens_kernel(const itk_append_args p, int* status) {
-    const int token = (blockIdx.x * kAppendThreads + threadIdx.x) >> 5;
+    const unsigned token = blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
-    if (token >= p.tokens) return;
+    if (token >= static_cast<unsigned>(p.tokens)) return;
     const long long slot = p.slots[token];
     if (slot < 0) return;
     if (slot >= static_cast<long long>(p.pages) * p.page_size) {

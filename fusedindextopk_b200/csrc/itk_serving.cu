@@ -68,6 +68,16 @@ bool strides_ok(std::initializer_list<long long> strides) {
     return true;
 }
 
+struct Bytes {
+    const void* first;
+    size_t count;
+};
+
+bool overlap(const Bytes& x, const Bytes& y) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(x.first), b = reinterpret_cast<uintptr_t>(y.first);
+    return x.count > 0 && y.count > 0 && a < b + y.count && b < a + x.count;
+}
+
 // Rows of a pool are counted in 31 bits; addresses are formed in 64.
 bool pool_rows_ok(long long pages, long long page_size) { return pages > 0 && page_size > 0 && pages * page_size < (1ll << 31); }
 
@@ -229,6 +239,23 @@ int itk_plan_pages(const itk_page_plan_args* args, itk_stream_t stream) {
     ITK_REQUIRE(a.table && a.old && a.fresh && a.cu_q && a.lengths && a.flat && a.pages_needed &&
                     (a.free_pages || a.free_count == 0) && ((a.slots && a.k_start && a.k_end) || a.rows == 0),
                 "page plan pointers must not be null");
+    // Every CTA reads the lengths and the free list for itself while others write: a plan's lengths, for one, cannot be the
+    // next plan's old lengths in the same buffers.
+    {
+        const size_t word = sizeof(int32_t), requests = a.requests, rows = a.rows;
+        const Bytes reads[] = {{a.old, requests * word}, {a.fresh, requests * word}, {a.free_pages, a.free_count * word}};
+        const Bytes writes[] = {{a.table, ((requests - 1) * a.table_stride + a.table_pages) * word},
+                                {a.slots, rows * sizeof(long long)},
+                                {a.cu_q, (requests + 1) * word},
+                                {a.lengths, requests * word},
+                                {a.flat, requests * a.table_pages * word},
+                                {a.k_start, rows * word},
+                                {a.k_end, rows * word},
+                                {a.pages_needed, word}};
+        for (const Bytes& written : writes)
+            for (const Bytes& read : reads)
+                ITK_REQUIRE(!overlap(written, read), "the request lengths and the free list must not share memory with the table or the plan");
+    }
     DeviceState device;
     const int rc = current_device(&device);
     if (rc != ITK_OK) return rc;

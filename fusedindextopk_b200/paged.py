@@ -206,7 +206,7 @@ def make_page_plan(requests: int, table_pages: int, rows: int, *, page_size: int
     import torch
 
     _require(0 < requests <= _lib.MAX_PLAN_REQUESTS, f"need 0 < requests <= {_lib.MAX_PLAN_REQUESTS}")
-    _require(table_pages > 0 and rows >= 0, "need table_pages > 0 and rows >= 0")
+    _require(table_pages > 0 and 0 <= rows < 1 << 31, "need table_pages > 0 and 0 <= rows < 2^31")
     _require(page_size >= TILE_KEYS and page_size % TILE_KEYS == 0, "page_size must be a positive multiple of 128")
     _require(requests * table_pages * page_size < 1 << 31, "requests * table_pages * page_size must stay below 2^31")
     device = torch.device(device)
@@ -225,7 +225,9 @@ def plan_pages(plan: PagePlan, block_table: Any, lengths: Any, new_tokens: Any, 
     Request ``b`` holds ``lengths[b]`` tokens (int32 ``[B]``) on the first ``ceil(lengths[b] / page_size)`` pages of its
     row of ``block_table`` (int32 ``[B, table_pages]``) and gets ``new_tokens[b]`` more; the pages it lacks are taken from
     ``free_pages`` (int32 ``[F]``) in request order, the first ``pages_needed[0]`` of them.  Everything lands in the
-    plan's buffers and in ``block_table`` itself; calling it again with the same arguments gives the same result.
+    plan's buffers and in ``block_table`` itself; calling it again with the same arguments gives the same result.  The
+    inputs must not share memory with those: ``plan.lengths`` serves as another plan's ``lengths`` (two plans in turn), not
+    as its own's.
 
     A request that outgrows its table row, a free list that is too short and more new tokens than ``rows`` are reported
     by ``check_serving_status``; their tokens get slot -1 (or no row), their cells -1, and nothing is written out of range.
@@ -307,7 +309,7 @@ def _check_append(torch: Any, slots: Any, k: Any, v: Any, k_pool: Any, v_pool: A
     _require(k.dim() == 3 and k.shape == v.shape, "k and v must both have shape [T, H, D]")
     tokens, heads, dim = k.shape
     _require(dim in (64, 128), "the head dimension must be 64 or 128")
-    _require(heads > 0, "need at least one head")
+    _require(heads > 0 and tokens < 1 << 31, "need at least one head and less than 2^31 tokens")
     _require(k.dtype in (torch.bfloat16, torch.float16), "k and v must be bfloat16 or float16")
     _require(k_pool.dim() == 4 and k_pool.shape == v_pool.shape and tuple(k_pool.shape[2:]) == (heads, dim),
              "the pools must both have shape [P, page_size, H, D]")

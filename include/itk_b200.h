@@ -361,7 +361,8 @@ int itk_serving_status(int* status, int clear);
  *   row r of request b at position pos: slots[r] = table[b, pos / page_size] * page_size + pos % page_size;
  *   flat = the used table entries of all requests one after another (0 behind them), and in that key space
  *   k_start[r] = page_size * pages of the requests before b, k_end[r] = k_start[r] + pos + 1.
- * Rows behind the last request: slot -1 and an empty range.  pages_needed[0] = pages taken from the free list. */
+ * Rows behind the last request: slot -1 and an empty range.  pages_needed[0] = pages taken from the free list.
+ * old, fresh and free_pages must not share memory with what is written (lengths of an earlier plan: use two plans in turn). */
 typedef struct itk_page_plan_args {
     int32_t* table;            /* int32 [requests, table_pages], row stride table_stride; updated in place */
     const int32_t* old;        /* int32 [requests] */

@@ -203,6 +203,30 @@ def test_slots_behind_the_pool_are_skipped_and_reported(device):
 
 
 @pytest.mark.gpu
+def test_more_tokens_than_a_32_bit_thread_number_counts(device):
+    tokens = (1 << 27) + 5
+    k = torch.randn((1, 1, 64), dtype=torch.bfloat16, device=device)
+    pools = [torch.zeros((1, 128, 1, 64), dtype=torch.bfloat16, device=device) for _ in range(2)]
+    slots = torch.full((tokens,), -1, dtype=torch.int64, device=device)
+    slots[-1], slots[1 << 20] = 7, 9
+    paged.append_tokens(slots, (k.expand(tokens, 1, 64), k.expand(tokens, 1, 64)), tuple(pools))
+    for pool in pools:
+        assert torch.equal(pool[0, 7], k[0]) and torch.equal(pool[0, 9], k[0]) and int((pool != 0).any(-1).sum()) == 2
+
+
+@pytest.mark.gpu
+def test_two_plans_take_turns_and_one_does_not_read_itself(device):
+    plans = [paged.make_page_plan(3, 4, 8, page_size=128, device=device) for _ in range(2)]
+    table = torch.full((3, 4), -1, dtype=torch.int32, device=device)
+    free, new = gpu(list(range(12)), device), gpu([1, 0, 2], device)
+    paged.plan_pages(plans[0], table, gpu([127, 0, 255], device), new, free)
+    paged.plan_pages(plans[1], table, plans[0].lengths, new, free[6:])
+    assert plans[1].lengths.tolist() == [129, 0, 259]
+    with pytest.raises(_lib.ItkError, match="share memory"):
+        paged.plan_pages(plans[1], table, plans[1].lengths, new, free)
+
+
+@pytest.mark.gpu
 def test_append_refusals(device):
     k = torch.ones((3, 2, 64), dtype=torch.bfloat16, device=device)
     pool = torch.zeros((2, 128, 2, 64), dtype=torch.bfloat16, device=device)
@@ -228,7 +252,7 @@ def test_append_refusals(device):
 
 
 def test_page_plan_sizes_are_refused_without_a_gpu():
-    for kwargs in (dict(requests=0), dict(requests=20000), dict(table_pages=0), dict(page_size=100), dict(rows=-1),
+    for kwargs in (dict(requests=0), dict(requests=20000), dict(table_pages=0), dict(page_size=100), dict(rows=-1), dict(rows=1 << 31),
                    dict(requests=16384, table_pages=1024), dict(device="cpu")):
         size = dict(requests=4, table_pages=4, rows=4, page_size=128, device="cuda") | kwargs
         with pytest.raises(ValueError):
@@ -247,6 +271,16 @@ def test_c_entries_refuse_before_any_launch():
     plan.requests = 4
     assert library.itk_plan_pages(ctypes.byref(plan), None) == -1
     assert b"must not be null" in library.itk_last_error()
+    apart = {name: (i + 1) << 20 for i, name in enumerate(
+        ("table", "old", "fresh", "free_pages", "slots", "cu_q", "lengths", "flat", "k_start", "k_end", "pages_needed"))}
+    plan.free_count, plan.rows = 5, 10
+    for read in ("old", "fresh", "free_pages"):
+        for written in ("table", "slots", "cu_q", "lengths", "flat", "k_start", "k_end", "pages_needed"):
+            for name, address in apart.items():
+                setattr(plan, name, address)
+            setattr(plan, read, apart[written] - 12)                # its last words on the other's first
+            assert library.itk_plan_pages(ctypes.byref(plan), None) == -1
+            assert b"share memory" in library.itk_last_error()
     assert library.itk_append_tokens(None, None) == -1
     assert library.itk_append_tokens(ctypes.byref(append), None) == -1
     append.tokens, append.kv_heads, append.dim, append.pages, append.page_size = 3, 2, 128, 2, 128

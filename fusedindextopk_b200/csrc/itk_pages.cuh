@@ -60,12 +60,84 @@ __device__ __forceinline__ PlanRequest plan_request(const itk_page_plan_args& p,
     return r;
 }
 
+// What every CTA knows of the requests: rows, free pages and flat entries before each.
+struct PlanState {
+    const int *cu, *taken, *first;
+};
+
+// Slots and key ranges, kRows neighbouring rows at a time.
+template <int kRows>
+__device__ __forceinline__ void plan_rows(const itk_page_plan_args& p, const PlanState& state, unsigned start, unsigned stride) {
+    const int last = state.cu[p.requests];
+    const unsigned units = (static_cast<unsigned>(p.rows) + kRows - 1) / kRows;
+    for (unsigned unit = start; unit < units; unit += stride) {
+        long long slots[kRows];
+        int starts[kRows], ends[kRows];
+        const unsigned base = unit * kRows;
+        PlanRequest r{};
+        int b = 0;
+        unsigned until = base;                  // rows below it are of request b
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            const unsigned row = base + i;
+            slots[i] = -1;
+            starts[i] = ends[i] = 0;
+            if (row >= static_cast<unsigned>(last)) continue;
+            if (row >= until) {
+                int low = b, high = p.requests;     // cu[low] <= row < cu[high]
+                while (high - low > 1) {
+                    const int middle = (low + high) >> 1;
+                    if (static_cast<unsigned>(state.cu[middle]) <= row) {
+                        low = middle;
+                    } else {
+                        high = middle;
+                    }
+                }
+                b = low;
+                until = state.cu[b + 1];
+                r = plan_request(p, b);
+            }
+            const long long position = static_cast<long long>(r.old) + row - state.cu[b];
+            starts[i] = state.first[b] * p.page_size;
+            ends[i] = starts[i] + static_cast<int>(min(position + 1, static_cast<long long>(r.length)));
+            if (position < r.length) {
+                const int column = static_cast<int>(position) / p.page_size;
+                int page = -1;
+                if (column < r.before) {
+                    page = p.table[b * p.table_stride + column];
+                } else {
+                    const int next = state.taken[b] + column - r.before;
+                    if (next < p.free_count) page = p.free_pages[next];
+                }
+                if (page >= 0) slots[i] = static_cast<long long>(page) * p.page_size + position % p.page_size;
+            }
+        }
+        if constexpr (kRows == 4) {
+            if (base + 4 <= static_cast<unsigned>(p.rows)) {
+                *reinterpret_cast<longlong2*>(p.slots + base) = make_longlong2(slots[0], slots[1]);
+                *reinterpret_cast<longlong2*>(p.slots + base + 2) = make_longlong2(slots[2], slots[3]);
+                *reinterpret_cast<int4*>(p.k_start + base) = make_int4(starts[0], starts[1], starts[2], starts[3]);
+                *reinterpret_cast<int4*>(p.k_end + base) = make_int4(ends[0], ends[1], ends[2], ends[3]);
+                continue;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+            if (base + i < static_cast<unsigned>(p.rows)) {
+                p.slots[base + i] = slots[i];
+                p.k_start[base + i] = starts[i];
+                p.k_end[base + i] = ends[i];
+            }
+    }
+}
+
 // One launch.  Every CTA scans all requests itself (a few KB that sit in L2) and keeps the prefix sums in shared
 // memory, so that table cells and rows can be filled by all CTAs with no second launch and no hand-off: the page of
 // a position is either an old cell of the table, which no CTA writes, or free_pages[taken before + ...], which is
-// computed, not read back.  Bound by latency for the batches of a decode step (one launch), by the writes for
-// large ones (16 B per row, 8 B per table cell).
-__global__ void __launch_bounds__(kPlanThreads) itk_plan_pages_kernel(const itk_page_plan_args p, int* status) {
+// computed, not read back.  Bound by latency for the batches of a decode step (8 requests: 4.3 us, of which the launch is
+// 2.2), by the chain search - lengths - page - store for large ones (1024 requests, 300000 rows: 9.4 us for 8 MB; the
+// writes alone, 16 B per row and 8 B per table cell, would take 1.2).
+__global__ void __launch_bounds__(kPlanThreads) itk_plan_pages_kernel(const itk_page_plan_args p, int wide, int* status) {
     extern __shared__ int plan_smem[];
     int* cu = plan_smem;                        // [B + 1] rows before request b, clamped to the row buffer
     int* taken = plan_smem + p.requests + 1;    // [B] free pages handed out before request b
@@ -137,41 +209,14 @@ __global__ void __launch_bounds__(kPlanThreads) itk_plan_pages_kernel(const itk_
     }
     for (unsigned entry = total_pages + start; entry < cells; entry += stride) p.flat[entry] = 0;
 
-    const int last = cu[p.requests];
-    for (unsigned at = start; at < static_cast<unsigned>(p.rows); at += stride) {
-        const int row = static_cast<int>(at);
-        long long slot = -1;
-        int k_start = 0, k_end = 0;
-        if (row < last) {
-            int low = 0, high = p.requests;     // cu[low] <= row < cu[high]
-            while (high - low > 1) {
-                const int middle = (low + high) >> 1;
-                if (cu[middle] <= row) {
-                    low = middle;
-                } else {
-                    high = middle;
-                }
-            }
-            const PlanRequest r = plan_request(p, low);
-            const long long position = static_cast<long long>(r.old) + row - cu[low];
-            k_start = first[low] * p.page_size;
-            k_end = k_start + static_cast<int>(min(position + 1, static_cast<long long>(r.length)));
-            if (position < r.length) {
-                const int column = static_cast<int>(position) / p.page_size;
-                int page = -1;
-                if (column < r.before) {
-                    page = p.table[low * p.table_stride + column];
-                } else {
-                    const int next = taken[low] + column - r.before;
-                    if (next < p.free_count) page = p.free_pages[next];
-                }
-                if (page >= 0) slot = static_cast<long long>(page) * p.page_size + position % p.page_size;
-            }
-        }
-        p.slots[row] = slot;
-        p.k_start[row] = k_start;
-        p.k_end[row] = k_end;
-    }
+    // Four neighbouring rows a thread when one each is not enough: most are of one request, so that it is looked for once, and
+    // their stores are wide (300000 rows of 1024 requests: 10.4 -> 9.4 us).  One each otherwise: four take longer than one
+    // (8 requests: 4.3 us, 6.3 with four).
+    const PlanState state{cu, taken, first};
+    if (wide && static_cast<unsigned>(p.rows) > stride)
+        plan_rows<4>(p, state, start, stride);
+    else
+        plan_rows<1>(p, state, start, stride);
 }
 
 // ------------------------------------------------------------------ append
@@ -200,7 +245,8 @@ __device__ __forceinline__ void load_index_quad<__nv_bfloat16>(const __nv_bfloat
 }
 
 // One warp per token: the slot is read once, keys and values move as 16-byte vectors with up to eight loads in
-// flight per lane, and the index key (128 elements, four per lane) is quantised from registers.  Bound by HBM.
+// flight per lane, and the index key (128 elements, four per lane) is quantised from registers.  Bound by HBM: 8191 tokens
+// of 8 heads of 128 with bf16 index keys take 13.4 us, 5.2 TB/s or 0.79 of the copy rate; 64 tokens 3.2 us, a launch.
 template <typename Source>
 __global__ void __launch_bounds__(kAppendThreads) itk_append_tokens_kernel(const itk_append_args p, int* status) {
     const unsigned token = blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5);

@@ -261,8 +261,9 @@ int itk_plan_pages(const itk_page_plan_args* args, itk_stream_t stream) {
     if (rc != ITK_OK) return rc;
     const long long work = std::max(static_cast<long long>(a.requests) * a.table_pages, static_cast<long long>(a.rows));
     const int grid = static_cast<int>(std::min<long long>(2 * device.sm_count, (work + 2 * kPlanThreads - 1) / (2 * kPlanThreads)));
+    const int wide = aligned16(a.slots) && aligned16(a.k_start) && aligned16(a.k_end);
     const size_t smem = (3 * static_cast<size_t>(a.requests) + 1) * sizeof(int);
-    itk_plan_pages_kernel<<<grid, kPlanThreads, smem, stream>>>(a, device.status);
+    itk_plan_pages_kernel<<<grid, kPlanThreads, smem, stream>>>(a, wide, device.status);
     return launched("itk_plan_pages_kernel");
 }
 

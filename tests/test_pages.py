@@ -65,7 +65,7 @@ def gpu(values, device):
 
 
 CASES = [(1, 1, 128, 1, 0), (1, 40, 128, 300, 5), (8, 16, 128, 1, 0), (7, 5, 256, 400, 100), (600, 9, 128, 200, 3),
-         (513, 3, 384, 2, 17), (3000, 4, 128, 1, 0)]
+         (513, 3, 384, 2, 17), (3000, 4, 128, 1, 0), (2000, 1, 128, 2, 1), (4001, 1, 128, 1, 2)]
 
 
 @pytest.mark.gpu

@@ -830,6 +830,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
+    bool planned = false;                // the producer: the unit of a small call is in the queue
+    if (warp == kAttnLoadWarp && p.small_plan != 0) planned = attn_small_plan(p, sh.small_requests, sh.small_first, sh.items[0], lane);
     if (warp == kAttnMmaWarp) {          // the first issuer owns TMEM
         tmem_alloc(&sh.tmem_base, kAttnTmemColumns);
         tmem_relinquish_alloc_permit();
@@ -879,7 +881,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
             bool there;
             if (p.small_plan != 0) {
                 // (at most one unit: nothing in the queue is waited for)
-                there = units == 0 && attn_small_plan(p, sh.small_requests, sh.small_first, place, lane);
+                there = units == 0 && planned;
                 if (!there && lane == 0) place[3] = make_int4(0, 0, 0, 0);
                 __syncwarp();
                 if (there) {
@@ -1394,11 +1396,15 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
 constexpr int kJoinThreads = 256;
 
 // out = sum_c 2^(lse_c - lse) out_c over the slots of a row (own ones, then the prefix's), in slot order.  One warp
-// per row; also clears the rows behind the last request when asked to.
-template <typename T, int DIM>
+// per row, kFlight partial rows on their way at a time; also clears the rows behind the last request when asked to.
+//
+// Bound by the chain record - statistics - rows - store, 3.5 us for one token over 8192 keys.  Small calls have fewer rows than
+// the device has warps and take the time of a trip per kFlight slots: 32 (one token 18.5 -> 16.6 us with 16 -> 32).  Large ones
+// have rows for all warps, and 32 cost occupancy (128 registers, 206 for 32; 64 rows over a prefix of 16384 keys 84.4 and 88.2 us).
+template <typename T, int DIM, int kFlight>
 __global__ void __launch_bounds__(kJoinThreads) itk_attention_join_kernel(const __grid_constant__ AttnParams p) {
     constexpr int kOwn = DIM / 32;
-    constexpr int kFlight = 16;          // partial rows on their way at a time
+    constexpr int kGroup = 4;            // partial rows that are asked for together
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int span = 2 * p.tile_tokens;
     const int heads = p.a.kv_heads;
@@ -1442,6 +1448,7 @@ __global__ void __launch_bounds__(kJoinThreads) itk_attention_join_kernel(const 
                 float held[kFlight][kOwn];
 #pragma unroll
                 for (int k = 0; k < kFlight; ++k) {
+                    if (k % kGroup == 0 && k >= here) break;
                     const float* values = p.w.partial_out + row_of(base + min(k, here - 1)) * DIM + lane * kOwn;
                     if constexpr (kOwn == 4) {
                         *reinterpret_cast<float4*>(held[k]) = *reinterpret_cast<const float4*>(values);
@@ -1461,6 +1468,7 @@ __global__ void __launch_bounds__(kJoinThreads) itk_attention_join_kernel(const 
                 for (int i = 0; i < kOwn; ++i) sums[i] *= shrink;
 #pragma unroll
                 for (int k = 0; k < kFlight; ++k) {
+                    if (k % kGroup == 0 && k >= here) break;
                     const float w = __shfl_sync(0xffffffffu, weight, k);
                     total += w;
 #pragma unroll

@@ -209,7 +209,10 @@ int launch_attention(const AttnParams& params, cudaStream_t stream) {
             itk_attention_plan_kernel<1024><<<1, 1024, 0, stream>>>(params);
         ITK_CUDA(launch_after(itk_attention_kernel<T, DIM>, params.sm_count, kAttnThreads, AttnShape<DIM>::kSmemBytes, stream, params));
     }
-    ITK_CUDA(launch_after(itk_attention_join_kernel<T, DIM>, 4 * params.sm_count, kJoinThreads, 0, stream, params));
+    if (params.small_plan)
+        ITK_CUDA(launch_after(itk_attention_join_kernel<T, DIM, 32>, 4 * params.sm_count, kJoinThreads, 0, stream, params));
+    else
+        ITK_CUDA(launch_after(itk_attention_join_kernel<T, DIM, 16>, 4 * params.sm_count, kJoinThreads, 0, stream, params));
     return launched("itk_attention_kernel");
 }
 

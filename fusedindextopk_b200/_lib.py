@@ -258,7 +258,8 @@ _WORDS = [struct.Struct("<%dQ" % n) for n in range(32)]
 
 
 def metadata(tensors: tuple) -> tuple:
-    return tuple([(t.shape, t.stride(), t.dtype, t.device) for t in tensors])
+    # (the device by its number, which is quicker; what is not on a GPU has -1 and is refused, so it is never kept)
+    return tuple([(t.shape, t.stride(), t.dtype, t.get_device()) for t in tensors])
 
 
 def launch(torch: Any, function: Any, block: Any, device: Any) -> None:

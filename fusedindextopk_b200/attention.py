@@ -152,7 +152,7 @@ def _attend(q: Any, own: tuple, prefix: tuple | None, prefix_keys: int, cu_seqle
         template = _lib.CallTemplate.keep(_TEMPLATES, key, _check_call(
             torch, q, own, prefix, prefix_keys, cu_seqlens_q, lengths, out, causal, scale))
     if out is None:
-        out = q.new_empty(q.shape)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)      # (new_empty takes 0.8 us longer)
     lse = q.new_empty(q.shape[:2], dtype=torch.float32) if return_lse else None
     if template.tokens:
         # of the caching allocator, on the call's stream: two calls, streams or captured graphs never share it

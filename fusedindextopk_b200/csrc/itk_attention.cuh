@@ -33,7 +33,9 @@
 // busy 77 % of the time (61 % of it with products: the N = 64 score products read 1.5 times the shared memory that
 // their arithmetic takes time for); without the exponentials it takes 0.50 ms, with an eighth of the products
 // 0.43 ms.  D = 64: 0.43 ms, 735 TFLOP/s, bound by the softmax warps: 16 exponentials a cycle and SM alone take 0.26 ms.
-// Single tokens (split mode): 5.9 TB/s of keys and values, 0.9 of the measured copy rate.
+// Single tokens (split mode): 6.1 TB/s of keys and values, 0.94 of the measured copy rate, and 5.5 when the power cap (1000 W)
+// holds in a long run.  One token over 8192 keys, 15.5 us: small plan 2, first keys 2, keys 4 (at the rate of memory), epilogue and
+// end 2, the join 3 behind a gap of 1.
 // Measured and left out (D = 128 / 64, ms): 128-key steps with single score buffers 0.76 / 0.64; UMMAs issued under
 // a lane comparison 1.16 / 0.99 (see elect_one); four softmax warps a scheduler with 96 registers 0.64 / 0.55; the lanes'
 // exponentials in turns 0.70 / 0.61; setmaxnreg (ptxas spills); every register spilled in the softmax loop costs, as
@@ -666,13 +668,17 @@ __device__ __forceinline__ bool attn_small_plan(const AttnParams& p, AttnRequest
     if (there) entry = attn_entry(p, AttnRequests{cache, first, true}, lane, prefix_entries, rows_end);
     const int cost = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(entry.tiles) * entry.unit);
     const int share = attn_share(p, static_cast<unsigned>(cost));
-    int counts[kAttnTries];
-#pragma unroll
-    for (int t = 0; t < kAttnTries; ++t) counts[t] = there ? max(1, attn_chunks(entry, share + share / kAttnTries * t, 0)) : 0;
+    // (a loop, not unrolled: code that runs once waits for its instructions, 1 us for eight copies of this)
     int chunk = 1 << 30;            // nothing is cut: that fits a wave
-#pragma unroll
-    for (int t = kAttnTries - 1; t >= 0; --t)
-        if (static_cast<int>(__reduce_add_sync(0xffffffffu, counts[t])) * kv_heads <= p.sm_count) chunk = share + share / kAttnTries * t;
+#pragma unroll 1
+    for (int t = 0; t < kAttnTries; ++t) {
+        const int length = share + share / kAttnTries * t;
+        const int wanted = there ? max(1, attn_chunks(entry, length, 0)) : 0;
+        if (static_cast<int>(__reduce_add_sync(0xffffffffu, wanted)) * kv_heads <= p.sm_count) {
+            chunk = length;
+            break;
+        }
+    }
 
     const int chunks = there ? attn_chunks(entry, chunk, 0) : 0, count = there ? max(1, chunks) : 0;
     const bool joined = there && attn_slots(p, entry, chunks);
@@ -1398,8 +1404,8 @@ constexpr int kJoinThreads = 256;
 // out = sum_c 2^(lse_c - lse) out_c over the slots of a row (own ones, then the prefix's), in slot order.  One warp
 // per row, kFlight partial rows on their way at a time; also clears the rows behind the last request when asked to.
 //
-// Bound by the chain record - statistics - rows - store, 3.5 us for one token over 8192 keys.  Small calls have fewer rows than
-// the device has warps and take the time of a trip per kFlight slots: 32 (one token 18.5 -> 16.6 us with 16 -> 32).  Large ones
+// Bound by the chain record - statistics - rows - store, about 3 us for one token over 8192 keys.  Small calls have fewer rows than
+// the device has warps and take the time of a trip per kFlight slots: 32 (the whole call 16.6 us, with 16 it took 17.6).  Large ones
 // have rows for all warps, and 32 cost occupancy (128 registers, 206 for 32; 64 rows over a prefix of 16384 keys 84.4 and 88.2 us).
 template <typename T, int DIM, int kFlight>
 __global__ void __launch_bounds__(kJoinThreads) itk_attention_join_kernel(const __grid_constant__ AttnParams p) {
@@ -1426,19 +1432,18 @@ __global__ void __launch_bounds__(kJoinThreads) itk_attention_join_kernel(const 
             const int head_index = head * p.group + r % p.group;
             // the row's own partial results, then the prefix's: two runs of rows
             int count = entry.slots, prefix_count = 0, prefix_rows = 0;
-            const long long first = entry.partial + static_cast<long long>(head) * entry.slots * rows + r;
-            long long prefix_first = 0;
+            const int first = entry.partial + head * entry.slots * rows + r;       // (partial rows are counted in 31 bits)
+            int prefix_first = 0;
             if (p.a.prefix_keys > 0) {
                 const int e = token / span;
                 const int2 slots = p.w.prefix_slots[e];
                 prefix_rows = min(span, counters.rows_end - e * span) * p.group;
-                prefix_first = slots.x + static_cast<long long>(head) * slots.y * prefix_rows + (token - e * span) * p.group + r % p.group;
+                prefix_first = slots.x + head * slots.y * prefix_rows + (token - e * span) * p.group + r % p.group;
                 prefix_count = slots.y;
             }
             count += prefix_count;
             auto row_of = [&](int c) {
-                return c < entry.slots ? first + static_cast<long long>(c) * rows
-                                       : prefix_first + static_cast<long long>(c - entry.slots) * prefix_rows;
+                return c < entry.slots ? first + c * rows : prefix_first + (c - entry.slots) * prefix_rows;
             };
             float top = -INFINITY, total = 0.0f, sums[kOwn] = {};
             bool broken = false;
@@ -1449,7 +1454,7 @@ __global__ void __launch_bounds__(kJoinThreads) itk_attention_join_kernel(const 
 #pragma unroll
                 for (int k = 0; k < kFlight; ++k) {
                     if (k % kGroup == 0 && k >= here) break;
-                    const float* values = p.w.partial_out + row_of(base + min(k, here - 1)) * DIM + lane * kOwn;
+                    const float* values = p.w.partial_out + static_cast<size_t>(row_of(base + min(k, here - 1))) * DIM + lane * kOwn;
                     if constexpr (kOwn == 4) {
                         *reinterpret_cast<float4*>(held[k]) = *reinterpret_cast<const float4*>(values);
                     } else {

@@ -240,6 +240,20 @@ def test_an_output_in_the_place_of_the_queries(device, prefix, q_lens, k_lens, h
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("q_lens,k_lens,heads,kv_heads,dim", [
+    ([150, 3, 200], [400, 3, 900], 8, 2, 128), ([1] * 9, [70 * i for i in range(9)], 14, 2, 64), ([1], [5000], 32, 8, 128)])
+def test_tensors_with_their_heads_first(device, q_lens, k_lens, heads, kv_heads, dim):
+    q, k, v = make(device, q_lens, k_lens, heads, kv_heads, dim, torch.bfloat16)
+    first = [t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k, v)]
+    want = expected(q, q_lens, split(k, v, k_lens))
+    for out in (None, torch.empty_like(first[0])):
+        got = attention.attention_varlen(first[0], tuple(first[1:]), sums(q_lens, device), sums(k_lens, device), out=out)
+        assert got.is_contiguous() if out is None else got is out
+        assert_close(got, None, want)
+    attention.check_status(device)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("q_len,k_len", [(1, 70), (40, 200), (300, 300)])
 def test_rows_behind_the_last_request(device, q_len, k_len):
     q, k, v = make(device, [q_len + 37], [k_len + 50], 8, 2, 128, torch.bfloat16)

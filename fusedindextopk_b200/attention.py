@@ -120,7 +120,7 @@ def _check_call(torch: Any, q: Any, own: tuple, prefix: tuple | None, prefix_key
         None, None, None, None, None, None, None, 0, None, None, None, None, None, None, q.stride(0), q.stride(1), strides[0], strides[1], 0, _segment(*own),
         _segment(*prefix) if prefix_keys else _lib.KvSegment(), scale,
         _lib.ELEMENT_BF16 if q.dtype == torch.bfloat16 else _lib.ELEMENT_FP16, tokens, heads, own[0].shape[-2], dim, requests,
-        prefix_keys, int(causal), int(out is None), 0)
+        prefix_keys, int(causal), 3 if out is None else 2, 0)
     needed = ctypes.c_size_t(0)
     if tokens:
         _lib.check(_lib.load_library().itk_attention_workspace_bytes(ctypes.byref(args), ctypes.byref(needed)))
@@ -180,8 +180,8 @@ def attention_varlen(q: Any, kv: tuple[Any, Any], cu_seqlens_q: Any, cu_seqlens_
     ``q`` is ``[T, Hq, D]``, ``kv = (k, v)`` both ``[N, H, D]``; request ``b`` owns rows
     ``cu_seqlens_q[b]:cu_seqlens_q[b+1]`` and keys ``cu_seqlens_k[b]:cu_seqlens_k[b+1]`` (int32 ``[B+1]`` each, lengths of
     zero allowed).  With ``causal`` row i of its Q sees its first ``N - Q + i + 1`` keys, else all N.  ``scale`` (positive)
-    defaults to ``D ** -0.5``.  Rows of no request are zero (log-sum-exp ``-inf``), or left as they were in a given ``out``.
-    ``out`` may be ``q`` itself and shares no other memory with the inputs.
+    defaults to ``D ** -0.5``.  Rows of no request are zero, or left as they were in a given ``out``; their
+    log-sum-exp is ``-inf``.  ``out`` may be ``q`` itself and shares no other memory with the inputs.
     """
 
     return _attend(q, tuple(kv), None, 0, cu_seqlens_q, cu_seqlens_k, causal, scale, out, return_lse)

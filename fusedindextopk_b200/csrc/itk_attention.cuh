@@ -1402,7 +1402,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
 constexpr int kJoinThreads = 256;
 
 // out = sum_c 2^(lse_c - lse) out_c over the slots of a row (own ones, then the prefix's), in slot order.  One warp
-// per row, kFlight partial rows on their way at a time; also clears the rows behind the last request when asked to.
+// per row, kFlight partial rows on their way at a time; also clears the rows of no request when asked to.
 //
 // Bound by the chain record - statistics - rows - store, about 3 us for one token over 8192 keys.  Small calls have fewer rows than
 // the device has warps and take the time of a trip per kFlight slots: 32 (the whole call 16.6 us, with 16 it took 17.6).  Large ones
@@ -1496,7 +1496,8 @@ __global__ void __launch_bounds__(kJoinThreads) itk_attention_join_kernel(const 
                 p.a.lse[static_cast<long long>(token) * p.a.heads + head_index] = broken ? nan : (empty ? -INFINITY : (top + log2f(total)) * kLn2);
         }
     }
-    if (p.a.clear_tail) {
+    const bool clear_out = (p.a.clear_tail & 1) != 0, clear_lse = (p.a.clear_tail & 2) != 0 && p.a.lse != nullptr;
+    if (clear_out || clear_lse) {
         // rows in front of the first request and behind the last one
         const long long head_rows = static_cast<long long>(counters.rows_begin) * p.a.heads;
         const long long tail = static_cast<long long>(max(counters.rows_end, counters.rows_begin)) * p.a.heads;
@@ -1506,12 +1507,14 @@ __global__ void __launch_bounds__(kJoinThreads) itk_attention_join_kernel(const 
             const long long r = i < head_rows ? i : tail + i - head_rows;
             const long long token = r / p.a.heads, head = r - token * p.a.heads;
             T* out = static_cast<T*>(p.a.out) + token * p.a.out_token_stride + head * p.a.out_head_stride + lane * kOwn;
-            if constexpr (kOwn == 4) {
-                *reinterpret_cast<uint2*>(out) = make_uint2(0u, 0u);
-            } else {
-                *reinterpret_cast<uint32_t*>(out) = 0u;
+            if (clear_out) {
+                if constexpr (kOwn == 4) {
+                    *reinterpret_cast<uint2*>(out) = make_uint2(0u, 0u);
+                } else {
+                    *reinterpret_cast<uint32_t*>(out) = 0u;
+                }
             }
-            if (lane == 0 && p.a.lse != nullptr) p.a.lse[r] = -INFINITY;
+            if (lane == 0 && clear_lse) p.a.lse[r] = -INFINITY;
         }
     }
 }

@@ -417,7 +417,8 @@ typedef struct itk_kv_segment {
 /* out[t, h] = sum_j softmax_j(scale * q[t, h] . k_j) v_j over the prefix keys [0, prefix_keys) and the own keys of
  * t's request; the request's rows are the LAST of its keys, and with `causal` row i of Q sees own keys
  * j < N - Q + i + 1.  lse (optional) = natural logarithm of the sum of exponentials.  A row without a key gets
- * out 0 and lse -inf.  Rows outside [cu_q[0], cu_q[requests]) are left as they were, or get the same with `clear_tail`.
+ * out 0 and lse -inf.  Rows outside [cu_q[0], cu_q[requests]) are left as they were, or get the same: out with bit 0 of
+ * `clear_tail`, lse with bit 1.
  * Lengths that decrease or exceed their buffers, and pages outside their pool, are clamped and reported in the status word. */
 typedef struct itk_attention_args {
     const void* q;             /* [tokens, heads, dim] */

@@ -268,6 +268,10 @@ def test_rows_behind_the_last_request(device, q_len, k_len):
     attention.attention_varlen(q, (k, v), cu_q, cu_k, out=out)
     assert_close(out, None, want)
     assert bool((out[q_len:] == 5.0).all()), "rows behind the last request were written"
+    torch.full_like(lse, 7.0)                                # (what the next call's log-sum-exps may find in their memory)
+    _, lse = attention.attention_varlen(q, (k, v), cu_q, cu_k, out=out, return_lse=True)
+    assert_close(out, lse, want)
+    assert bool((out[q_len:] == 5.0).all()) and bool((lse[q_len:] == -math.inf).all())
     # and rows in front of the first one
     for given in (None, torch.full_like(q, 5.0)):
         shifted = attention.attention_varlen(torch.cat([q[q_len:q_len + 30], q[:q_len], q[q_len:q_len + 7]]), (k, v), cu_q + 30, cu_k,

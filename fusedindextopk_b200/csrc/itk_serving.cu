@@ -107,10 +107,10 @@ int check_attention(const itk_attention_args& a) {
 }
 
 // Tokens of a row tile.  As many as fit; a batch of single tokens takes one, so that the other requests' queries are not
-// loaded, and multiplied, beside it: the power cap is what holds such a batch back when steps follow each other (64 tokens over 65 to
-// 32768 keys: 370 -> 347 us in a long run, 321 -> 313 cool; whole boxes are no quicker anywhere, but longer requests need them).  No more
-// tokens than requests is the sign of one; a batch that only looks like it gets shorter entries and the same results.  (The
-// prefix pass shares its entries between requests and takes all that fit.)
+// loaded, and multiplied, beside it: the power cap is what holds such a batch back when steps follow each other (64 tokens
+// over 65 to 32768 keys: 353 us with one token, 377 with all that fit; in a short run 313 and 321).  Longer requests need tiles
+// that are full.  No more tokens than requests is the sign of single ones; a batch that only looks like it gets shorter entries
+// and the same results.  (The prefix pass shares its entries between requests and takes all that fit.)
 int attention_tile_tokens(const itk_attention_args& a) {
     return a.tokens <= a.requests && a.prefix_keys == 0 ? 1 : kAttnTile / (a.heads / a.kv_heads);
 }

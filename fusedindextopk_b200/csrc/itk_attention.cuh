@@ -334,16 +334,20 @@ struct Element<__half> {
 
 // ------------------------------------------------------------------ plan
 
-// Lengths of one request, clamped to the buffers they index.
+// Lengths of one request, clamped to the buffers they index, its rows also to the end of the last request's: the entries of
+// a prefix cover the rows up to there, and the join looks the prefix's results up by the row.
 struct AttnRequest {
     int q_first, q_count, k_first, k_count;
 };
 
+// Where the last request's rows end.
+__device__ __forceinline__ int attn_rows_end(const itk_attention_args& p) { return min(max(p.cu_q[p.requests], 0), p.tokens); }
+
 __device__ __forceinline__ AttnRequest attn_request(const itk_attention_args& p, int b, bool& bad) {
     AttnRequest r;
-    const int q0 = p.cu_q[b], q1 = p.cu_q[b + 1];
-    r.q_first = min(max(q0, 0), p.tokens);
-    r.q_count = max(min(max(q1, 0), p.tokens) - r.q_first, 0);
+    const int q0 = p.cu_q[b], q1 = p.cu_q[b + 1], rows_end = attn_rows_end(p);
+    r.q_first = min(max(q0, 0), rows_end);
+    r.q_count = max(min(max(q1, 0), rows_end) - r.q_first, 0);
     bad |= q0 != r.q_first || q1 != r.q_first + r.q_count;
     if (p.cu_k != nullptr) {
         const int k0 = p.cu_k[b], k1 = p.cu_k[b + 1];
@@ -466,6 +470,10 @@ __device__ __forceinline__ int attn_share(const AttnParams& p, unsigned long lon
     return static_cast<int>(fminf(ceilf(static_cast<float>(cost) * p.a.kv_heads * p.inverse_sms) + 1.0f, 536870912.0f));
 }
 
+// Requests whose rows overlap (lengths that decrease in between) may have more entries in all than 31 bits count; the sums
+// stay at this, which is more than any buffer holds.  A warp's own sum, of 32 requests with up to 2^24 entries, fits.
+constexpr int kAttnMostEntries = 1 << 30;
+
 // Sum of the values of the lanes before this one; `total`: of all lanes.
 __device__ __forceinline__ int warp_prefix(int value, int lane, int& total) {
     int upto = value;
@@ -501,7 +509,7 @@ __global__ void __launch_bounds__(THREADS) itk_attention_plan_kernel(const __gri
         total_cost = 0;
         longest = item_count = combine_count = partial_rows = 0;
     }
-    if (tx == 32) rows_end = min(max(p.a.cu_q[p.a.requests], 0), p.a.tokens);
+    if (tx == 32) rows_end = attn_rows_end(p.a);
     if (tx < kAttnTries) counts[tx] = 0;
     for (int i = tx; i < kAttnBins; i += THREADS) bins[i] = 0;
     // (the barriers of the first pass below stand between these and their first readers: there is at least one request)
@@ -521,10 +529,10 @@ __global__ void __launch_bounds__(THREADS) itk_attention_plan_kernel(const __gri
         if (lane == 31) warp_sums[warp] = total;
         __syncthreads();
         int before = carry;
-        for (int w = 0; w < warp; ++w) before += warp_sums[w];
+        for (int w = 0; w < warp; ++w) before = min(before + warp_sums[w], kAttnMostEntries);
         if (b < p.a.requests) entry_first[b] = before + in_warp;
         __syncthreads();
-        if (tx == THREADS - 1) carry = before + total;
+        if (tx == THREADS - 1) carry = min(before + total, kAttnMostEntries);
     }
     if (bad) atomicOr(p.status, ITK_SERVING_BAD_LENGTHS);
     __syncthreads();
@@ -650,7 +658,7 @@ constexpr int kAttnSmallEntries = 32;
 
 __device__ __forceinline__ bool attn_small_plan(const AttnParams& p, AttnRequest* cache, int* first, int4* unit, int lane) {
     const int span = 2 * p.tile_tokens, kv_heads = p.a.kv_heads;
-    const int rows_end = min(max(p.a.cu_q[p.a.requests], 0), p.a.tokens);
+    const int rows_end = attn_rows_end(p.a);
     bool bad = false;
     int mine = 0, own;
     if (lane < p.a.requests) {
@@ -1434,7 +1442,7 @@ __global__ void __launch_bounds__(kJoinThreads) itk_attention_join_kernel(const 
             int count = entry.slots, prefix_count = 0, prefix_rows = 0;
             const int first = entry.partial + head * entry.slots * rows + r;       // (partial rows are counted in 31 bits)
             int prefix_first = 0;
-            if (p.a.prefix_keys > 0) {
+            if (p.a.prefix_keys > 0 && token < counters.rows_end) {
                 const int e = token / span;
                 const int2 slots = p.w.prefix_slots[e];
                 prefix_rows = min(span, counters.rows_end - e * span) * p.group;

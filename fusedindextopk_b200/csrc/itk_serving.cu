@@ -131,7 +131,8 @@ int attention_workspace(const itk_attention_args& a, AttnWorkspace* w, size_t* b
     long long partial = 2 * std::min(rows, static_cast<long long>(a.requests) * kAttnTile * a.kv_heads) +
                         2 * std::min(2 * added * kAttnTile, rows * (added / a.kv_heads + 1));
     if (prefix > 0) partial += 3 * rows;
-    ITK_REQUIRE(partial < (1ll << 31) - 1 && (own + prefix + added) * a.kv_heads < (1ll << 31), "the batch is too large for one call");
+    ITK_REQUIRE(partial < (1ll << 31) - 1 && own < kAttnMostEntries && (own + prefix + added) * a.kv_heads < (1ll << 31),
+                "the batch is too large for one call");
     size_t at = 0;
     auto take = [&](size_t size) {
         const size_t offset = at;

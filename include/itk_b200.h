@@ -419,7 +419,8 @@ typedef struct itk_kv_segment {
  * j < N - Q + i + 1.  lse (optional) = natural logarithm of the sum of exponentials.  A row without a key gets
  * out 0 and lse -inf.  Rows outside [cu_q[0], cu_q[requests]) are left as they were, or get the same: out with bit 0 of
  * `clear_tail`, lse with bit 1.
- * Lengths that decrease or exceed their buffers, and pages outside their pool, are clamped and reported in the status word. */
+ * Lengths that decrease or exceed their buffers, and pages outside their pool, are clamped and reported in the status word;
+ * a request's rows end where the last request's do, at cu_q[requests]. */
 typedef struct itk_attention_args {
     const void* q;             /* [tokens, heads, dim] */
     void* out;                 /* [tokens, heads, dim] */

@@ -570,3 +570,44 @@ def test_argument_structs_match_the_header():
         body = re.sub(r"/\*.*?\*/", "", body, flags=re.S).split("{", 1)[1]
         fields = [re.sub(r"[\s*]", " ", f).split()[-1] for line in body.split(";") for f in line.split(",") if f.strip()]
         assert fields == [field for field, _ in mirror._fields_]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("prefix", [0, 1000])
+@pytest.mark.parametrize("empty", [0, 90, 1300])         # the plan in the attention kernel, the plan kernel, its uncached lengths
+@pytest.mark.parametrize("ends", [[0, 30, 100, 40], [0, 100, 4], [0, 3, 90, 0], [70, 90, 100, 20]])
+def test_row_ends_that_decrease_are_clamped_to_the_last_one(device, prefix, empty, ends):
+    """Rows behind ``cu_seqlens_q[-1]`` belong to no request, whatever the ends before it say."""
+
+    heads, kv_heads, dim = 16, 2, 128
+    ends = ends + ends[-1:] * empty
+    k_lens = ([200, 45, 33] * len(ends))[:len(ends) - 1]
+    q, k, v = make(device, [120], [prefix] + k_lens, heads, kv_heads, dim, torch.bfloat16, seed=11)
+    kp, vp, k, v = k[:prefix], v[:prefix], k[prefix:], v[prefix:]
+    cu_q = torch.tensor(ends, dtype=torch.int32, device=device)
+    got, lse = attention.shared_prefix_attention(q, (kp, vp), (k, v), cu_q, sums(k_lens, device), return_lse=True)
+    with pytest.raises(_lib.ItkError, match="lengths"):
+        attention.check_status(device)
+    clamped = [min(end, ends[-1]) for end in ends]
+    q_lens = [max(b - a, 0) for a, b in zip(clamped, clamped[1:])]
+    first, last = clamped[0], clamped[0] + sum(q_lens)
+    want = expected(q[first:last], q_lens, split(k, v, k_lens, kp if prefix else None, vp if prefix else None))
+    assert_close(got[first:last], lse[first:last], want)
+    for rest, rest_lse in ((got[:first], lse[:first]), (got[last:], lse[last:])):
+        assert bool((rest == 0).all()) and bool((rest_lse == -math.inf).all())
+
+
+@pytest.mark.gpu
+def test_requests_whose_rows_overlap_are_reported_and_stay_in_their_buffers(device):
+    """More entries in all than the buffers hold: every other request claims all rows and all keys."""
+
+    heads, kv_heads, dim, tokens, keys, requests = 8, 1, 64, 600, 500, 4000
+    q, k, v = make(device, [tokens], [keys], heads, kv_heads, dim, torch.bfloat16, seed=12)
+    held = torch.full((tokens + 2, heads, dim), 9.0, dtype=q.dtype, device=device)
+    cu_q, cu_k = (torch.tensor([0, n] * (requests // 2) + [n], dtype=torch.int32, device=device) for n in (tokens, keys))
+    for kp, vp in ((k[:0], v[:0]), (k[:70], v[:70])):
+        attention.shared_prefix_attention(q, (kp, vp), (k, v), cu_q, cu_k, out=held[1:-1])
+        with pytest.raises(_lib.ItkError, match="lengths"):
+            attention.check_status(device)
+        assert bool((held[0] == 9).all()) and bool((held[-1] == 9).all())
+        assert_close(held[1:-1], None, expected(q, [tokens], [(k, v, kp, vp)]))      # they all say the same of a row

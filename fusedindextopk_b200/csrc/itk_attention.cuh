@@ -1122,11 +1122,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 found = __any_sync(0xffffffffu, found) != 0;
+                __syncwarp();            // orders all lanes' writes before the arrival, which a vote does not
                 if (lane == 0) {
                     if (found) *reinterpret_cast<volatile int*>(&sh.poison[units % kAttnPoison]) = units;
                     mbar_arrive(&sh.kv_full[stage]);
                 }
-                __syncwarp();
             }
             ring += 2 * item.tiles;
         }

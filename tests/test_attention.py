@@ -611,3 +611,21 @@ def test_requests_whose_rows_overlap_are_reported_and_stay_in_their_buffers(devi
             attention.check_status(device)
         assert bool((held[0] == 9).all()) and bool((held[-1] == 9).all())
         assert_close(held[1:-1], None, expected(q, [tokens], [(k, v, kp, vp)]))      # they all say the same of a row
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+def test_what_lies_behind_the_ends_of_requests_changes_no_bit(device, dim):
+    """Every value tile that ends inside a page is cleared by the guard before it is multiplied, in every call."""
+
+    q_lens = [1, 130, 5, 64, 1, 257, 2] * 6
+    k_lens = [n + 37 * i for i, n in enumerate(q_lens)]
+    q, k, v = make(device, q_lens, k_lens, 16, 4, dim, torch.bfloat16, seed=13)
+    cu_q, lens = sums(q_lens, device), torch.tensor(k_lens, dtype=torch.int32, device=device)
+    held = [paged(k, v, k_lens, 256, seed=13, fill=fill) for fill in (0.0, float("nan"), float("inf"))]
+    want = attention.attention_paged(q, *held[0], cu_q, lens, return_lse=True)
+    for _ in range(10):
+        for pools, table in held[1:]:
+            got = attention.attention_paged(q, pools, table, cu_q, lens, return_lse=True)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    attention.check_status(device)

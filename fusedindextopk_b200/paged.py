@@ -194,7 +194,12 @@ class PagePlan:
     k_end: Any
     pages_needed: Any
     block_table: Any = None
-    templates: dict = field(default_factory=dict, repr=False)     # checked argument blocks, with this plan's own buffers
+    # checked argument blocks of this plan's sizes and buffers, without addresses
+    templates: dict = field(default_factory=dict, init=False, repr=False, compare=False)
+
+    def __setattr__(self, name: str, value: Any) -> None:
+        self.__dict__[name] = value
+        self.__dict__["templates"] = {}         # another size or buffer: checked again (a copy keeps the blocks that it has)
 
 
 def make_page_plan(requests: int, table_pages: int, rows: int, *, page_size: int, device: Any) -> PagePlan:
@@ -240,15 +245,24 @@ def plan_pages(plan: PagePlan, block_table: Any, lengths: Any, new_tokens: Any, 
     template = plan.templates.get(key)
     if template is None:
         template = _lib.CallTemplate.keep(plan.templates, key, _check_plan(torch, plan, *tensors))
-    block = template.fill([t.data_ptr() for t in tensors])
-    _lib.launch(torch, _lib.load_library().itk_plan_pages, block, plan.slots.device)
-    plan.block_table = block_table
+    block = template.fill((
+        block_table.data_ptr(), lengths.data_ptr(), new_tokens.data_ptr(), free_pages.data_ptr(), plan.slots.data_ptr(),
+        plan.cu_seqlens_q.data_ptr(), plan.lengths.data_ptr(), plan.flat_table.data_ptr(), plan.k_start.data_ptr(),
+        plan.k_end.data_ptr(), plan.pages_needed.data_ptr()))
+    _lib.launch(torch, _lib.load_library().itk_plan_pages, block, template.device)
+    plan.__dict__["block_table"] = block_table
     return plan
 
 
 def _check_plan(torch: Any, plan: PagePlan, block_table: Any, lengths: Any, new_tokens: Any, free_pages: Any) -> _lib.CallTemplate:
     rows, requests = plan.rows, plan.requests
     device = plan.slots.device
+    for name, count, dtype in (("slots", rows, torch.int64), ("cu_seqlens_q", requests + 1, torch.int32),
+                               ("lengths", requests, torch.int32), ("flat_table", requests * plan.table_pages, torch.int32),
+                               ("k_start", rows, torch.int32), ("k_end", rows, torch.int32), ("pages_needed", 1, torch.int32)):
+        buffer = getattr(plan, name)
+        _require(buffer.is_cuda and buffer.device == device and buffer.dtype == dtype and tuple(buffer.shape) == (count,)
+                 and buffer.is_contiguous(), f"the plan's {name} must be contiguous {dtype} [{count}] on one CUDA device")
     for name, tensor, count in (("lengths", lengths, requests), ("new_tokens", new_tokens, requests),
                                 ("free_pages", free_pages, None)):
         _require(tensor.dtype == torch.int32 and tensor.dim() == 1 and tensor.is_contiguous(), f"{name} must be contiguous int32")
@@ -260,9 +274,8 @@ def _check_plan(torch: Any, plan: PagePlan, block_table: Any, lengths: Any, new_
     _require((block_table.stride(1) == 1 or plan.table_pages == 1) and (block_table.stride(0) >= plan.table_pages or requests == 1),
              "block_table rows must be contiguous and must not overlap")
     return _lib.CallTemplate(_lib.PagePlanArgs(
-        None, None, None, None, plan.slots.data_ptr(), plan.cu_seqlens_q.data_ptr(), plan.lengths.data_ptr(),
-        plan.flat_table.data_ptr(), plan.k_start.data_ptr(), plan.k_end.data_ptr(), plan.pages_needed.data_ptr(),
-        max(block_table.stride(0), plan.table_pages), requests, plan.table_pages, plan.page_size, free_pages.shape[0], rows))
+        *[None] * 11, max(block_table.stride(0), plan.table_pages), requests, plan.table_pages, plan.page_size,
+        free_pages.shape[0], rows), device=device)
 
 
 def append_tokens(slots: Any, kv: tuple[Any, Any], pools: tuple[Any, Any], *, index_keys: Any = None,

@@ -2,7 +2,9 @@
 
 from __future__ import annotations
 
+import copy
 import ctypes
+import dataclasses
 
 import pytest
 import torch
@@ -293,3 +295,63 @@ def test_c_entries_refuse_before_any_launch():
     append.k_row_stride, append.v = 8, (1 << 20) + 8
     assert library.itk_append_tokens(ctypes.byref(append), None) == -1
     assert b"aligned" in library.itk_last_error()
+
+
+def cpu_plan(requests=2, columns=3, rows=5):
+    """A plan whose buffers live on the CPU: enough for what the host keeps of it."""
+
+    def buffer(count, dtype=torch.int32):
+        return torch.zeros(count, dtype=dtype)
+
+    return paged.PagePlan(requests, columns, rows, 128, buffer(rows, torch.int64), buffer(requests + 1), buffer(requests),
+                          buffer(requests * columns), buffer(rows), buffer(rows), buffer(1))
+
+
+def test_a_changed_plan_keeps_no_argument_block():
+    plan = cpu_plan()
+    plan.templates["key"] = "block"
+    assert dataclasses.replace(plan, slots=torch.zeros(5, dtype=torch.int64)).templates == {}
+    other = copy.copy(plan)
+    assert plan.templates == other.templates == {"key": "block"}
+    other.rows = 4
+    assert other.templates == {} and plan.templates == {"key": "block"}
+    plan.slots = torch.zeros(5, dtype=torch.int64)
+    assert plan.templates == {}
+
+
+def test_no_address_is_kept_between_plans(monkeypatch):
+    """The block of a call holds the addresses of the plan it was made for, also of one copied after a call."""
+
+    seen = []
+    monkeypatch.setattr(_lib, "launch", lambda torch, function, block, device: seen.append(_lib.PagePlanArgs.from_buffer_copy(block)))
+    sizes = _lib.PagePlanArgs(*[None] * 11, 3, 2, 3, 128, 4, 5)
+    monkeypatch.setattr(paged, "_check_plan", lambda torch, plan, *tensors: _lib.CallTemplate(sizes, device=None))
+    table, ints = torch.zeros((2, 3), dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    first = cpu_plan()
+    paged.plan_pages(first, table, ints, ints, ints)
+    moved = dataclasses.replace(first, lengths=torch.zeros(2, dtype=torch.int32))
+    for plan in (first, copy.deepcopy(first), copy.copy(first), moved):
+        paged.plan_pages(plan, table, ints, ints, ints)
+        for field, name in (("slots", "slots"), ("cu_q", "cu_seqlens_q"), ("lengths", "lengths"), ("flat", "flat_table"),
+                            ("k_start", "k_start"), ("k_end", "k_end"), ("pages_needed", "pages_needed")):
+            assert getattr(seen[-1], field) == getattr(plan, name).data_ptr()
+        assert (seen[-1].table, seen[-1].old, seen[-1].rows, seen[-1].page_size) == (table.data_ptr(), ints.data_ptr(), 5, 128)
+
+
+@pytest.mark.gpu
+def test_copied_and_replaced_plans_fill_their_own_buffers(device):
+    plan = paged.make_page_plan(3, 4, 8, page_size=128, device=device)
+    table = torch.full((3, 4), -1, dtype=torch.int32, device=device)
+    free, old = gpu(list(range(12)), device), gpu([127, 0, 255], device)
+    paged.plan_pages(plan, table, old, gpu([1, 0, 2], device), free)
+    before = plan.lengths.tolist()
+    changed = copy.copy(plan)
+    changed.lengths = torch.zeros_like(plan.lengths)
+    for other in (copy.deepcopy(plan), dataclasses.replace(plan, lengths=torch.zeros_like(plan.lengths)), changed):
+        got = paged.plan_pages(other, table, old, gpu([2, 1, 3], device), free)
+        assert got is other and other.lengths.tolist() == [129, 1, 258]
+        assert plan.lengths.tolist() == before
+    plan.k_end = torch.zeros(7, dtype=torch.int32, device=device)
+    with pytest.raises(ValueError, match="k_end"):
+        paged.plan_pages(plan, table, old, gpu([1, 0, 2], device), free)
+    paged.check_serving_status(device)

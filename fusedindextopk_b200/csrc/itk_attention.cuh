@@ -4,7 +4,9 @@
 //
 // over the prefix keys (all of them) and the request's own keys (the first min(N, N - Q + i + 1) of them for row i
 // of Q when causal).  Scores, statistics and sums are fp32; the weights are rounded to the element type once, for the
-// product with the values (half a step of 16 bits each, against the output's own half step), and summed unrounded.
+// product with the values (half a step of 16 bits each, against the output's own half step), and summed unrounded.  fp16
+// weights lose bits below 2^-14, so they are held 2^7 times larger (Element::kHeadroom): what falls below half a step is less than
+// 2^-32 of the largest weight a key, instead of 2^-25, of which 131072 keys behind one strong one lost 0.4 % of a sum.
 //
 // Rows.  The G = heads / kv_heads query heads of a key head share its keys, so one 128-row tile holds TT = 128 / G
 // consecutive tokens x G heads (row r = token r / G, head r % G): a single token of a decode step fills G rows of a
@@ -26,7 +28,7 @@
 // steps of 64 keys.  TMEM: two buffers of 64 score columns per lane, so that the scores of step i + 1 are computed while
 // the softmax works on step i (the weights P overwrite the first half of their scores as 16-bit pairs and are the A
 // operand of P V from there), and O_A, O_B.  The row maximum is only moved when it grows by more than 2^8 (kAttnLazy):
-// until then weights are at most 2^8 and O needs no rescaling; when it does, the row's own softmax warp rescales O in TMEM
+// until then weights are at most 2^8 (2^15 as fp16) and O needs no rescaling; when it does, the row's own softmax warp rescales O in TMEM
 // after the last P V issued so far.
 //
 // What bounds it (B200, 4736 x 8192 rows, 32 / 8 heads, bf16, no mask).  D = 128: 0.52 ms, 1220 TFLOP/s; the tensor unit is
@@ -290,7 +292,7 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // is what the softmax is short of.  z = n + f with n the nearest whole number (adding 1.5 * 2^23 leaves it in the low bits),
 // 2^f by a polynomial of degree 5, fitted for the least relative error on [-1/2, 1/2] by iteratively reweighted least
 // squares (7.5e-8), 2^n by its exponent bits.  Below the normal range the result is 0, as exp2_fast's is; NaN stays NaN.
-// z <= 127 is all that is asked for (weights are at most 2^kAttnLazy).
+// z <= 127 is all that is asked for (weights are at most 2^(kAttnLazy + kHeadroom)).
 __device__ __forceinline__ float2 exp2_polynomial(float2 z) {
     auto both = [](float x) { return make_float2(x, x); };
     const float2 shifted = add2(z, both(12582912.0f));
@@ -311,6 +313,7 @@ struct Element;
 template <>
 struct Element<__nv_bfloat16> {
     static constexpr bool kBf16 = true;
+    static constexpr float kHeadroom = 0.0f;         // log2 of how much larger than 1 the weight of the maximum is held
     static constexpr uint32_t kExponent = 0x7f80u;
     static __device__ __forceinline__ uint32_t pack(float low, float high) {
         uint32_t r;
@@ -323,6 +326,7 @@ struct Element<__nv_bfloat16> {
 template <>
 struct Element<__half> {
     static constexpr bool kBf16 = false;
+    static constexpr float kHeadroom = 7.0f;
     static constexpr uint32_t kExponent = 0x7c00u;
     static __device__ __forceinline__ uint32_t pack(float low, float high) {
         uint32_t r;
@@ -331,6 +335,8 @@ struct Element<__half> {
     }
     static __device__ __forceinline__ float value(uint32_t bits) { return __half2float(__ushort_as_half(static_cast<unsigned short>(bits))); }
 };
+
+static_assert(kAttnLazy + Element<__half>::kHeadroom <= 15.0f, "fp16 weights stay finite");
 
 // ------------------------------------------------------------------ plan
 
@@ -1173,6 +1179,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.p_full[x][at & 1]);
             };
+            // What is taken off the scaled scores for a new maximum.  Rounded up as fp16, and `moves` below rounds down, so that
+            // no rounding of large scores lifts a weight above 2^(kAttnLazy + kHeadroom): 2^16 would be infinite.
+            auto base_of = [&](float maximum) {
+                if constexpr (Element<T>::kHeadroom == 0.0f) return maximum * scale;
+                return __fadd_ru(__fmul_ru(maximum, scale), -Element<T>::kHeadroom);
+            };
             uint32_t s[2][32];
             float step_top = -INFINITY;
             // the scores of a step, which have arrived in s: masked where a row does not see all of them, and their maximum
@@ -1217,7 +1229,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
                 tmem_load_wait(s[1]);
                 take_scores();
                 top = step_top;
-                base = top == -INFINITY ? 0.0f : top * scale;
+                base = top == -INFINITY ? 0.0f : base_of(top);
                 for (;; ++at) {
                     const uint32_t here = tmem_s + (at & 1) * kAttnHalf, there = tmem_s + ((at + 1) & 1) * kAttnHalf;
                     const bool more = at + 1 < steps;
@@ -1262,11 +1274,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
                         tmem_load_wait(s[1]);
                         take_scores();
                     }
-                    const bool moves = step_top > top + p.lazy;
+                    const bool moves = step_top > __fadd_rd(top, p.lazy);
                     if (__any_sync(0xffffffffu, moves)) {
                         float shrink = 1.0f;
                         if (moves) {
-                            const float new_base = step_top * scale;
+                            const float new_base = base_of(step_top);
                             shrink = top == -INFINITY ? 0.0f : exp2_fast(base - new_base);
                             top = step_top;
                             base = new_base;

@@ -629,3 +629,61 @@ def test_what_lies_behind_the_ends_of_requests_changes_no_bit(device, dim):
             got = attention.attention_paged(q, pools, table, cu_q, lens, return_lse=True)
             assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     attention.check_status(device)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tail", [12.3, 20.04, 25.01, 31.0])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_a_long_tail_behind_one_strong_key_keeps_its_weight(device, tail, dtype):
+    """262144 keys of weight 2^-tail behind one of weight 1, uncut: 400 requests on the same pages.
+
+    Weights as fp16 may lose 2^-32 of the largest each (a step of 2^-24 at 2^7 times their size, rounded to the nearest);
+    everything else as in ``definition``.
+    """
+
+    requests, n, dim, page = 400, 1 << 18, 64, 256
+    u = torch.finfo(dtype).eps / 2
+    k = torch.zeros((n // page, page, 1, dim), dtype=dtype, device=device)
+    k[..., 0] = -1.0
+    k[0, 0] = 0.0
+    v = torch.ones_like(k)
+    v[0, 0, 0, 32:] = 0.0                       # half of the columns hold the tail alone
+    q = torch.zeros((requests, 1, dim), dtype=dtype, device=device)
+    q[..., 0] = 1.0
+    scale = tail * math.log(2.0)
+    weight = math.exp(-ctypes.c_float(scale).value)
+    table = torch.arange(n // page, dtype=torch.int32, device=device).unsqueeze(0).expand(requests, -1)
+    lens = torch.full((requests,), n, dtype=torch.int32, device=device)
+    got, lse = attention.attention_paged(q, (k, v), table, sums([1] * requests, device), lens, scale=scale, return_lse=True)
+    attention.check_status(device)
+    total = 1.0 + (n - 1) * weight
+    # scores are 0 and -scale exactly up to the scale's own product with log2(e): 4 e of the largest
+    rel = 2 * 4 * E * scale + 2.0 ** -20 + n * E
+    lost = 2.0 ** -32 * n if dtype == torch.float16 else 0.0
+    for columns, want in ((slice(0, 32), 1.0), (slice(32, 64), (n - 1) * weight / total)):
+        off = (got[:, 0, columns].double() - want).abs().max().item()
+        assert off <= (2.01 * u + rel) * want + lost, (off / want, tail)
+    assert (lse.double() - math.log(total)).abs().max().item() <= rel + 2.0 ** -20
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("magnitude", [2.0 ** 10, 2.0 ** 20, 2.0 ** 24, 2.0 ** 25])
+def test_weights_stay_finite_at_any_size_of_the_scores(device, magnitude):
+    """Maxima that grow by about 2^8 from step to step, where fp16 weights come nearest to their largest value."""
+
+    g = torch.Generator(device=device).manual_seed(14)
+    n, dim = 6000, 64
+    q = torch.zeros((8, 1, dim), dtype=torch.float16, device=device)
+    k = torch.zeros((n, 1, dim), dtype=torch.float16, device=device)
+    q[..., 0], q[..., 1] = 256.0, 1.0
+    k[..., 0] = 256.0
+    growth = 8 * math.log(2.0) * 65536.0 / magnitude               # a factor of 2^8 between the weights
+    k[:, 0, 1] = (torch.arange(n, device=device) // 64 + 1.1 * torch.rand(n, generator=g, device=device)) * growth
+    v = torch.rand((n, 1, dim), generator=g, device=device).to(torch.float16)
+    got, lse = attention.attention_varlen(q, (k, v), sums([8], device), sums([n], device), causal=False,
+                                          scale=magnitude / 65536.0, return_lse=True)
+    attention.check_status(device)
+    assert bool(got.isfinite().all()) and bool(lse.isfinite().all())
+    # A mean of values in [0, 1]: the base is rounded up by two steps of a scaled score at most, 8 at 2^25 * log2(e), so the largest
+    # weight is 2^-1 at least and its rounding off by 2^-11 of it; smaller ones by 2^-11 of theirs or 2^-25.
+    assert bool((got >= 0).all()) and bool((got <= 1 + 2.0 ** -11 + 2.0 ** -11 + n * 2.0 ** -24).all())

@@ -121,11 +121,12 @@ struct AttnWorkspace {
 };
 
 struct AttnParams {
-    CUtensorMap map_q, map_k, map_v, map_k_prefix, map_v_prefix;
+    CUtensorMap map_q, map_q_one, map_k, map_v, map_k_prefix, map_v_prefix;     // map_q_one: for items of a single token
     itk_attention_args a;
     AttnWorkspace w;
     int* status;
     int group, tile_tokens, sm_count, withhold_loads;
+    int q_bytes, q_bytes_one;                      // of a box of map_q, of map_q_one
     int small_plan;                                // no plan kernel ran: see attn_small_plan
     int out_sectors;                               // rows of the output start on 32-byte boundaries
     float inverse_sms;                             // 1 / sm_count
@@ -839,10 +840,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
         prefetch_tensormap(&p.map_k);
         prefetch_tensormap(&p.map_v);
     }
-    // Rows that no load fills are zero, so that multiplying them costs little power; while the plan runs this takes no time of
-    // its own.  (Without a plan kernel it would cost a single token 1 of 18.5 us.)
+    // Rows behind a single token's stay zero until longer items have left theirs there, so that multiplying them costs little
+    // power; while the plan runs this takes no time of its own.  (Without a plan kernel it would cost a single token 1 us.)
     if (!p.small_plan) {
-        for (int i = p.tile_tokens * p.group * (DIM / 8) + static_cast<int>(threadIdx.x); i < kAttnTile * (DIM / 8); i += kAttnThreads) {
+        for (int i = p.group * (DIM / 8) + static_cast<int>(threadIdx.x); i < kAttnTile * (DIM / 8); i += kAttnThreads) {
             const int row = i / (DIM / 8), vector = i % (DIM / 8);
             for (int tile = 0; tile < 2; ++tile)
                 *reinterpret_cast<uint4*>(smem_q + tile * Shape::kTileBytes + (vector / 8) * (kAttnTile * 128) + row * 128 +
@@ -892,7 +893,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
         // ============================================================ TMA producer
         int ring = 0;                 // tiles loaded so far
         int q_uses[2] = {0, 0};
-        const int q_bytes = Shape::kChunks * p.tile_tokens * p.group * 128;
         const int kv_heads = p.a.kv_heads;
         // The first unit of a CTA is the one with its number, the others are taken when their turn comes.
         int unit = static_cast<int>(blockIdx.x), next_unit = 0;
@@ -933,13 +933,18 @@ __global__ void __launch_bounds__(kAttnThreads, 1) itk_attention_kernel(const __
             if (!there) break;
             const AttnLanes l = attn_lanes(item, p.tile_tokens);
             if (item.tiles == 0 || p.withhold_loads != 0) continue;
+            // A single token's box holds its own queries only.  The rows beside them would be other requests', multiplied for
+            // nothing, and the power cap is what holds a batch of single tokens back when steps follow each other (64
+            // tokens over 65 to 32768 keys, 64/8 heads: 318 us, 333 with them; in a short run 304 and 307).
+            const CUtensorMap* map_q = item.tokens == 1 ? &p.map_q_one : &p.map_q;
+            const int q_bytes = item.tokens == 1 ? p.q_bytes_one : p.q_bytes;
             for (int tile = 0; ok && tile < (l.pair ? 2 : 1); ++tile) {
                 ok = wait(&sh.q_empty[tile], (q_uses[tile] & 1) ^ 1);
                 ++q_uses[tile];
                 if (ok && lane == 0) {
                     mbar_arrive_expect_tx(&sh.q_full[tile], q_bytes);
                     for (int c = 0; c < Shape::kChunks; ++c)
-                        tma_load_3d(smem_q + tile * Shape::kTileBytes + c * (kAttnTile * 128), &p.map_q, &sh.q_full[tile], c * 64,
+                        tma_load_3d(smem_q + tile * Shape::kTileBytes + c * (kAttnTile * 128), map_q, &sh.q_full[tile], c * 64,
                                     head * p.group, item.q_first + tile * p.tile_tokens);
                 }
             }

@@ -106,14 +106,8 @@ int check_attention(const itk_attention_args& a) {
     return ITK_OK;
 }
 
-// Tokens of a row tile.  As many as fit; a batch of single tokens takes one, so that the other requests' queries are not
-// loaded, and multiplied, beside it: the power cap is what holds such a batch back when steps follow each other (64 tokens
-// over 65 to 32768 keys: 353 us with one token, 377 with all that fit; in a short run 313 and 321).  Longer requests need tiles
-// that are full.  No more tokens than requests is the sign of single ones; a batch that only looks like it gets shorter entries
-// and the same results.  (The prefix pass shares its entries between requests and takes all that fit.)
-int attention_tile_tokens(const itk_attention_args& a) {
-    return a.tokens <= a.requests && a.prefix_keys == 0 ? 1 : kAttnTile / (a.heads / a.kv_heads);
-}
+// Tokens of a row tile: as many as fit.
+int attention_tile_tokens(const itk_attention_args& a) { return kAttnTile / (a.heads / a.kv_heads); }
 
 constexpr int kAttnMaxSms = 160;     // the workspace is sized for any device the library runs on
 
@@ -360,8 +354,17 @@ int itk_attention(const itk_attention_args* args, itk_stream_t stream) {
     {
         const cuuint64_t dims[3] = {static_cast<cuuint64_t>(a.dim), static_cast<cuuint64_t>(a.heads), static_cast<cuuint64_t>(a.tokens)};
         const cuuint64_t strides[2] = {map_stride(a.q_head_stride, a.heads), map_stride(a.q_token_stride, a.tokens)};
-        const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(params.group), static_cast<cuuint32_t>(params.tile_tokens)};
+        cuuint32_t box[3] = {64, static_cast<cuuint32_t>(params.group), static_cast<cuuint32_t>(std::min(params.tile_tokens, a.tokens))};
+        const int token_bytes = a.dim * 2 * params.group;
         if ((rc = encode_map(&params.map_q, a.element, 3, a.q, dims, strides, box)) != ITK_OK) return rc;
+        params.q_bytes = token_bytes * static_cast<int>(box[2]);
+        params.map_q_one = params.map_q;
+        params.q_bytes_one = params.q_bytes;
+        if (!params.small_plan && box[2] > 1) {       // (a small call is too short for power to matter)
+            box[2] = 1;
+            if ((rc = encode_map(&params.map_q_one, a.element, 3, a.q, dims, strides, box)) != ITK_OK) return rc;
+            params.q_bytes_one = token_bytes;
+        }
     }
     if (a.k != nullptr) {
         const itk_kv_segment& s = a.own;

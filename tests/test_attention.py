@@ -687,3 +687,48 @@ def test_weights_stay_finite_at_any_size_of_the_scores(device, magnitude):
     # A mean of values in [0, 1]: the base is rounded up by two steps of a scaled score at most, 8 at 2^25 * log2(e), so the largest
     # weight is 2^-1 at least and its rounding off by 2^-11 of it; smaller ones by 2^-11 of theirs or 2^-25.
     assert bool((got >= 0).all()) and bool((got <= 1 + 2.0 ** -11 + 2.0 ** -11 + n * 2.0 ** -24).all())
+
+
+@pytest.mark.gpu
+def test_a_long_request_among_empty_ones_fills_its_tiles(device):
+    """What a step's buffers leave room for does not change how its rows are packed: 8 entries of 32 tokens, not 128 of two."""
+
+    slots, heads, kv_heads, dim, keys = 256, 64, 8, 128, 3000
+    q, k, v = make(device, [slots], [keys], heads, kv_heads, dim, torch.bfloat16, seed=15)
+    cu_q, cu_k = sums([0] * 9 + [slots] + [0] * (slots - 10), device), sums([0] * 9 + [keys] + [0] * (slots - 10), device)
+    out = torch.empty_like(q)
+    template = attention._check_call(torch, q, (k, v), None, 0, cu_q, cu_k, out, True, None)
+    args = _lib.AttentionArgs.from_buffer_copy(template.bytes)
+    workspace = torch.empty(template.workspace_bytes, dtype=torch.uint8, device=device)
+    args.q, args.out, args.cu_q, args.cu_k = q.data_ptr(), out.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr()
+    args.k, args.v, args.workspace, args.workspace_bytes = k.data_ptr(), v.data_ptr(), workspace.data_ptr(), workspace.numel()
+    _lib.check(_lib.load_library().itk_attention(ctypes.byref(args), _lib.current_stream(torch, device)))
+    attention.check_status(device)
+    assert_close(out, None, expected(q, [slots], [(k, v, None, None)]))
+    items = int(workspace[:4].view(torch.int32))          # the plan's first counter: units of work for every key head
+    sms = torch.cuda.get_device_properties(device).multi_processor_count
+    assert 8 <= items and items * kv_heads <= sms         # 64 entries fit a wave, cut as far as that allows
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 2, 128), (14, 2, 64), (96, 1, 128)])
+def test_a_replayed_step_changes_between_single_tokens_and_chunks(device, heads, kv_heads, dim):
+    """One graph of a step with 64 slots and 64 rows: single tokens, one long request, both, some rows unused."""
+
+    slots = 64
+    q, k, v = make(device, [slots], [6000], heads, kv_heads, dim, torch.bfloat16, seed=16)
+    cu_q, cu_k = sums([1] * slots, device), sums([5] * slots, device)
+    attention.attention_varlen(q, (k, v), cu_q, cu_k)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held, lse = attention.attention_varlen(q, (k, v), cu_q, cu_k, return_lse=True)
+    for q_lens, k_lens in (([1] * 64, [90] * 64), ([0] * 30 + [64] + [0] * 33, [7] * 30 + [5000] + [3] * 33),
+                           ([1] * 20 + [40] + [0] * 43, [150] * 20 + [900] + [1] * 43), ([2, 0, 3, 1] * 10 + [0] * 24, [60] * 64)):
+        cu_q.copy_(sums(q_lens, device))
+        cu_k.copy_(sums(k_lens, device))
+        graph.replay()
+        rows = sum(q_lens)
+        assert_close(held, lse, expected(q[:rows], q_lens, split(k[:sum(k_lens)], v[:sum(k_lens)], k_lens)))
+        assert bool((held[rows:] == 0).all()) and bool((lse[rows:] == -math.inf).all())
+    attention.check_status(device)

@@ -732,3 +732,71 @@ def test_a_replayed_step_changes_between_single_tokens_and_chunks(device, heads,
         assert_close(held, lse, expected(q[:rows], q_lens, split(k[:sum(k_lens)], v[:sum(k_lens)], k_lens)))
         assert bool((held[rows:] == 0).all()) and bool((lse[rows:] == -math.inf).all())
     attention.check_status(device)
+
+
+def planned_rows(q_lens, k_lens, prefix, heads, kv_heads, sms, causal=True):
+    """Partial rows and items of a plan, in plain arithmetic: entries, chunk length, slots (as ``csrc/itk_attention.cuh`` plans)."""
+
+    group = heads // kv_heads
+    tile_tokens = 128 // group
+    span = 2 * tile_tokens
+    entries = []                                              # tokens, key tiles, of the prefix
+    if prefix:
+        total_q = sum(q_lens)
+        entries += [(min(span, total_q - at), -(-prefix // 128), True) for at in range(0, total_q, span)]
+    for count, keys in zip(q_lens, k_lens):
+        for at in range(0, count, span):
+            tokens = min(span, count - at)
+            seen = max(0, min(keys, keys - count + at + tokens)) if causal else keys
+            entries.append((tokens, -(-seen // 128), False))
+    units = [4 if tokens > tile_tokens else 3 for tokens, _, _ in entries]
+    share = min(math.ceil(sum(t * u for (_, t, _), u in zip(entries, units)) * kv_heads / sms) + 1, 1 << 29)
+
+    def chunks(tiles, unit, cost, whole):
+        if whole and tiles * unit <= whole:
+            return min(tiles, 1)
+        return -(-tiles // max(2, -(-cost // unit)))
+
+    cost, whole = min(share, max(share // 6, 24 * 4)), share // 2
+    for eighth in range(8):
+        length = share + share // 8 * eighth
+        if sum(max(1, chunks(t, u, length, 0)) for (_, t, _), u in zip(entries, units)) * kv_heads <= sms:
+            cost, whole = length, 0
+            break
+    rows = items = 0
+    for (tokens, tiles, _), unit in zip(entries, units):
+        cut = chunks(tiles, unit, cost, whole)
+        slots = cut * (2 if unit == 3 and cut and -(-tiles // cut) > 1 else 1)
+        items += max(1, cut)
+        if prefix or slots > 1:
+            rows += slots * tokens * group * kv_heads
+    return rows, items
+
+
+def test_the_workspace_holds_every_plan():
+    """Against plans of random batches, of one long request among short ones, and of many equal ones."""
+
+    build()
+    import random
+
+    library, rng, fullest = _lib.load_library(), random.Random(17), 0.0
+    for case in range(600):
+        kv_heads = rng.choice([1, 2, 3, 8, 16])
+        heads, dim, sms = kv_heads * rng.choice([1, 2, 5, 7, 8, 16, 96]), rng.choice([64, 128]), rng.choice([132, 148, 160])
+        requests = int(100 ** rng.random())
+        q_lens = [int(10 ** rng.uniform(0, 3.3)) - 1 if rng.random() < 0.5 else 1 for _ in range(requests)]
+        k_lens = [int(10 ** rng.uniform(0, rng.choice([2, 4, 5.5]))) for _ in range(requests)]
+        if case % 3 == 0:                                     # one entry has nearly all of the work
+            q_lens, k_lens = [1] * requests, [1] * requests
+            q_lens[0], k_lens[0] = min(2 * (128 // (heads // kv_heads)), 1 + rng.randrange(300)), 1 << rng.randint(10, 20)
+        prefix = rng.choice([0, 0, 100, 5000, 200000])
+        args = _lib.AttentionArgs()
+        args.tokens, args.requests, args.heads, args.kv_heads, args.dim, args.prefix_keys = (
+            max(1, sum(q_lens)), requests, heads, kv_heads, dim, prefix)
+        needed = ctypes.c_size_t(0)
+        assert library.itk_attention_workspace_bytes(ctypes.byref(args), ctypes.byref(needed)) == 0
+        rows, items = planned_rows(q_lens, k_lens, prefix, heads, kv_heads, sms, causal=rng.random() < 0.5)
+        used = rows * 4 * (dim + 1) + 48 * items
+        assert used <= needed.value, (case, used, needed.value)
+        fullest = max(fullest, used / needed.value)
+    assert 0.5 < fullest          # and it is no more than twice what some plan needs

@@ -142,7 +142,8 @@ __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddep
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Waits for the phase with the given parity, `polls` probes at most; each may be parked until the phase completes or the
-// hint runs out.  (The bound is a count, not a time: a deadline costs registers that the softmax loop does not have.)
+// hardware's own limit runs out, 4.1 us (with hints of 1 and 20 us alike).  (The bound is a count, not a time: a deadline costs
+// registers that the softmax loop does not have.)
 __device__ __forceinline__ bool attn_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint32_t polls) {
     for (uint32_t n = 0; n < polls; ++n) {
         if (mbar_try_wait(bar, parity)) return true;

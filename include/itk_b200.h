@@ -437,7 +437,8 @@ typedef struct itk_attention_args {
     const void* v_prefix;
     const int32_t* prefix_table; /* int32 [table_pages], or null: packed */
     long long q_token_stride, q_head_stride, out_token_stride, out_head_stride;
-    unsigned long long wait_limit_ns;   /* 0 = default (2 s); counted in probes, a thousand nanoseconds each at least nominally */
+    unsigned long long wait_limit_ns;   /* 0 = default (2 s).  Counted in probes, one per 1000 ns, of up to 4.1 us each: a wait
+                                         * in which nothing arrives gives up after about four times the limit */
     itk_kv_segment own;
     itk_kv_segment prefix;
     float scale;

@@ -30,6 +30,7 @@ MAX_CTAS = 256
 STATIC_MAX_ROWS = 256
 STATUS_WAIT_EXPIRED = 1
 MAX_PLAN_REQUESTS = 16384
+MAX_ATTENTION_KEYS = (1 << 31) - 1024
 ELEMENT_BF16 = 0
 ELEMENT_FP16 = 1
 SERVING_STATUS = {
@@ -299,7 +300,7 @@ def pointer_table(tensors: list[Any]) -> Any:
 
 __all__ = [
     "AppendArgs", "AttentionArgs", "BLOCK_Q", "ELEMENT_BF16", "ELEMENT_FP16", "EXPORTED_SYMBOLS", "FusedArgs", "HEADS",
-    "HEAD_DIM", "ItkError", "KvSegment", "LIBRARY_PATH", "MAX_KEYS", "MAX_PAIR_SOURCES", "MAX_PLAN_REQUESTS", "PagePlanArgs",
+    "HEAD_DIM", "ItkError", "KvSegment", "LIBRARY_PATH", "MAX_ATTENTION_KEYS", "MAX_KEYS", "MAX_PAIR_SOURCES", "MAX_PLAN_REQUESTS", "PagePlanArgs",
     "SERVING_STATUS", "REPAIR_CHUNK", "SPILL_U64_PER_ROW", "STATUS_WAIT_EXPIRED", "TOP_K", "WorkspaceSizes",
     "check", "check_serving_status", "current_stream", "load_library", "pointer_table", "ptr", "resource_report", "version",
     "workspace_sizes", "c_int32", "c_uint64",

@@ -52,7 +52,7 @@ def _check_kv(q: Any, k: Any, v: Any, what: str, rank: int) -> None:
              f"the query heads must be a multiple of the {what} key heads, at most 128 times as many")
     _require(k.numel() == 0 or (_rows_ok(k) and _rows_ok(v)),
              f"{what} keys and values must be contiguous in their last dimension and 16-byte aligned in every row")
-    _require(rank == 4 or k.shape[0] < 1 << 31, f"need less than 2^31 {what} keys")
+    _require(rank == 4 or k.shape[0] <= _lib.MAX_ATTENTION_KEYS, f"need less than 2^31 {what} keys, at most {_lib.MAX_ATTENTION_KEYS}")
     if rank == 4:
         pages, page_size = k.shape[:2]
         _require(pages > 0 and page_size > 0 and page_size % TILE_KEYS == 0, "page_size must be a positive multiple of 128")
@@ -107,6 +107,7 @@ def _check_call(torch: Any, q: Any, own: tuple, prefix: tuple | None, prefix_key
         if paged:
             _check_ints(torch, prefix[2], "prefix_table", device, None)
             _require(0 <= prefix_keys <= prefix[2].shape[0] * own[0].shape[1], "prefix_table does not cover the prefix keys")
+            _require(prefix_keys <= _lib.MAX_ATTENTION_KEYS, f"need at most {_lib.MAX_ATTENTION_KEYS} prefix keys")
     if out is not None:
         _require(out.shape == q.shape and out.dtype == q.dtype and out.device == device and (out.numel() == 0 or _rows_ok(out)),
                  "out must have the shape, type and device of q and 16-byte aligned rows")

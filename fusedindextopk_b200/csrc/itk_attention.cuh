@@ -366,7 +366,7 @@ __device__ __forceinline__ AttnRequest attn_request(const itk_attention_args& p,
         const int n = p.lens_k[b];
         const long long room = static_cast<long long>(p.own.table_pages) * p.own.page_size;
         r.k_first = 0;
-        r.k_count = static_cast<int>(min(static_cast<long long>(max(n, 0)), room));
+        r.k_count = static_cast<int>(min(static_cast<long long>(min(max(n, 0), ITK_MAX_ATTENTION_KEYS)), room));
         bad |= n != r.k_count;
     }
     return r;

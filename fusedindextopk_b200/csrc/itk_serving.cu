@@ -92,6 +92,7 @@ int check_segment(const itk_kv_segment& s, const void* k, const void* v, const i
         ITK_REQUIRE(s.table_pages >= 0 && s.table_stride >= 0, "%s: table sizes must not be negative", what);
     } else {
         ITK_REQUIRE(s.pages == 1, "%s: keys without a table are one page", what);
+        ITK_REQUIRE(s.page_size <= ITK_MAX_ATTENTION_KEYS, "%s: need at most %d keys", what, ITK_MAX_ATTENTION_KEYS);
     }
     return ITK_OK;
 }
@@ -336,6 +337,7 @@ int itk_attention(const itk_attention_args* args, itk_stream_t stream) {
         if ((rc = check_segment(a.prefix, a.k_prefix, a.v_prefix, a.prefix_table, "prefix keys")) != ITK_OK) return rc;
         const long long room = a.prefix_table != nullptr ? static_cast<long long>(a.prefix.table_pages) * a.prefix.page_size : a.prefix.page_size;
         ITK_REQUIRE(a.prefix_keys <= room, "prefix_keys exceeds the prefix");
+        ITK_REQUIRE(a.prefix_keys <= ITK_MAX_ATTENTION_KEYS, "need at most %d prefix keys", ITK_MAX_ATTENTION_KEYS);
     } else {
         ITK_REQUIRE(a.prefix_keys == 0, "prefix keys: keys and values must not be null");
     }

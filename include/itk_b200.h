@@ -381,6 +381,8 @@ typedef struct itk_page_plan_args {
 int itk_plan_pages(const itk_page_plan_args* args, itk_stream_t stream);
 
 #define ITK_MAX_PLAN_REQUESTS 16384
+/* keys of a request, of a prefix and of a packed batch at most: key tiles and rows a tile behind them are counted in 31 bits */
+#define ITK_MAX_ATTENTION_KEYS 2147482624
 #define ITK_ELEMENT_BF16 0
 #define ITK_ELEMENT_FP16 1
 

@@ -800,3 +800,45 @@ def test_the_workspace_holds_every_plan():
         assert used <= needed.value, (case, used, needed.value)
         fullest = max(fullest, used / needed.value)
     assert 0.5 < fullest          # and it is no more than twice what some plan needs
+
+
+def test_key_counts_whose_tiles_do_not_fit_31_bits_are_refused():
+    build()
+    library, args = _lib.load_library(), _lib.AttentionArgs()
+    args.tokens, args.requests, args.heads, args.kv_heads, args.dim, args.scale = 1, 1, 1, 1, 64, 1.0
+    args.q = args.out = args.cu_q = args.cu_k = args.k = args.v = 1 << 20
+    args.own.pages = 1
+    args.own.k_row_stride = args.own.k_head_stride = args.own.v_row_stride = args.own.v_head_stride = 64
+    for keys in (_lib.MAX_ATTENTION_KEYS + 1, (1 << 31) - 1):
+        args.own.page_size = keys
+        assert library.itk_attention(ctypes.byref(args), None) == -1
+        assert b"own keys: need at most 2147482624 keys" in library.itk_last_error()
+    args.own.page_size = 1000
+    args.k_prefix = args.v_prefix = args.prefix_table = 1 << 20
+    args.prefix.pages, args.prefix.page_size, args.prefix.table_pages = 1, 128, 1 << 24
+    for keys in (_lib.MAX_ATTENTION_KEYS + 1, (1 << 31) - 1):
+        args.prefix_keys = keys
+        assert library.itk_attention(ctypes.byref(args), None) == -1
+        assert b"at most 2147482624 prefix keys" in library.itk_last_error()
+
+
+@pytest.mark.gpu
+def test_the_most_keys_a_request_may_have(device):
+    """A table that names one page over and over; more keys than are allowed are clamped and reported."""
+
+    page, columns, dim = 1024, 1 << 21, 64
+    q, k, v = make(device, [1], [page], 1, 1, dim, torch.bfloat16, seed=18)
+    pools = tuple(x.view(1, page, 1, dim) for x in (k, v))
+    table = torch.zeros((1, columns), dtype=torch.int32, device=device)
+    cu_q = sums([1], device)
+    once = expected(q, [1], [(k, v, None, None)])[1].item()
+    for keys in (_lib.MAX_ATTENTION_KEYS, (1 << 31) - 1):
+        lens = torch.tensor([keys], dtype=torch.int32, device=device)
+        got, lse = attention.attention_paged(q, pools, table, cu_q, lens, return_lse=True)
+        if keys > _lib.MAX_ATTENTION_KEYS:
+            with pytest.raises(_lib.ItkError, match="lengths"):
+                attention.check_status(device)
+        attention.check_status(device)
+        assert bool(got.isfinite().all())
+        # sums of 32 weights are added one after another by every thread: of n / 32 / 2 lanes / 148 CTAs, e each
+        assert abs(lse.item() - once - math.log(_lib.MAX_ATTENTION_KEYS / page)) <= 2 * (1 << 31) / 32 / 2 / 148 * E + 1e-3

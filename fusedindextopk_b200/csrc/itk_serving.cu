@@ -298,8 +298,8 @@ int itk_append_tokens(const itk_append_args* args, itk_stream_t stream) {
     DeviceState device;
     const int rc = current_device(&device);
     if (rc != ITK_OK) return rc;
-    constexpr int kTokensPerBlock = kAppendThreads / 32;
-    const unsigned grid = static_cast<unsigned>((a.tokens + kTokensPerBlock - 1) / kTokensPerBlock);
+    constexpr unsigned kTokensPerBlock = kAppendThreads / 32;
+    const unsigned grid = (static_cast<unsigned>(a.tokens) + kTokensPerBlock - 1) / kTokensPerBlock;
     if (a.index_source != nullptr && a.index_dtype == ITK_SOURCE_BF16)
         itk_append_tokens_kernel<__nv_bfloat16><<<grid, kAppendThreads, 0, stream>>>(a, device.status);
     else

@@ -355,3 +355,16 @@ def test_copied_and_replaced_plans_fill_their_own_buffers(device):
     with pytest.raises(ValueError, match="k_end"):
         paged.plan_pages(plan, table, old, gpu([1, 0, 2], device), free)
     paged.check_serving_status(device)
+
+
+@pytest.mark.gpu
+def test_as_many_tokens_as_an_append_takes(device):
+    tokens = (1 << 31) - 1
+    k = torch.randn((1, 1, 64), dtype=torch.bfloat16, device=device)
+    pools = [torch.zeros((1, 128, 1, 64), dtype=torch.bfloat16, device=device) for _ in range(2)]
+    slots = torch.full((tokens,), -1, dtype=torch.int64, device=device)
+    slots[-1], slots[0] = 7, 9
+    paged.append_tokens(slots, (k.expand(tokens, 1, 64), k.expand(tokens, 1, 64)), tuple(pools))
+    for pool in pools:
+        assert torch.equal(pool[0, 7], k[0]) and torch.equal(pool[0, 9], k[0]) and int((pool != 0).any(-1).sum()) == 2
+    paged.check_serving_status(device)

@@ -14,6 +14,10 @@ using namespace itk;
 // One status word per device context, part of the library image: every serving kernel reports into it, and no
 // caller has to carry a buffer for it.
 __device__ int g_serving_status;
+__device__ int g_serving_taken;
+
+// Reads the word, and clears it in the same step: a bit that another stream sets meanwhile is in this report or in the next.
+__global__ void itk_take_status_kernel(int clear) { g_serving_taken = clear ? atomicExch(&g_serving_status, 0) : atomicOr(&g_serving_status, 0); }
 
 constexpr int kMaxDevices = 64;
 
@@ -230,9 +234,12 @@ int itk_serving_status(int* status, int clear) {
     DeviceState device;
     const int rc = current_device(&device);
     if (rc != ITK_OK) return rc;
+    static std::mutex taking;                  // of the word in between
+    std::lock_guard<std::mutex> lock(taking);
     ITK_CUDA(cudaDeviceSynchronize());
-    ITK_CUDA(cudaMemcpy(status, device.status, sizeof(int), cudaMemcpyDeviceToHost));
-    if (clear) ITK_CUDA(cudaMemset(device.status, 0, sizeof(int)));
+    itk_take_status_kernel<<<1, 1>>>(clear);
+    ITK_CUDA(cudaGetLastError());
+    ITK_CUDA(cudaMemcpyFromSymbol(status, g_serving_taken, sizeof(int)));
     return ITK_OK;
 }
 

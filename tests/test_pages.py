@@ -368,3 +368,42 @@ def test_as_many_tokens_as_an_append_takes(device):
     for pool in pools:
         assert torch.equal(pool[0, 7], k[0]) and torch.equal(pool[0, 9], k[0]) and int((pool != 0).any(-1).sum()) == 2
     paged.check_serving_status(device)
+
+
+@pytest.mark.gpu
+def test_a_report_is_not_lost_while_another_one_is_read(device):
+    """Calls on another stream, of another thread, while this one reads and clears the status again and again."""
+
+    import random
+    import threading
+    import time
+
+    k = torch.ones((1, 1, 64), dtype=torch.bfloat16, device=device)
+    pools = tuple(torch.zeros((1, 128, 1, 64), dtype=torch.bfloat16, device=device) for _ in range(2))
+    slots = torch.full((1,), 500, dtype=torch.int64, device=device)            # behind the pool
+    paged.check_serving_status(device)
+    stream, rng = torch.cuda.Stream(device), random.Random(19)
+
+    def call(delay):
+        until = time.perf_counter() + delay
+        while time.perf_counter() < until:
+            pass
+        with torch.cuda.stream(stream):
+            paged.append_tokens(slots, (k, k), pools)
+
+    def reported():
+        try:
+            paged.check_serving_status(device)
+        except _lib.ItkError:
+            return True
+        return False
+
+    torch.cuda.synchronize()
+    for number in range(400):
+        thread = threading.Thread(target=call, args=(rng.random() * 2e-4,))
+        thread.start()
+        seen = False
+        while thread.is_alive():
+            seen |= reported()
+        thread.join()
+        assert reported() or seen, f"the report of call {number} was lost"

@@ -236,16 +236,13 @@ class CallTemplate:
     LIMIT = 1024
 
     def __init__(self, args: ctypes.Structure, **extra: Any) -> None:
-        self.block = ctypes.c_char * ctypes.sizeof(args)
         self.bytes = bytes(args)
         self.__dict__.update(extra)
 
-    def fill(self, words: Any) -> Any:
+    def fill(self, words: Any) -> bytes:
         """A copy of the block with the 64-bit words it begins with put in."""
 
-        block = self.block.from_buffer_copy(self.bytes)
-        _WORDS[len(words)].pack_into(block, 0, *words)
-        return block
+        return _WORDS[len(words)].pack(*words) + self.bytes[8 * len(words):]
 
     @classmethod
     def keep(cls, templates: dict, key: Any, template: "CallTemplate") -> "CallTemplate":
@@ -258,22 +255,36 @@ class CallTemplate:
 _WORDS = [struct.Struct("<%dQ" % n) for n in range(32)]
 
 
-def metadata(tensors: tuple) -> tuple:
+def metadata(torch: Any, tensors: tuple) -> tuple:
     # (the device by its number, which is quicker; what is not on a GPU has -1 and is refused, so it is never kept)
+    if torch.autograd.forward_ad._current_level >= 0 and any(
+            torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError("there is no forward-mode derivative: detach")
     return tuple([(t.shape, t.stride(), t.dtype, t.get_device()) for t in tensors])
 
 
-def launch(torch: Any, function: Any, block: Any, device: Any) -> None:
-    """Calls a C entry on the current stream of ``device``."""
+def refuse_gradients(torch: Any, *tensors: Any) -> None:
+    """Raise where a call would drop the gradients that its tensors ask for."""
+
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise ValueError("there is no backward pass: call it under torch.no_grad() or detach")
+
+
+def launch(torch: Any, function: Any, block: Any, device: Any, written: tuple = ()) -> None:
+    """Calls a C entry on the current stream of ``device``; ``written`` are the caller's tensors that it writes to."""
 
     index = device.index
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:
         status = function(block, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
             status = function(block, torch._C._cuda_getCurrentRawStream(index))
     if status:
         check(status)
+    if written:         # a graph that has saved one of them finds that it has changed
+        torch._C._increment_version(written)
 
 
 def check_serving_status(device: Any = None) -> None:

@@ -142,16 +142,13 @@ def _attend(q: Any, own: tuple, prefix: tuple | None, prefix_keys: int, cu_seqle
         tensors += (out,)
     if scale is not None:
         scale = float(scale)
-    if torch.is_grad_enabled():
-        learns = q.requires_grad or own[0].requires_grad or own[1].requires_grad
-        if prefix is not None:
-            learns = learns or prefix[0].requires_grad or prefix[1].requires_grad
-        _require(not learns, "there is no backward pass: call it under torch.no_grad() or detach")
-    key = (_lib.metadata(tensors), len(own), prefix is not None, prefix_keys, bool(causal), scale)
+    _lib.refuse_gradients(torch, *tensors)
+    key = (_lib.metadata(torch, tensors), len(own), prefix is not None, prefix_keys, bool(causal), scale)
     template = _TEMPLATES.get(key)
     if template is None:
         template = _lib.CallTemplate.keep(_TEMPLATES, key, _check_call(
             torch, q, own, prefix, prefix_keys, cu_seqlens_q, lengths, out, causal, scale))
+    written = () if out is None else (out,)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)      # (new_empty takes 0.8 us longer)
     lse = q.new_empty(q.shape[:2], dtype=torch.float32) if return_lse else None
@@ -170,7 +167,7 @@ def _attend(q: Any, own: tuple, prefix: tuple | None, prefix_keys: int, cu_seqle
             words += [k, v, prefix[2].data_ptr() if template.paged else 0]
             aligned |= k | v
         _require(aligned & 15 == 0, "q, out, keys and values must be 16-byte aligned")
-        _lib.launch(torch, _lib.load_library().itk_attention, template.fill(words), template.device)
+        _lib.launch(torch, _lib.load_library().itk_attention, template.fill(words), template.device, written)
     return (out, lse) if return_lse else out
 
 

@@ -241,7 +241,7 @@ def plan_pages(plan: PagePlan, block_table: Any, lengths: Any, new_tokens: Any, 
     import torch
 
     tensors = (block_table, lengths, new_tokens, free_pages)
-    key = _lib.metadata(tensors)
+    key = _lib.metadata(torch, tensors)
     template = plan.templates.get(key)
     if template is None:
         template = _lib.CallTemplate.keep(plan.templates, key, _check_plan(torch, plan, *tensors))
@@ -249,7 +249,8 @@ def plan_pages(plan: PagePlan, block_table: Any, lengths: Any, new_tokens: Any, 
         block_table.data_ptr(), lengths.data_ptr(), new_tokens.data_ptr(), free_pages.data_ptr(), plan.slots.data_ptr(),
         plan.cu_seqlens_q.data_ptr(), plan.lengths.data_ptr(), plan.flat_table.data_ptr(), plan.k_start.data_ptr(),
         plan.k_end.data_ptr(), plan.pages_needed.data_ptr()))
-    _lib.launch(torch, _lib.load_library().itk_plan_pages, block, template.device)
+    _lib.launch(torch, _lib.load_library().itk_plan_pages, block, template.device, (
+        block_table, plan.slots, plan.cu_seqlens_q, plan.lengths, plan.flat_table, plan.k_start, plan.k_end, plan.pages_needed))
     plan.__dict__["block_table"] = block_table
     return plan
 
@@ -300,7 +301,8 @@ def append_tokens(slots: Any, kv: tuple[Any, Any], pools: tuple[Any, Any], *, in
     if index_keys is not None or index_pools is not None:
         _require(index_keys is not None and index_pools is not None, "index_keys and index_pools go together")
         tensors += (index_keys, *index_pools)
-    key = _lib.metadata(tensors)
+    _lib.refuse_gradients(torch, *tensors)
+    key = _lib.metadata(torch, tensors)
     template = _APPEND_TEMPLATES.get(key)
     if template is None:
         template = _lib.CallTemplate.keep(_APPEND_TEMPLATES, key, _check_append(torch, *tensors))
@@ -309,7 +311,8 @@ def append_tokens(slots: Any, kv: tuple[Any, Any], pools: tuple[Any, Any], *, in
     for address in addresses[1:7]:
         aligned |= address
     _require(aligned & 15 == 0, "keys, values, index keys and their pools must be 16-byte aligned")
-    _lib.launch(torch, _lib.load_library().itk_append_tokens, template.fill(addresses), template.device)
+    _lib.launch(torch, _lib.load_library().itk_append_tokens, template.fill(addresses), template.device,
+                (k_pool, v_pool) if index_pools is None else (k_pool, v_pool, *index_pools))
 
 
 _APPEND_TEMPLATES: dict = {}

@@ -842,3 +842,32 @@ def test_the_most_keys_a_request_may_have(device):
         assert bool(got.isfinite().all())
         # sums of 32 weights are added one after another by every thread: of n / 32 / 2 lanes / 148 CTAs, e each
         assert abs(lse.item() - once - math.log(_lib.MAX_ATTENTION_KEYS / page)) <= 2 * (1 << 31) / 32 / 2 / 148 * E + 1e-3
+
+
+def test_attention_drops_no_gradient_and_no_tangent(monkeypatch):
+    monkeypatch.setattr(_lib, "launch", lambda *_: pytest.fail("a launch"))
+    q, k, v, kp, vp = (torch.ones(4, 2, 64) for _ in range(5))
+    ends, out = torch.zeros(2, dtype=torch.int32), torch.ones(4, 2, 64)
+    forward = torch.autograd.forward_ad
+
+    def call(tensors, out=None):
+        attention.shared_prefix_attention(tensors[0], tensors[3:], tensors[1:3], ends, ends, out=out)
+
+    plain = [q, k, v, kp, vp]
+    for i in range(5):
+        with pytest.raises(ValueError, match="no backward"):
+            call(plain[:i] + [plain[i].clone().requires_grad_()] + plain[i + 1:])
+        with forward.dual_level(), torch.no_grad(), pytest.raises(ValueError, match="no forward-mode"):
+            call(plain[:i] + [forward.make_dual(plain[i], torch.ones(4, 2, 64))] + plain[i + 1:])
+    with pytest.raises(ValueError, match="no backward"):
+        call(plain, out=out.clone().requires_grad_())
+    with forward.dual_level(), pytest.raises(ValueError, match="CUDA"):         # a level without tangents changes nothing
+        call(plain, out=out)
+
+
+@pytest.mark.gpu
+def test_a_given_output_counts_as_changed(device):
+    q, k, v = make(device, [4], [30], 4, 2, 128, torch.bfloat16)
+    out = torch.zeros_like(q)
+    attention.attention_varlen(q, (k, v), sums([4], device), sums([30], device), out=out)
+    assert (out._version, q._version, k._version) == (1, 0, 0)

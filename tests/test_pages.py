@@ -323,7 +323,7 @@ def test_no_address_is_kept_between_plans(monkeypatch):
     """The block of a call holds the addresses of the plan it was made for, also of one copied after a call."""
 
     seen = []
-    monkeypatch.setattr(_lib, "launch", lambda torch, function, block, device: seen.append(_lib.PagePlanArgs.from_buffer_copy(block)))
+    monkeypatch.setattr(_lib, "launch", lambda torch, function, block, *rest: seen.append(_lib.PagePlanArgs.from_buffer_copy(block)))
     sizes = _lib.PagePlanArgs(*[None] * 11, 3, 2, 3, 128, 4, 5)
     monkeypatch.setattr(paged, "_check_plan", lambda torch, plan, *tensors: _lib.CallTemplate(sizes, device=None))
     table, ints = torch.zeros((2, 3), dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
@@ -407,3 +407,66 @@ def test_a_report_is_not_lost_while_another_one_is_read(device):
             seen |= reported()
         thread.join()
         assert reported() or seen, f"the report of call {number} was lost"
+
+
+def cpu_append(**changes):
+    """Arguments of an append whose checks and launch are left out."""
+
+    given = dict(slots=torch.arange(3), k=torch.ones(3, 2, 64), v=torch.ones(3, 2, 64), k_pool=torch.zeros(2, 128, 2, 64),
+                 v_pool=torch.zeros(2, 128, 2, 64), index_keys=torch.ones(3, 128), index_pool=torch.zeros(2, 128, 128),
+                 index_scales=torch.zeros(2, 128)) | changes
+    return ((given["slots"], (given["k"], given["v"]), (given["k_pool"], given["v_pool"])),
+            dict(index_keys=given["index_keys"], index_pools=(given["index_pool"], given["index_scales"])), given)
+
+
+@pytest.mark.parametrize("name", ["k", "v", "k_pool", "v_pool", "index_keys", "index_pool", "index_scales"])
+def test_an_append_drops_no_gradient_and_no_tangent(monkeypatch, name):
+    monkeypatch.setattr(_lib, "launch", lambda *_: pytest.fail("a launch"))
+    plain = cpu_append()[2][name]
+    args, kwargs, _ = cpu_append(**{name: plain.clone().requires_grad_()})
+    with pytest.raises(ValueError, match="no backward"):
+        paged.append_tokens(*args, **kwargs)
+    forward = torch.autograd.forward_ad
+    with forward.dual_level(), torch.no_grad():
+        args, kwargs, _ = cpu_append(**{name: forward.make_dual(plain, torch.ones_like(plain))})
+        with pytest.raises(ValueError, match="no forward-mode"):
+            paged.append_tokens(*args, **kwargs)
+
+
+def test_what_the_calls_write_counts_as_changed(monkeypatch):
+    """Autograd refuses to use a saved tensor that was written meanwhile: that takes its version."""
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 0, raising=False)
+    monkeypatch.setattr(_lib, "load_library", lambda: type("Library", (), {
+        "itk_append_tokens": staticmethod(lambda block, stream: 0), "itk_plan_pages": staticmethod(lambda block, stream: 0)}))
+    template = _lib.CallTemplate(_lib.AppendArgs(), device=torch.device("cuda", 0))
+    monkeypatch.setattr(paged, "_check_append", lambda *_: template)
+    monkeypatch.setattr(paged, "_APPEND_TEMPLATES", {})
+    args, kwargs, given = cpu_append()
+    monkeypatch.setattr(paged, "_require", lambda condition, message: None)         # (the alignment of CPU tensors)
+    paged.append_tokens(*args, **kwargs)
+    assert {name: t._version for name, t in given.items()} == dict(
+        slots=0, k=0, v=0, k_pool=1, v_pool=1, index_keys=0, index_pool=1, index_scales=1)
+    saved = torch.ones(2, 128, 2, 64, requires_grad=True)
+    product = saved * given["k_pool"]
+    paged.append_tokens(*args, **kwargs)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.sum().backward()
+    plan = cpu_plan()
+    monkeypatch.setattr(paged, "_check_plan", lambda *_: _lib.CallTemplate(_lib.PagePlanArgs(), device=torch.device("cuda", 0)))
+    table, ints = torch.zeros((2, 3), dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    paged.plan_pages(plan, table, ints, ints, ints)
+    assert ints._version == 0 and table._version == plan.slots._version == plan.lengths._version == plan.k_end._version == 1
+
+
+@pytest.mark.gpu
+def test_an_append_raises_the_versions_of_its_pools(device):
+    k = torch.ones((3, 2, 64), dtype=torch.bfloat16, device=device)
+    pools = tuple(torch.zeros((2, 128, 2, 64), dtype=torch.bfloat16, device=device) for _ in range(2))
+    paged.append_tokens(torch.arange(3, device=device), (k, k), pools)
+    assert [t._version for t in (k, *pools)] == [0, 1, 1]
+    with torch.inference_mode():
+        held = tuple(p.clone() for p in pools)
+    paged.append_tokens(torch.arange(3, device=device), (k, k), held)           # inference tensors have no versions
+    paged.check_serving_status(device)

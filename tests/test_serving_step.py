@@ -139,3 +139,29 @@ def test_a_step_in_a_graph_follows_the_batch(device):
             used = int(cache.plan.pages_needed)
             cache.lengths.copy_(cache.plan.lengths)
             cache.free.copy_(torch.cat([cache.free[used:], cache.free[:used]]))
+
+
+@pytest.mark.gpu
+def test_the_whole_step_in_a_graph_follows_the_batch(device):
+    """Plan, append, quantisation, selection and attention captured once, replayed for steps of other lengths."""
+
+    eager, captured = Cache(device), Cache(device)
+    tokens = projections(device, 6)
+    new_tokens = torch.zeros(REQUESTS, dtype=torch.int32, device=device)
+    step(captured, new_tokens, tokens)                      # workspaces and buffers are made outside of the graph
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held_ids, held = step(captured, new_tokens, tokens)
+    for counts in ([2300, 0, 129], [1, 1, 1], [0, 700, 1], [1, 1, 1]):
+        new_tokens.copy_(torch.tensor(counts, dtype=torch.int32))
+        graph.replay()
+        ids, out = held_ids.clone(), held.clone()
+        want_ids, want = (x.clone() for x in step(eager, new_tokens, tokens))
+        paged.check_serving_status(device)
+        assert torch.equal(ids.sort(dim=-1).values, want_ids.sort(dim=-1).values) and torch.equal(out, want)
+        assert bool((ids[:sum(counts), 0] >= 0).all())
+        for cache in (eager, captured):
+            used = int(cache.plan.pages_needed)
+            cache.lengths.copy_(cache.plan.lengths)
+            cache.free.copy_(torch.cat([cache.free[used:], cache.free[:used]]))

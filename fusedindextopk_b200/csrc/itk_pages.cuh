@@ -202,7 +202,10 @@ __global__ void __launch_bounds__(kPlanThreads) itk_plan_pages_kernel(const itk_
             page = *entry;
         } else {
             const int next = taken[b] + column - r.before;
-            if (column < r.after && next < p.free_count) page = p.free_pages[next];
+            if (column < r.after && next < p.free_count) {
+                page = p.free_pages[next];
+                if (page < 0) atomicOr(status, ITK_SERVING_OUT_OF_PAGES);      // a free list padded to a fixed length
+            }
             *entry = page;
         }
         if (column < r.after) p.flat[first[b] + column] = page;

@@ -234,8 +234,9 @@ def plan_pages(plan: PagePlan, block_table: Any, lengths: Any, new_tokens: Any, 
     inputs must not share memory with those: ``plan.lengths`` serves as another plan's ``lengths`` (two plans in turn), not
     as its own's.
 
-    A request that outgrows its table row, a free list that is too short and more new tokens than ``rows`` are reported
-    by ``check_serving_status``; their tokens get slot -1 (or no row), their cells -1, and nothing is written out of range.
+    A request that outgrows its table row, a free list that is too short (negative entries are no pages: padding) and more
+    new tokens than ``rows`` are reported by ``check_serving_status``; their tokens get slot -1 (or no row), their cells -1, and
+    nothing is written out of range.  A cell that an earlier plan left without a page is not reported again.
     """
 
     import torch

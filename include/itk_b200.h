@@ -367,7 +367,7 @@ typedef struct itk_page_plan_args {
     int32_t* table;            /* int32 [requests, table_pages], row stride table_stride; updated in place */
     const int32_t* old;        /* int32 [requests] */
     const int32_t* fresh;      /* int32 [requests] */
-    const int32_t* free_pages; /* int32 [free_count] */
+    const int32_t* free_pages; /* int32 [free_count]; a negative one is none: padding of a list of fixed length */
     long long* slots;          /* int64 [rows] */
     int32_t* cu_q;             /* int32 [requests + 1] */
     int32_t* lengths;          /* int32 [requests] */

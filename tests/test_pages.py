@@ -470,3 +470,17 @@ def test_an_append_raises_the_versions_of_its_pools(device):
         held = tuple(p.clone() for p in pools)
     paged.append_tokens(torch.arange(3, device=device), (k, k), held)           # inference tensors have no versions
     paged.check_serving_status(device)
+
+
+@pytest.mark.gpu
+def test_padding_of_the_free_list_counts_as_no_page(device):
+    plan = paged.make_page_plan(3, 2, 300, page_size=128, device=device)
+    table = torch.full((3, 2), -1, dtype=torch.int32, device=device)
+    old, padded = gpu([0, 0, 0], device), gpu([4, 9, -1, -1], device)
+    paged.plan_pages(plan, table, old, gpu([100, 100, 0], device), padded)
+    paged.check_serving_status(device)                                        # the padding is not needed
+    got = paged.plan_pages(plan, table, old, gpu([100, 130, 0], device), padded)
+    assert table.tolist() == [[4, -1], [9, -1], [-1, -1]] and got.pages_needed.tolist() == [3]
+    assert bool((got.slots[:228] >= 0).all()) and bool((got.slots[228:] == -1).all())
+    with pytest.raises(_lib.ItkError, match="out of pages"):
+        paged.check_serving_status(device)

@@ -270,6 +270,9 @@ int itk_plan_pages(const itk_page_plan_args* args, itk_stream_t stream) {
         for (const Bytes& written : writes)
             for (const Bytes& read : reads)
                 ITK_REQUIRE(!overlap(written, read), "the request lengths and the free list must not share memory with the table or the plan");
+        for (const Bytes& written : writes)
+            for (const Bytes* other = writes; other != &written; ++other)
+                ITK_REQUIRE(!overlap(written, *other), "the table and the plan's buffers must not share memory with one another");
     }
     DeviceState device;
     const int rc = current_device(&device);

@@ -484,3 +484,19 @@ def test_padding_of_the_free_list_counts_as_no_page(device):
     assert bool((got.slots[:228] >= 0).all()) and bool((got.slots[228:] == -1).all())
     with pytest.raises(_lib.ItkError, match="out of pages"):
         paged.check_serving_status(device)
+
+
+def test_buffers_that_share_memory_are_refused():
+    build()
+    library, plan = _lib.load_library(), _lib.PagePlanArgs()
+    plan.requests, plan.table_pages, plan.page_size, plan.table_stride, plan.free_count, plan.rows = 4, 6, 128, 8, 5, 10
+    names = ("table", "slots", "cu_q", "lengths", "flat", "k_start", "k_end", "pages_needed")
+    for first in names:
+        for second in names:
+            if first == second:
+                continue
+            for i, name in enumerate(("old", "fresh", "free_pages", *names)):
+                setattr(plan, name, (i + 1) << 20)
+            setattr(plan, first, getattr(plan, second))        # a table that is the plan's flat one, for example
+            assert library.itk_plan_pages(ctypes.byref(plan), None) == -1
+            assert b"share memory with one another" in library.itk_last_error()

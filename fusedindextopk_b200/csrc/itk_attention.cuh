@@ -104,9 +104,9 @@ struct AttnCombine {
 };
 
 struct AttnCounters {
-    int items, combines, partial_rows, rows_end;
+    int items, combines;
+    int rows_end, rows_begin; // behind the rows of the last request, at those of the first
     int next;                 // the first unit of work (item, key head) that no CTA has taken yet
-    int rows_begin;           // rows of the first request; rows_end: behind the last one
 };
 
 struct AttnWorkspace {
@@ -654,8 +654,8 @@ __global__ void __launch_bounds__(THREADS) itk_attention_plan_kernel(const __gri
             if (place + c < p.w.max_items) p.w.items[place + c] = attn_chunk(entry, c, count);
     }
     __syncthreads();
-    if (tx == 0) *p.w.counters = AttnCounters{min(item_count, p.w.max_items), min(combine_count, p.w.max_combines), partial_rows, rows_end, p.sm_count,
-                                               min(max(p.a.cu_q[0], 0), p.a.tokens)};
+    if (tx == 0) *p.w.counters = AttnCounters{min(item_count, p.w.max_items), min(combine_count, p.w.max_combines), rows_end,
+                                               min(max(p.a.cu_q[0], 0), p.a.tokens), p.sm_count};
 }
 
 // The plan of a call with at most 32 requests and 32 entries that fit one wave of CTAs uncut: every CTA's producer warp
@@ -720,7 +720,7 @@ __device__ __forceinline__ bool attn_small_plan(const AttnParams& p, AttnRequest
         for (int r = 0; r < wanted; ++r)
             if (at + r < p.w.max_combines)
                 p.w.combines[at + r] = AttnCombine{entry.item.q_first, entry.item.tokens, entry.item.partial, usable, r * kAttnCombineRows, {}};
-        if (lane == 0) *p.w.counters = AttnCounters{items, min(records, p.w.max_combines), partial, rows_end, 0, min(max(p.a.cu_q[0], 0), p.a.tokens)};
+        if (lane == 0) *p.w.counters = AttnCounters{items, min(records, p.w.max_combines), rows_end, min(max(p.a.cu_q[0], 0), p.a.tokens), 0};
     }
     __syncwarp();
     return __any_sync(0xffffffffu, found) != 0;

@@ -121,24 +121,24 @@ constexpr int kAttnMaxSms = 160;     // the workspace is sized for any device th
 // SM's share of the work (less a hundredth: the share is rounded up, its part down), so that chunking adds at most
 // kAttnWaves items per SM over all key heads.
 // Partial rows.  Entries of up to TT tokens, at most one per request and 128 rows per key head each, have two lanes.  Without a
-// prefix longer ones have partial results only when they are cut, which takes an added chunk each; with one every own
-// row and every prefix row has a result, the last prefix entry two.  An added chunk has one result for each of up to 256 rows or
+// prefix longer ones have partial results only when they are cut, which takes half a share of work each, so that there are two
+// of them per SM at most; with one every own row and every prefix row has a result, the last prefix entry two.  An added chunk has one result for each of up to 256 rows or
 // two for each of up to 128, and no row has more of them than there are for one key head.
 //
-// 64 tokens of 64/8 heads of 128 ask for 135 MB, which is the added chunks' part of every larger call too (128 MB at dimension 128:
-// the lengths are not known here, and one long entry among short ones can take all of them); 8192 rows of 64 heads behind a
-// prefix ask for 670 MB, two results in fp32 per row.
+// 64 tokens of 64/8 heads of 128 ask for 135 MB, of which the added chunks' part, 128 MB at dimension 128, is the same for every larger
+// call (the lengths are not known here, and one long entry among short ones can take all of them); 4096 rows of one request ask
+// for 172 MB, 8192 rows of 64 heads behind a prefix for 674, two results in fp32 per row.
 int attention_workspace(const itk_attention_args& a, AttnWorkspace* w, size_t* bytes) {
     const long long span = 2 * attention_tile_tokens(a);
     const long long rows = static_cast<long long>(a.tokens) * a.heads;
     const long long own = a.tokens / span + a.requests, prefix = a.prefix_keys > 0 ? a.tokens / span + 1 : 0;
-    constexpr long long kAdded = kAttnMaxSms * kAttnWaves * 101ll / 100 + 1;
+    constexpr long long kAdded = kAttnMaxSms * kAttnWaves * 101ll / 100 + 1, kCut = kAttnMaxSms * 2 * 101ll / 100 + 1;
     const long long short_rows = std::min(rows, static_cast<long long>(a.requests) * kAttnTile * a.kv_heads);
     long long partial = std::min(kAdded * 2 * kAttnTile, 2 * rows * (kAdded / a.kv_heads));
     if (prefix > 0)
         partial += rows + short_rows + rows + static_cast<long long>(kAttnTile) * a.kv_heads;
     else
-        partial += 2 * short_rows + std::min(rows, kAdded * 2 * kAttnTile);
+        partial += 2 * short_rows + std::min(rows, kCut * 2 * kAttnTile);
     ITK_REQUIRE(partial < (1ll << 31) - 1 && own < kAttnMostEntries && (own + prefix + kAdded) * a.kv_heads < (1ll << 31),
                 "the batch is too large for one call");
     size_t at = 0;

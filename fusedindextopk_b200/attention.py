@@ -15,10 +15,18 @@ head ``h // (Hq // H)``.  The reference selects keys only and attends nowhere.
   whole batch shares, read once for all requests, in front of every request's own keys.
 
 All of them take bf16 or fp16 with head dimension 64 or 128, keep scores, softmax
-statistics and sums in fp32 and never read lengths back to the host, so a call can be
+statistics and sums in fp32, round the softmax weights to the element type once, for the
+product with the values, and never read lengths back to the host, so a call can be
 captured into a CUDA graph and replayed with other lengths in the same buffers.  A row
-that sees no key gets zeros and a log-sum-exp of ``-inf``.  There is no backward pass:
-the framework serves.
+that sees no key, or whose scores are all ``-inf``, gets zeros and a log-sum-exp of
+``-inf``.  There is no backward pass: the framework serves, and tensors that ask for
+gradients or carry forward-mode tangents are refused.
+
+A call takes its workspace from the caching allocator, and a captured graph keeps its
+own: 4 MB for a single token, up to 175 MB for the partial results of long entries that
+are cut (64 tokens of 64/8 heads: 135 MB), and about 1 KB per row and query head more
+with a prefix (8192 rows of 64 heads: 674 MB).  The first call with given shapes and types
+takes about 45 us of host time for its checks, later ones 18.
 """
 
 from __future__ import annotations

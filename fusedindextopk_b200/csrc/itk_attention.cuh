@@ -293,8 +293,9 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // 2^z on the FMA pipe, for some of the weights: the special-function unit gives 16 exponentials a cycle to an SM, which
 // is what the softmax is short of.  z = n + f with n the nearest whole number (adding 1.5 * 2^23 leaves it in the low bits),
 // 2^f by a polynomial of degree 5, fitted for the least relative error on [-1/2, 1/2] by iteratively reweighted least
-// squares (7.5e-8), 2^n by its exponent bits.  Below the normal range the result is 0, as exp2_fast's is; NaN stays NaN.
-// z <= 127 is all that is asked for (weights are at most 2^(kAttnLazy + kHeadroom)).
+// squares (7.5e-8 in exact arithmetic, 2.2e-7 as evaluated in fp32), 2^n by its exponent bits.  Below the normal range the
+// result is 0, as exp2_fast's is; NaN stays NaN.  z <= 127 is all that is asked for (weights are at most
+// 2^(kAttnLazy + kHeadroom)).
 __device__ __forceinline__ float2 exp2_polynomial(float2 z) {
     auto both = [](float x) { return make_float2(x, x); };
     const float2 shifted = add2(z, both(12582912.0f));
@@ -1431,8 +1432,8 @@ constexpr int kJoinThreads = 256;
 // per row, kFlight partial rows on their way at a time; also clears the rows of no request when asked to.
 //
 // Bound by the chain record - statistics - rows - store, about 3 us for one token over 8192 keys.  Small calls have fewer rows than
-// the device has warps and take the time of a trip per kFlight slots: 32 (the whole call 16.6 us, with 16 it took 17.6).  Large ones
-// have rows for all warps, and 32 cost occupancy (128 registers, 206 for 32; 64 rows over a prefix of 16384 keys 84.4 and 88.2 us).
+// the device has warps and take the time of a trip per kFlight slots: 32 (a call of 15.5 us took 1 us longer with 16).  Large ones
+// have rows for all warps, and 32 cost occupancy (128 registers, 197 for 32; 64 rows over a prefix of 16384 keys 84.4 and 88.2 us).
 template <typename T, int DIM, int kFlight>
 __global__ void __launch_bounds__(kJoinThreads) itk_attention_join_kernel(const __grid_constant__ AttnParams p) {
     constexpr int kOwn = DIM / 32;

@@ -237,6 +237,10 @@ def plan_pages(plan: PagePlan, block_table: Any, lengths: Any, new_tokens: Any, 
     A request that outgrows its table row, a free list that is too short (negative entries are no pages: padding) and more
     new tokens than ``rows`` are reported by ``check_serving_status``; their tokens get slot -1 (or no row), their cells -1, and
     nothing is written out of range.  A cell that an earlier plan left without a page is not reported again.
+
+    The key space of ``flat_table``, ``k_start`` and ``k_end`` has ``requests * table_pages * page_size`` keys;
+    ``fused_index_topk_paged`` takes 262144 of them at most.  A larger plan serves appends and attention; its keys cannot be
+    selected from in one call.
     """
 
     import torch
@@ -290,8 +294,9 @@ def append_tokens(slots: Any, kv: tuple[Any, Any], pools: tuple[Any, Any], *, in
     ``quantize.quantize_contiguous_index_kv`` does into ``index_pools = (kv_pool e4m3 [P, page_size, 128], scale_pool fp32
     [P, page_size])``, the pools ``fused_index_topk_paged`` reads.
 
-    Slots must differ from one another: of two tokens with the same slot either may be kept, in parts too.  A slot behind the
-    pool is skipped and reported by ``check_serving_status``.
+    Slots must differ from one another: of two tokens with the same slot either may be kept, in parts too.  The pools share no
+    memory with one another or with the tokens.  A slot behind the pool is skipped and reported by
+    ``check_serving_status``.  Tensors that ask for gradients or carry forward-mode tangents are refused.
     """
 
     import torch

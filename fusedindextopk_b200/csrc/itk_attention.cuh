@@ -28,8 +28,8 @@
 // steps of 64 keys.  TMEM: two buffers of 64 score columns per lane, so that the scores of step i + 1 are computed while
 // the softmax works on step i (the weights P overwrite the first half of their scores as 16-bit pairs and are the A
 // operand of P V from there), and O_A, O_B.  The row maximum is only moved when it grows by more than 2^8 (kAttnLazy):
-// until then weights are at most 2^8 (2^15 as fp16) and O needs no rescaling; when it does, the row's own softmax warp rescales O in TMEM
-// after the last P V issued so far.
+// until then weights are at most 2^8 (2^15 as fp16) and O needs no rescaling; when it does, the row's own softmax warp
+// rescales O in TMEM after the last P V issued so far.
 //
 // What bounds it (B200, 4736 x 8192 rows, 32 / 8 heads, bf16, no mask).  D = 128: 0.52 ms, 1220 TFLOP/s; the tensor unit is
 // busy 77 % of the time (61 % of it with products: the N = 64 score products read 1.5 times the shared memory that

@@ -122,8 +122,8 @@ constexpr int kAttnMaxSms = 160;     // the workspace is sized for any device th
 // kAttnWaves items per SM over all key heads.
 // Partial rows.  Entries of up to TT tokens, at most one per request and 128 rows per key head each, have two lanes.  Without a
 // prefix longer ones have partial results only when they are cut, which takes half a share of work each, so that there are two
-// of them per SM at most; with one every own row and every prefix row has a result, the last prefix entry two.  An added chunk has one result for each of up to 256 rows or
-// two for each of up to 128, and no row has more of them than there are for one key head.
+// of them per SM at most; with one every own row and every prefix row has a result, the last prefix entry two.  An added chunk has
+// one result for each of up to 256 rows or two for each of up to 128, and no row has more of them than there are for one key head.
 //
 // 64 tokens of 64/8 heads of 128 ask for 135 MB, of which the added chunks' part, 128 MB at dimension 128, is the same for every larger
 // call (the lengths are not known here, and one long entry among short ones can take all of them); 4096 rows of one request ask

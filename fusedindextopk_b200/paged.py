@@ -267,8 +267,9 @@ def _check_plan(torch: Any, plan: PagePlan, block_table: Any, lengths: Any, new_
                                ("lengths", requests, torch.int32), ("flat_table", requests * plan.table_pages, torch.int32),
                                ("k_start", rows, torch.int32), ("k_end", rows, torch.int32), ("pages_needed", 1, torch.int32)):
         buffer = getattr(plan, name)
-        _require(buffer.is_cuda and buffer.device == device and buffer.dtype == dtype and tuple(buffer.shape) == (count,)
-                 and buffer.is_contiguous(), f"the plan's {name} must be contiguous {dtype} [{count}] on one CUDA device")
+        _require(buffer.is_cuda and buffer.device == device and buffer.dtype == dtype and buffer.dim() == 1
+                 and buffer.shape[0] >= count and buffer.is_contiguous(),
+                 f"the plan's {name} must be contiguous {dtype} with {count} entries on one CUDA device")
     for name, tensor, count in (("lengths", lengths, requests), ("new_tokens", new_tokens, requests),
                                 ("free_pages", free_pages, None)):
         _require(tensor.dtype == torch.int32 and tensor.dim() == 1 and tensor.is_contiguous(), f"{name} must be contiguous int32")

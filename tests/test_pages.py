@@ -500,3 +500,13 @@ def test_buffers_that_share_memory_are_refused():
             setattr(plan, first, getattr(plan, second))        # a table that is the plan's flat one, for example
             assert library.itk_plan_pages(ctypes.byref(plan), None) == -1
             assert b"share memory with one another" in library.itk_last_error()
+
+
+@pytest.mark.gpu
+def test_a_plan_may_have_more_room_than_it_says(device):
+    plan = dataclasses.replace(paged.make_page_plan(3, 4, 20, page_size=128, device=device), rows=5)
+    table = torch.full((3, 4), -1, dtype=torch.int32, device=device)
+    plan.slots.fill_(77)
+    got = paged.plan_pages(plan, table, gpu([0, 0, 0], device), gpu([1, 2, 1], device), gpu([3, 1, 2], device))
+    assert got.slots.tolist() == [384, 128, 129, 256, -1] + [77] * 15
+    paged.check_serving_status(device)

@@ -32,9 +32,9 @@
 // rescales O in TMEM after the last P V issued so far.
 //
 // What bounds it (B200, 4736 x 8192 rows, 32 / 8 heads, bf16, no mask).  D = 128: 0.52 ms, 1220 TFLOP/s; the tensor unit is
-// busy 77 % of the time (61 % of it with products: the N = 64 score products read 1.5 times the shared memory that
+// busy 74 % of the time (58 % of it with products: the N = 64 score products read 1.5 times the shared memory that
 // their arithmetic takes time for); without the exponentials it takes 0.50 ms, with an eighth of the products
-// 0.43 ms.  D = 64: 0.43 ms, 735 TFLOP/s, bound by the softmax warps: 16 exponentials a cycle and SM alone take 0.26 ms.
+// 0.43 ms.  D = 64: 0.43 ms, 735 TFLOP/s, bound by the softmax warps: 16 exponentials a cycle and SM alone take 0.26 ms, 61 % of it.
 // Single tokens (split mode): 6.1 TB/s of keys and values, 0.94 of the measured copy rate, and 5.5 when the power cap (1000 W)
 // holds in a long run.  One token over 8192 keys, 15.5 us: small plan 2, first keys 2, keys 4 (at the rate of memory), epilogue and
 // end 2, the join 3 behind a gap of 1.
